@@ -69,8 +69,14 @@ typedef enum yuuka_dtype {
     YUUKA_DTYPE_BF16 = 30
 } yuuka_dtype;
 
-/* KV pool formats: model/qwen35/kv_format.go:16-24 */
-typedef enum yuuka_kv_format { YUUKA_KV_F32 = 0, YUUKA_KV_F16 = 1, YUUKA_KV_Q8_0 = 2 } yuuka_kv_format;
+/* KV pool formats: model/qwen35/kv_format.go:16-24. F8 is not in the reference and serves the kernel-level cache
+ * calls (yuuka_kv_write, yuuka_kv_read, yuuka_attention_decode) only; sessions refuse it. */
+typedef enum yuuka_kv_format {
+    YUUKA_KV_F32 = 0,
+    YUUKA_KV_F16 = 1,
+    YUUKA_KV_Q8_0 = 2,
+    YUUKA_KV_F8 = 3
+} yuuka_kv_format;
 
 /* yuuka_hip.h:49-53 */
 YUUKA_API uint32_t yuuka_abi_version(void);
@@ -88,12 +94,19 @@ YUUKA_API yuuka_status yuuka_device_memory_get(const yuuka_device * dev, uint64_
 
 YUUKA_API yuuka_status yuuka_buffer_alloc(yuuka_device * dev, uint64_t bytes, yuuka_buffer ** out);
 YUUKA_API void yuuka_buffer_free(yuuka_buffer * buf);
+/* A handle on device memory of another owner (another runtime's allocation, a part of a larger one), for every call
+ * that takes a buffer. The memory must be a device allocation of dev, all of it, and stay valid as long as the handle
+ * is used; yuuka_buffer_free then frees the handle alone. */
+YUUKA_API yuuka_status yuuka_buffer_view(yuuka_device * dev, void * device_ptr, uint64_t bytes, yuuka_buffer ** out);
 YUUKA_API uint64_t yuuka_buffer_size(const yuuka_buffer * buf);
 YUUKA_API void * yuuka_buffer_ptr(const yuuka_buffer * buf);
 
 /* yuuka_hip.h:66-72. Events here can also be recorded explicitly and timed,
  * which the reference does inside yuuka_plan_execute_profiled (:491-496). */
 YUUKA_API yuuka_status yuuka_stream_create(yuuka_device * dev, yuuka_stream ** out);
+/* A handle on a stream of another owner (a cudaStream_t of dev's primary context; NULL is its default stream), so that
+ * calls are ordered with that owner's work and can be captured with it. yuuka_stream_destroy frees the handle alone. */
+YUUKA_API yuuka_status yuuka_stream_view(yuuka_device * dev, void * cuda_stream, yuuka_stream ** out);
 YUUKA_API void yuuka_stream_destroy(yuuka_stream * stream);
 YUUKA_API yuuka_status yuuka_stream_synchronize(yuuka_stream * stream);
 YUUKA_API yuuka_status yuuka_event_create(yuuka_device * dev, yuuka_event ** out);
@@ -198,6 +211,98 @@ YUUKA_API uint64_t yuuka_weights_tiled_bytes(uint32_t dtype, uint64_t n_out, uin
 YUUKA_API yuuka_status yuuka_weights_tile(yuuka_stream * stream, yuuka_buffer * dst, uint64_t dst_offset,
                                           const yuuka_buffer * src, uint64_t src_offset, uint32_t dtype,
                                           uint64_t n_out, uint64_t n_in, yuuka_event * completion);
+
+/* ---- A paged key-value cache for hosts with layers of their own ----
+ * What YUUKA_OP_ATTENTION_PREFILL_PAGED reads and the KV half of ATTENTION_PREP writes (yuuka_hip.h:104-149), as calls on
+ * buffers of the caller: rows go into the pools in the pools' format, come back as plain numbers, and are attended to by
+ * one new token per sequence. Sessions do the same on pools of their own.
+ *
+ * K and V pools are [pool_blocks][block_size][yuuka_kv_row_bytes], a row all KV heads of a token behind one another;
+ * position p of sequence s lies in row p % block_size of block tables[s][p / block_size] (memory.Table.Map). Formats:
+ *   F32, F16  the values; F16 rounds half up on the dropped bits, as sessions do (tensor/half.go:36-68)
+ *   Q8_0      blocks of 32 values: f16 scale amax / 127, int8 x / scale rounded half away from zero (kv_format.go:97-131)
+ *   F8        kv_heads * head_dim E4M3 values x * (448 / amax), rounded to nearest even, amax over a token's head; then
+ *             kv_heads f32 scales amax / 448; zeros up to a multiple of 16 bytes. A value is its E4M3 times the scale.
+ *             A head for which 448 / amax passes 3e38 (amax below 1.5e-36) is stored as zeros.
+ * head_dim is 64, 128 or 256. Offsets of pools are multiples of 16 bytes, of tables of 4. */
+typedef struct yuuka_kv_cache {
+    yuuka_buffer * k;
+    yuuka_buffer * v;
+    const yuuka_buffer * tables; /* int32 [sequences][table_stride] on the device */
+    uint64_t k_offset, v_offset, tables_offset;
+    int32_t format; /* yuuka_kv_format */
+    int32_t kv_heads, head_dim;
+    int32_t block_size, pool_blocks;
+    int32_t sequences, table_stride;
+} yuuka_kv_cache;
+/* Bytes of one row of a pool; 0 for a format or head dimension without a form. */
+YUUKA_API uint64_t yuuka_kv_row_bytes(int32_t format, int32_t kv_heads, int32_t head_dim);
+
+/* Device data (sequence ids, positions, lengths, block ids) is checked by the kernels: a call touches no memory outside
+ * its buffers whatever they hold. What is out of range is not written, or read as NaN, and the bits below are or-ed into
+ * `status`, an int32 on the device that the caller zeroes (NULL: not recorded). */
+#define YUUKA_KV_STATUS_BLOCK 0x1    /* a block id outside 0..pool_blocks-1 */
+#define YUUKA_KV_STATUS_SEQUENCE 0x2 /* a sequence id outside 0..sequences-1 */
+#define YUUKA_KV_STATUS_POSITION 0x4 /* a position or length beyond table_stride * block_size, or a length below 0 */
+
+/* K and V rows of tokens, [rows][kv_heads][head_dim] each, of type F32, F16 or BF16. Row r is position pos[r] of sequence
+ * seq[r]; a row with a negative position names no token (the rest of a padded batch). */
+typedef struct yuuka_kv_rows {
+    yuuka_buffer * k; /* yuuka_kv_write reads them, yuuka_kv_read writes them */
+    yuuka_buffer * v;
+    const yuuka_buffer * pos; /* int32 [rows] on the device */
+    const yuuka_buffer * seq; /* int32 [rows] on the device; NULL: row r is sequence r */
+    yuuka_buffer * status;    /* or NULL */
+    uint64_t k_offset, v_offset, pos_offset, seq_offset, status_offset; /* bytes */
+    uint64_t k_stride, v_stride; /* elements from row to row; 0: kv_heads * head_dim */
+    uint64_t rows;               /* 1..2^31 - 1 */
+    uint32_t dtype;
+} yuuka_kv_rows;
+/* Writes the rows into the pools, in the pools' format; rows without a token leave everything as it is. The tokens of a
+ * call are distinct: where two rows name the same one, each head of it holds values of either. Asynchronous on stream. k and
+ * v start at multiples of 16 bytes from row to row. */
+YUUKA_API yuuka_status yuuka_kv_write(yuuka_stream * stream, const yuuka_kv_cache * cache, const yuuka_kv_rows * rows,
+                                      yuuka_event * completion);
+/* Reads rows back as numbers of the given type (rounded to nearest even where the type is narrower). Rows without a token
+ * are left as they were, rows out of range become NaN. Asynchronous on stream. */
+YUUKA_API yuuka_status yuuka_kv_read(yuuka_stream * stream, const yuuka_kv_cache * cache, const yuuka_kv_rows * rows,
+                                     yuuka_event * completion);
+
+/* Attention of one new token per sequence (decode) over a paged cache, split over the cache's length and joined.
+ * For row b of the batch, sequence s = seq_ids[b], query head h over KV head h / (heads / kv_heads), with n = lens[b] and
+ * keys j of positions max(0, n - window) .. n - 1 (the new token's own row is the last: write it first):
+ *   s_j = scale * q . k_j    out = sum_j exp(s_j) v_j / sum_j exp(s_j)    lse = ln sum_j exp(s_j)
+ * and out *= 1 / (1 + exp(-gate)) with a gate (the qwen35 output gate, model/qwen35/forward.go:188-220). Without keys
+ * (length 0) out is 0 and lse -infinity. Scores, statistics and sums are f32; with q of type F32 queries and
+ * probabilities enter the products with 22 bits, with F16 or BF16 with 11. Lengths live on the device, so that a
+ * captured call stays valid as sequences grow. A row whose length or sequence or one of whose blocks is out of range
+ * becomes NaN. Rows and values of the cache beyond a sequence's length are never used, whatever they hold. */
+typedef struct yuuka_attention_decode_args {
+    const yuuka_buffer * q; /* [batch][heads][head_dim] */
+    yuuka_buffer * out;     /* the same shape and type */
+    const yuuka_buffer * gate; /* NULL, or with the strides of q (it may lie between the heads of q) */
+    yuuka_buffer * lse;        /* NULL, or f32 [batch][heads] */
+    const yuuka_buffer * lens; /* int32 [batch] */
+    const yuuka_buffer * seq_ids; /* int32 [batch]; NULL: row b is sequence b. Rows may name the same sequence */
+    yuuka_buffer * status;        /* or NULL */
+    uint64_t q_offset, out_offset, gate_offset, lse_offset, lens_offset, seq_ids_offset, status_offset; /* bytes */
+    uint64_t q_row_stride, q_head_stride;     /* elements; 0: q_head_stride head_dim, q_row_stride heads * q_head_stride */
+    uint64_t out_row_stride, out_head_stride; /* the same; rows and heads of out do not overlap */
+    uint32_t dtype;        /* of q, gate and out: F32, F16 or BF16 */
+    int32_t batch, heads;  /* heads a multiple of kv_heads */
+    int32_t window;        /* 0: none */
+    float scale;           /* 0: 1 / sqrt(head_dim) */
+} yuuka_attention_decode_args;
+/* Device memory for the joining of split sequences: one for all shapes, a few MB. Calls that use the same one are
+ * ordered (one stream, or events between them); graphs that may run at the same time are captured with one each. */
+typedef struct yuuka_attention_scratch yuuka_attention_scratch;
+YUUKA_API yuuka_status yuuka_attention_scratch_create(yuuka_device * dev, yuuka_attention_scratch ** out);
+YUUKA_API void yuuka_attention_scratch_destroy(yuuka_attention_scratch * scratch);
+/* Asynchronous on stream. q, gate and out start at multiples of 16 bytes from row to row and head to head. out and lse lie
+ * over no other operand. */
+YUUKA_API yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_attention_scratch * scratch,
+                                              const yuuka_kv_cache * cache, const yuuka_attention_decode_args * args,
+                                              yuuka_event * completion);
 
 /* ------------------------------------------------------------------------
  * Model and verify session (what engine/gpu's Model/Session/plan builders do

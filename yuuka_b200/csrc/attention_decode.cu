@@ -1,0 +1,155 @@
+// yuuka_attention_decode: checks of arguments, scratch, choice of the kernel.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "attention_decode.cuh"
+
+struct yuuka_attention_scratch {
+    yuuka_device * dev = nullptr;
+    uint8_t * memory = nullptr;
+};
+
+namespace yk {
+
+// The largest partial of any shape: 16 columns of 256 dimensions.
+constexpr size_t DEC_PART_MAX = 16 * (256 + 2) * sizeof(float);
+static size_t scratch_joins_bytes(const yuuka_device * dev) { return ((size_t)dev->sm_count * sizeof(int4) + 255) / 256 * 256; }
+
+// rows and heads of an output: either all heads of a row behind one another or all rows of a head
+static bool strides_disjoint(uint64_t rows, uint64_t row, uint64_t heads, uint64_t head, uint64_t dim) {
+    const unsigned __int128 r = row, h = head;
+    return (h >= dim && r >= (heads - 1) * h + dim) || (r >= dim && h >= (rows - 1) * r + dim);
+}
+
+}  // namespace yk
+
+extern "C" yuuka_status yuuka_attention_scratch_create(yuuka_device * dev, yuuka_attention_scratch ** out) {
+    using namespace yk;
+    return guard([&] {
+        YK_REQUIRE(out, YUUKA_ERR_INVALID_ARGUMENT, "attention_scratch_create: null argument");
+        *out = nullptr;
+        YK_REQUIRE(dev, YUUKA_ERR_INVALID_ARGUMENT, "attention_scratch_create: null argument");
+        set_device(dev);
+        void * ptr = nullptr;
+        const size_t bytes = scratch_joins_bytes(dev) + (size_t)dev->sm_count * 2 * DEC_PART_MAX;
+        const cudaError_t err = cudaMalloc(&ptr, bytes);
+        if (err != cudaSuccess) {
+            cudaGetLastError();
+            YK_REQUIRE(false, YUUKA_ERR_ALLOCATION, "cudaMalloc(%llu) failed: %s", (unsigned long long)bytes, cudaGetErrorString(err));
+        }
+        auto * s = new (std::nothrow) yuuka_attention_scratch();
+        if (!s) {
+            cudaFree(ptr);
+            throw std::bad_alloc();
+        }
+        s->dev = dev;
+        s->memory = (uint8_t *)ptr;
+        *out = s;
+    });
+}
+
+extern "C" void yuuka_attention_scratch_destroy(yuuka_attention_scratch * scratch) {
+    if (!scratch) return;
+    if (scratch->memory) {
+        cudaSetDevice(scratch->dev->index);
+        cudaFree(scratch->memory);
+    }
+    delete scratch;
+}
+
+extern "C" yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_attention_scratch * scratch, const yuuka_kv_cache * cache,
+                                               const yuuka_attention_decode_args * a, yuuka_event * completion) {
+    using namespace yk;
+    return guard([&] {
+        const char * op = "attention_decode";
+        YK_REQUIRE(stream && scratch && cache && a, YUUKA_ERR_INVALID_ARGUMENT, "%s: null argument", op);
+        const yuuka_device * dev = stream->dev;
+        YK_REQUIRE(scratch->dev->index == dev->index, YUUKA_ERR_INVALID_ARGUMENT, "%s: the scratch is on device %d, the stream on device %d", op,
+                   scratch->dev->index, dev->index);
+        DecodeParams p;
+        p.cache = check_cache(op, cache, dev);
+        YK_REQUIRE(a->dtype == YUUKA_DTYPE_F32 || a->dtype == YUUKA_DTYPE_F16 || a->dtype == YUUKA_DTYPE_BF16, YUUKA_ERR_UNSUPPORTED,
+                   "%s: dtype %u is not F32, F16 or BF16", op, a->dtype);
+        YK_REQUIRE(a->batch >= 1 && a->batch <= 65536, YUUKA_ERR_INVALID_ARGUMENT, "%s: batch %d is not 1..65536", op, a->batch);
+        YK_REQUIRE(a->heads >= 1 && a->heads <= 65536 && a->heads % cache->kv_heads == 0, YUUKA_ERR_INVALID_ARGUMENT,
+                   "%s: %d heads are not a multiple of %d KV heads up to 65536", op, a->heads, cache->kv_heads);
+        YK_REQUIRE(a->seq_ids || a->batch <= cache->sequences, YUUKA_ERR_INVALID_ARGUMENT, "%s: batch %d without sequence ids exceeds %d sequences", op,
+                   a->batch, cache->sequences);
+        YK_REQUIRE(a->window >= 0, YUUKA_ERR_INVALID_ARGUMENT, "%s: window %d", op, a->window);
+        YK_REQUIRE(std::isfinite(a->scale), YUUKA_ERR_INVALID_ARGUMENT, "%s: scale is not finite", op);
+        const uint64_t size = a->dtype == YUUKA_DTYPE_F32 ? 4 : 2, hd = (uint64_t)cache->head_dim, heads = (uint64_t)a->heads,
+                       batch = (uint64_t)a->batch;
+        const uint64_t qh = a->q_head_stride ? a->q_head_stride : hd, oh = a->out_head_stride ? a->out_head_stride : hd;
+        YK_REQUIRE(qh <= UINT64_MAX / heads && oh <= UINT64_MAX / heads, YUUKA_ERR_INVALID_ARGUMENT, "%s: head stride out of range", op);
+        const uint64_t qr = a->q_row_stride ? a->q_row_stride : heads * qh, orow = a->out_row_stride ? a->out_row_stride : heads * oh;
+        for (const uint64_t s : {qh, qr, oh, orow})
+            YK_REQUIRE(s <= (1ull << 48) && s * size % 16 == 0, YUUKA_ERR_INVALID_ARGUMENT, "%s: strides must be multiples of 16 bytes", op);
+        YK_REQUIRE(strides_disjoint(batch, orow, heads, oh, hd), YUUKA_ERR_INVALID_ARGUMENT, "%s: rows or heads of out overlap", op);
+        const uint64_t qb = span_bytes(batch, qr, heads, qh, hd, size), ob = span_bytes(batch, orow, heads, oh, hd, size);
+        check_range(op, "q", a->q, a->q_offset, qb, 16, dev);
+        check_range(op, "out", a->out, a->out_offset, ob, 16, dev);
+        if (a->gate) check_range(op, "gate", a->gate, a->gate_offset, qb, 16, dev);
+        if (a->lse) check_range(op, "lse", a->lse, a->lse_offset, 4 * batch * heads, 4, dev);
+        check_range(op, "lens", a->lens, a->lens_offset, 4 * batch, 4, dev);
+        if (a->seq_ids) check_range(op, "seq_ids", a->seq_ids, a->seq_ids_offset, 4 * batch, 4, dev);
+        if (a->status) check_range(op, "status", a->status, a->status_offset, 4, 4, dev);
+        const uint64_t pool = (uint64_t)p.cache.row_bytes * (uint64_t)cache->block_size * (uint64_t)cache->pool_blocks,
+                       tb = 4ull * (uint64_t)cache->sequences * (uint64_t)cache->table_stride, lb = 4 * batch * heads;
+        struct Range {
+            const char * name;
+            const yuuka_buffer * buf;
+            uint64_t offset, bytes;
+        };
+        const Range outs[2] = {{"out", a->out, a->out_offset, ob}, {"lse", a->lse, a->lse_offset, lb}};
+        const Range ins[8] = {{"q", a->q, a->q_offset, qb},
+                              {"gate", a->gate, a->gate_offset, qb},
+                              {"lens", a->lens, a->lens_offset, 4 * batch},
+                              {"seq_ids", a->seq_ids, a->seq_ids_offset, 4 * batch},
+                              {"status", a->status, a->status_offset, 4},
+                              {"the K pool", cache->k, cache->k_offset, pool},
+                              {"the V pool", cache->v, cache->v_offset, pool},
+                              {"the block table", cache->tables, cache->tables_offset, tb}};
+        for (const Range & x : outs)
+            for (const Range & y : ins) check_apart(op, x.name, x.buf, x.offset, x.bytes, y.name, y.buf, y.offset, y.bytes);
+        check_apart(op, "out", a->out, a->out_offset, ob, "lse", a->lse, a->lse_offset, lb);
+
+        p.q = (const uint8_t *)a->q->ptr + a->q_offset;
+        p.gate = a->gate ? (const uint8_t *)a->gate->ptr + a->gate_offset : nullptr;
+        p.out = (uint8_t *)a->out->ptr + a->out_offset;
+        p.lse = a->lse ? (float *)((uint8_t *)a->lse->ptr + a->lse_offset) : nullptr;
+        p.lens = (const int32_t *)((const uint8_t *)a->lens->ptr + a->lens_offset);
+        p.seq_ids = a->seq_ids ? (const int32_t *)((const uint8_t *)a->seq_ids->ptr + a->seq_ids_offset) : nullptr;
+        p.status = a->status ? (int32_t *)((uint8_t *)a->status->ptr + a->status_offset) : nullptr;
+        p.q_row = (int64_t)qr;
+        p.q_head = (int64_t)qh;
+        p.out_row = (int64_t)orow;
+        p.out_head = (int64_t)oh;
+        p.batch = a->batch;
+        p.heads = a->heads;
+        p.group = a->heads / cache->kv_heads;
+        // Tiles of up to 16 query heads share one reading of the keys (8 over f32 pools, see launch_decode_f32)
+        const int widest = cache->format == YUUKA_KV_F32 ? 8 : 16;
+        p.head_tiles = (p.group + widest - 1) / widest;
+        p.tile_heads = (p.group + p.head_tiles - 1) / p.head_tiles;
+        const int cols = p.tile_heads <= 8 ? 8 : 16;
+        p.window = a->window;
+        p.dtype = (int)a->dtype;
+        const double scale = a->scale != 0.0f ? (double)a->scale : 1.0 / std::sqrt((double)cache->head_dim);
+        p.scale_log2 = (float)(scale * 1.4426950408889634);
+        p.joins = (int4 *)scratch->memory;
+        p.partial = (float *)(scratch->memory + scratch_joins_bytes(dev));
+        p.min_tiles = 4;
+        // tiles of a warp are counted in 32 bits
+        const double tiles = (double)a->batch * cache->kv_heads * p.head_tiles * (p.cache.capacity / DEC_TILE + 1.0);
+        YK_REQUIRE(tiles / (4.0 * dev->sm_count) < 1e9, YUUKA_ERR_UNSUPPORTED, "%s: %g tiles of keys are too many for one call", op, tiles);
+        set_device(dev);
+        switch (cache->format) {
+        case YUUKA_KV_F32: launch_decode_f32(stream->s, p, cache->head_dim, cols, dev->sm_count); break;
+        case YUUKA_KV_F16: launch_decode_f16(stream->s, p, cache->head_dim, cols, dev->sm_count); break;
+        case YUUKA_KV_Q8_0: launch_decode_q8_0(stream->s, p, cache->head_dim, cols, dev->sm_count); break;
+        default: launch_decode_f8(stream->s, p, cache->head_dim, cols, dev->sm_count); break;
+        }
+        record_completion(stream, completion);
+    });
+}

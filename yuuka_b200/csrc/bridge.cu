@@ -125,9 +125,33 @@ yuuka_status yuuka_buffer_alloc(yuuka_device * dev, uint64_t bytes, yuuka_buffer
     });
 }
 
+yuuka_status yuuka_buffer_view(yuuka_device * dev, void * device_ptr, uint64_t bytes, yuuka_buffer ** out) {
+    return guard([&] {
+        YK_REQUIRE(out, YUUKA_ERR_INVALID_ARGUMENT, "buffer_view: null argument");
+        *out = nullptr;
+        YK_REQUIRE(dev && device_ptr, YUUKA_ERR_INVALID_ARGUMENT, "buffer_view: null argument");
+        YK_REQUIRE(bytes > 0 && (uint64_t)(uintptr_t)device_ptr + bytes > bytes, YUUKA_ERR_INVALID_ARGUMENT, "buffer_view: invalid size");
+        set_device(dev);
+        // (the last byte too: a size beyond the memory is the likeliest mistake)
+        for (const uint64_t at : {(uint64_t)0, bytes - 1}) {
+            cudaPointerAttributes attr{};
+            const cudaError_t err = cudaPointerGetAttributes(&attr, (const uint8_t *)device_ptr + at);
+            if (err != cudaSuccess) cudaGetLastError();
+            YK_REQUIRE(err == cudaSuccess && (attr.type == cudaMemoryTypeDevice || attr.type == cudaMemoryTypeManaged) && attr.device == dev->index,
+                       YUUKA_ERR_INVALID_ARGUMENT, "buffer_view: byte %llu is not memory of device %d", (unsigned long long)at, dev->index);
+        }
+        auto * buf = new yuuka_buffer();
+        buf->dev = dev;
+        buf->ptr = device_ptr;
+        buf->bytes = bytes;
+        buf->view = true;
+        *out = buf;
+    });
+}
+
 void yuuka_buffer_free(yuuka_buffer * buf) {
     if (!buf) return;
-    if (buf->ptr) {
+    if (buf->ptr && !buf->view) {
         cudaSetDevice(buf->dev->index);
         cudaFree(buf->ptr);
     }
@@ -153,11 +177,24 @@ yuuka_status yuuka_stream_create(yuuka_device * dev, yuuka_stream ** out) {
     });
 }
 
+yuuka_status yuuka_stream_view(yuuka_device * dev, void * cuda_stream, yuuka_stream ** out) {
+    return guard([&] {
+        YK_REQUIRE(out, YUUKA_ERR_INVALID_ARGUMENT, "stream_view: null argument");
+        *out = nullptr;
+        YK_REQUIRE(dev, YUUKA_ERR_INVALID_ARGUMENT, "stream_view: null argument");
+        auto * s = new yuuka_stream();
+        s->dev = dev;
+        s->s = (cudaStream_t)cuda_stream;
+        s->view = true;
+        *out = s;
+    });
+}
+
 void yuuka_stream_destroy(yuuka_stream * stream) {
     if (!stream) return;
-    if (stream->s) {
+    if (stream->s || stream->view) {
         cudaSetDevice(stream->dev->index);
-        cudaStreamDestroy(stream->s);
+        if (!stream->view) cudaStreamDestroy(stream->s);
         stream->scratch.release();
     }
     delete stream;

@@ -85,6 +85,7 @@ struct yuuka_buffer {
     yuuka_device * dev = nullptr;
     void * ptr = nullptr;
     uint64_t bytes = 0;
+    bool view = false;  // memory of another owner
 };
 
 namespace yk {
@@ -158,6 +159,7 @@ private:
 struct yuuka_stream {
     yuuka_device * dev = nullptr;
     cudaStream_t s = nullptr;
+    bool view = false;  // a stream of another owner
     yk::StreamScratch scratch;
 };
 

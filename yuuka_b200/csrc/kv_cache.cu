@@ -1,0 +1,394 @@
+// Rows of a paged key-value cache: written in the cache's format, read back as plain numbers (yuuka_kv_write, yuuka_kv_read).
+//
+// Both move a row once and compute little, so what bounds them is memory: rows * 2 * (numbers + pool row) bytes. A warp takes
+// 256 values of a row (eight per lane, one 16- or 32-byte load), which holds whole Q8_0 blocks (four lanes each) and whole
+// heads (8, 16 or 32 lanes each), so the maxima that the scales come from need shuffles alone.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "kv_cache.cuh"
+#include "quant.cuh"
+
+namespace yk {
+
+// ---------------------------------------------------------------------------
+// checks of arguments
+
+uint64_t kv_row_bytes(int32_t format, int32_t kv_heads, int32_t head_dim) {
+    if (kv_heads < 1 || kv_heads > 1024 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return 0;
+    const uint64_t n = (uint64_t)kv_heads * head_dim;
+    switch (format) {
+    case YUUKA_KV_F32: return 4 * n;
+    case YUUKA_KV_F16: return 2 * n;
+    case YUUKA_KV_Q8_0: return n / 32 * 34;
+    case YUUKA_KV_F8: return (n + 4 * (uint64_t)kv_heads + 15) / 16 * 16;
+    default: return 0;
+    }
+}
+
+void check_geometry(const char * op, const yuuka_kv_cache * c) {
+    YK_REQUIRE(c->format >= YUUKA_KV_F32 && c->format <= YUUKA_KV_F8, YUUKA_ERR_INVALID_ARGUMENT, "%s: unknown KV format %d", op, c->format);
+    YK_REQUIRE(c->kv_heads >= 1 && c->kv_heads <= 1024, YUUKA_ERR_INVALID_ARGUMENT, "%s: %d KV heads are not 1..1024", op, c->kv_heads);
+    YK_REQUIRE(kv_row_bytes(c->format, c->kv_heads, c->head_dim) > 0, YUUKA_ERR_UNSUPPORTED, "%s: head_dim %d is not 64, 128 or 256", op,
+               c->head_dim);
+    YK_REQUIRE(c->block_size >= 1 && c->pool_blocks >= 1 && (uint64_t)c->block_size * (uint64_t)c->pool_blocks <= INT_MAX,
+               YUUKA_ERR_INVALID_ARGUMENT, "%s: %d blocks of %d rows are not 1..2^31 - 1 rows", op, c->pool_blocks, c->block_size);
+    YK_REQUIRE(c->sequences >= 1 && c->table_stride >= 1, YUUKA_ERR_INVALID_ARGUMENT, "%s: %d block tables of %d ids", op, c->sequences,
+               c->table_stride);
+}
+
+uint64_t span_bytes(uint64_t rows, uint64_t row_stride, uint64_t heads, uint64_t head_stride, uint64_t dim, uint64_t size) {
+    const unsigned __int128 n =
+        ((unsigned __int128)(rows - 1) * row_stride + (unsigned __int128)(heads - 1) * head_stride + dim) * size;
+    return n >> 62 ? UINT64_MAX : (uint64_t)n;
+}
+
+void check_range(const char * op, const char * what, const yuuka_buffer * buf, uint64_t offset, uint64_t bytes, uint64_t align,
+                 const yuuka_device * dev) {
+    YK_REQUIRE(buf, YUUKA_ERR_INVALID_ARGUMENT, "%s: %s is null", op, what);
+    YK_REQUIRE(buf->dev->index == dev->index, YUUKA_ERR_INVALID_ARGUMENT, "%s: %s is on device %d, the stream on device %d", op, what,
+               buf->dev->index, dev->index);
+    YK_REQUIRE(offset <= buf->bytes && bytes <= buf->bytes - offset, YUUKA_ERR_INVALID_ARGUMENT, "%s: %s range exceeds the buffer", op, what);
+    YK_REQUIRE(((uint64_t)(uintptr_t)buf->ptr + offset) % align == 0, YUUKA_ERR_INVALID_ARGUMENT,
+               "%s: %s does not start at a multiple of %llu bytes", op, what, (unsigned long long)align);
+}
+
+void check_apart(const char * op, const char * a_name, const yuuka_buffer * a, uint64_t a_offset, uint64_t a_bytes, const char * b_name,
+                 const yuuka_buffer * b, uint64_t b_offset, uint64_t b_bytes) {
+    if (!a || !b) return;
+    const uint64_t a0 = (uint64_t)(uintptr_t)a->ptr + a_offset, b0 = (uint64_t)(uintptr_t)b->ptr + b_offset;
+    YK_REQUIRE(a0 + a_bytes <= b0 || b0 + b_bytes <= a0, YUUKA_ERR_INVALID_ARGUMENT, "%s: %s lies over %s", op, a_name, b_name);
+}
+
+PagedCache check_cache(const char * op, const yuuka_kv_cache * c, const yuuka_device * dev) {
+    check_geometry(op, c);
+    const uint64_t rb = kv_row_bytes(c->format, c->kv_heads, c->head_dim), pool = rb * (uint64_t)c->block_size * (uint64_t)c->pool_blocks;
+    check_range(op, "the K pool", c->k, c->k_offset, pool, 16, dev);
+    check_range(op, "the V pool", c->v, c->v_offset, pool, 16, dev);
+    check_range(op, "the block table", c->tables, c->tables_offset, 4ull * (uint64_t)c->sequences * (uint64_t)c->table_stride, 4, dev);
+    check_apart(op, "the K pool", c->k, c->k_offset, pool, "the V pool", c->v, c->v_offset, pool);
+    PagedCache p;
+    p.k = (uint8_t *)c->k->ptr + c->k_offset;
+    p.v = (uint8_t *)c->v->ptr + c->v_offset;
+    p.tables = (const int32_t *)((const uint8_t *)c->tables->ptr + c->tables_offset);
+    p.row_bytes = (int64_t)rb;
+    p.format = c->format;
+    p.kv_heads = c->kv_heads;
+    p.block_size = c->block_size;
+    p.pool_blocks = c->pool_blocks;
+    p.sequences = c->sequences;
+    p.table_stride = c->table_stride;
+    p.shift = -1;
+    for (int s = 0; s < 31; s++)
+        if (c->block_size == 1 << s) p.shift = s;
+    p.capacity = (int)std::min<uint64_t>((uint64_t)c->table_stride * (uint64_t)c->block_size, INT_MAX);
+    return p;
+}
+
+// ---------------------------------------------------------------------------
+// kernels
+
+struct MoveParams {
+    PagedCache cache;
+    uint8_t * k;  // rows of numbers
+    uint8_t * v;
+    int64_t k_stride, v_stride;  // elements
+    const int32_t * pos;
+    const int32_t * seq;
+    int32_t * status;
+    int rows, kv_dim, chunks;  // chunks of 256 values in a row
+};
+
+template <typename T> __device__ __forceinline__ void load8(const T * src, float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(src)), b = __ldg(reinterpret_cast<const float4 *>(src) + 1);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(src));
+        const T * e = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)e[i];
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T * dst, const float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        uint4 raw;
+        T * e = reinterpret_cast<T *>(&raw);
+#pragma unroll
+        for (int i = 0; i < 8; i++) e[i] = (T)x[i];
+        *reinterpret_cast<uint4 *>(dst) = raw;
+    }
+}
+
+// f32 -> f16 bits, half up on the dropped bits. Magnitudes whose result is a normal f16 take one add and a conversion that
+// cuts off; the others the codec's own steps.
+__device__ __forceinline__ uint16_t half_up(float f) {
+    const uint32_t b = __float_as_uint(f), a = b & 0x7fffffffu;
+    if (a >= 0x38800000u && a < 0x477ff000u) return __half_as_ushort(__float2half_rz(__uint_as_float(b + 0x1000u)));
+    return f32_to_f16_ref(f);
+}
+// The nearest integer to v / scale, halves away from zero, of the f32 quotient. The product with 1 / scale is within 2^-22
+// of the quotient (relative; at most 127.5 in magnitude, so 2^-15 in all): away from a half it rounds to the same integer.
+__device__ __forceinline__ int quantize_q8(float v, float scale, float inv) {
+    const float y = v * inv, t = truncf(y), d = fabsf(y - t);
+    if (fabsf(d - 0.5f) > 1e-4f) return (int)t + (d > 0.5f ? (v < 0.0f ? -1 : 1) : 0);
+    return (int)round((double)(v / scale));
+}
+
+// Where row r's token lies: the pool row, -1 for a row without a token, -2 for one out of range.
+__device__ __forceinline__ int move_slot(const MoveParams & p, int r) {
+    const int pos = __ldg(p.pos + r);
+    int bad;
+    const int slot = kv_token_slot(p.cache, p.seq && pos >= 0 ? __ldg(p.seq + r) : r, pos, bad);
+    if (bad && p.status && (threadIdx.x & 31) == 0) atomicOr(p.status, bad);
+    return slot;
+}
+
+constexpr int MOVE_WARPS = 8;
+constexpr int Q8_CHUNK = 272;  // bytes of 256 values in Q8_0
+
+// The pool is aligned to 16 bytes, a row of Q8_0 to 4: rows are put together in shared memory and stored by words.
+template <int FMT, int HD, typename T>
+__global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MoveParams p) {
+    __shared__ __align__(16) uint8_t stage_all[FMT == YUUKA_KV_Q8_0 ? MOVE_WARPS * Q8_CHUNK : 16];
+    pdl_entry();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t units = (int64_t)p.rows * 2 * p.chunks;
+    for (int64_t unit = (int64_t)blockIdx.x * MOVE_WARPS + warp; unit < units; unit += (int64_t)gridDim.x * MOVE_WARPS) {
+        const int r = (int)(unit / (2 * p.chunks)), rest = (int)(unit - (int64_t)r * 2 * p.chunks);
+        const bool is_v = rest >= p.chunks;
+        const int chunk = is_v ? rest - p.chunks : rest, first = chunk * 256 + lane * 8;
+        const bool live = first < p.kv_dim;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = 0.0f;
+        const T * src = reinterpret_cast<const T *>(is_v ? p.v : p.k) + (int64_t)r * (is_v ? p.v_stride : p.k_stride) + first;
+        if (live) load8(src, x);
+        const int slot = move_slot(p, r);
+        if (slot < 0) continue;  // (the whole warp: one row)
+        uint8_t * row = (is_v ? p.cache.v : p.cache.k) + (int64_t)slot * p.cache.row_bytes;
+        if constexpr (FMT == YUUKA_KV_F32) {
+            if (live) store8(reinterpret_cast<float *>(row) + first, x);
+        } else if constexpr (FMT == YUUKA_KV_F16) {
+            if (live) {
+                uint4 raw;
+                uint16_t * e = reinterpret_cast<uint16_t *>(&raw);
+#pragma unroll
+                for (int i = 0; i < 8; i++) e[i] = half_up(x[i]);
+                *reinterpret_cast<uint4 *>(row + 2 * first) = raw;
+            }
+        } else if constexpr (FMT == YUUKA_KV_Q8_0) {
+            float amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const float scale = amax / 127.0f, inv = 1.0f / scale;
+            int q[8];
+            if (scale == 0.0f) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) q[i] = 0;
+            } else if (inv <= 3.0e38f) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) q[i] = quantize_q8(x[i], scale, inv);
+            } else {  // (a scale whose inverse is no finite number)
+#pragma unroll
+                for (int i = 0; i < 8; i++) q[i] = (int)round((double)(x[i] / scale));
+            }
+            uint8_t * stage = stage_all + warp * Q8_CHUNK;
+            uint16_t * blk = reinterpret_cast<uint16_t *>(stage + (lane >> 2) * 34);
+            __syncwarp();  // (the words of the unit before have been read)
+            if ((lane & 3) == 0) blk[0] = half_up(scale);
+#pragma unroll
+            for (int i = 0; i < 4; i++) blk[1 + (lane & 3) * 4 + i] = (uint16_t)((q[2 * i] & 0xff) | (q[2 * i + 1] << 8));
+            __syncwarp();
+            const int words = min(256, p.kv_dim - chunk * 256) / 32 * 34 / 4;
+            uint32_t * dst = reinterpret_cast<uint32_t *>(row + chunk * Q8_CHUNK);
+            for (int w = lane; w < words; w += 32) dst[w] = reinterpret_cast<const uint32_t *>(stage)[w];
+        } else {
+            float amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));
+#pragma unroll
+            for (int o = HD / 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            const bool none = !(448.0f / amax <= 3.0e38f);  // (nothing but zeros, or too small for a finite factor)
+            const float inv = none ? 0.0f : 448.0f / amax;  // (0 keeps a NaN)
+            uint2 raw;
+            __nv_fp8x2_storage_t * e = reinterpret_cast<__nv_fp8x2_storage_t *>(&raw);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                e[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i] * inv, x[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+            if (live) {
+                *reinterpret_cast<uint2 *>(row + first) = raw;
+                if (first % HD == 0) *reinterpret_cast<float *>(row + p.kv_dim + first / HD * 4) = none ? 0.0f : amax / 448.0f;
+                // (the zeros behind the scales)
+                if (first + 8 == p.kv_dim)
+                    for (int at = p.kv_dim + 4 * (p.kv_dim / HD); at < p.cache.row_bytes; at += 4) *reinterpret_cast<uint32_t *>(row + at) = 0;
+            }
+        }
+    }
+}
+
+template <int FMT, int HD, typename T>
+__global__ void __launch_bounds__(MOVE_WARPS * 32) kv_read_kernel(const MoveParams p) {
+    __shared__ __align__(16) uint8_t stage_all[FMT == YUUKA_KV_Q8_0 ? MOVE_WARPS * Q8_CHUNK : 16];
+    pdl_entry();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t units = (int64_t)p.rows * 2 * p.chunks;
+    for (int64_t unit = (int64_t)blockIdx.x * MOVE_WARPS + warp; unit < units; unit += (int64_t)gridDim.x * MOVE_WARPS) {
+        const int r = (int)(unit / (2 * p.chunks)), rest = (int)(unit - (int64_t)r * 2 * p.chunks);
+        const bool is_v = rest >= p.chunks;
+        const int chunk = is_v ? rest - p.chunks : rest, first = chunk * 256 + lane * 8;
+        const int slot = move_slot(p, r);
+        if (slot == -1) continue;
+        const bool live = first < p.kv_dim;
+        const uint8_t * row = (is_v ? p.cache.v : p.cache.k) + (int64_t)max(slot, 0) * p.cache.row_bytes;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __uint_as_float(0x7fffffffu);
+        if (slot >= 0) {
+            if constexpr (FMT == YUUKA_KV_F32) {
+                if (live) load8(reinterpret_cast<const float *>(row) + first, x);
+            } else if constexpr (FMT == YUUKA_KV_F16) {
+                if (live) load8(reinterpret_cast<const __half *>(row) + first, x);
+            } else if constexpr (FMT == YUUKA_KV_Q8_0) {
+                uint8_t * stage = stage_all + warp * Q8_CHUNK;
+                const int words = min(256, p.kv_dim - chunk * 256) / 32 * 34 / 4;
+                const uint32_t * src = reinterpret_cast<const uint32_t *>(row + chunk * Q8_CHUNK);
+                __syncwarp();
+                for (int w = lane; w < words; w += 32) reinterpret_cast<uint32_t *>(stage)[w] = __ldg(src + w);
+                __syncwarp();
+                if (live) {
+                    const uint16_t * blk = reinterpret_cast<const uint16_t *>(stage + (lane >> 2) * 34);
+                    const float d = __half2float(__ushort_as_half(blk[0]));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint16_t q = blk[1 + (lane & 3) * 4 + i];
+                        x[2 * i] = d * (float)(int8_t)(q & 0xff);
+                        x[2 * i + 1] = d * (float)(int8_t)(q >> 8);
+                    }
+                }
+            } else if (live) {
+                const uint2 raw = __ldg(reinterpret_cast<const uint2 *>(row + first));
+                const float d = __ldg(reinterpret_cast<const float *>(row + p.kv_dim) + first / HD);
+                const __nv_fp8x2_storage_t * e = reinterpret_cast<const __nv_fp8x2_storage_t *>(&raw);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 v = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(e[i], __NV_E4M3)));
+                    x[2 * i] = d * v.x;
+                    x[2 * i + 1] = d * v.y;
+                }
+            }
+        }
+        if (live) store8(reinterpret_cast<T *>(is_v ? p.v : p.k) + (int64_t)r * (is_v ? p.v_stride : p.k_stride) + first, x);
+    }
+}
+
+template <int FMT, int HD, typename T>
+static void launch_move_as(yuuka_stream * stream, const MoveParams & p, bool write) {
+    const int64_t units = (int64_t)p.rows * 2 * p.chunks;
+    // eight CTAs of eight warps fill an SM
+    const int64_t grid = std::min<int64_t>((units + MOVE_WARPS - 1) / MOVE_WARPS, (int64_t)stream->dev->sm_count * 8);
+    launch_k(write ? kv_write_kernel<FMT, HD, T> : kv_read_kernel<FMT, HD, T>, (unsigned)grid, MOVE_WARPS * 32, 0, stream->s, p);
+}
+template <int FMT, typename T> static void launch_move_format(yuuka_stream * stream, const MoveParams & p, bool write, int head_dim) {
+    if constexpr (FMT == YUUKA_KV_F8) {  // (the other formats know no heads)
+        if (head_dim == 64) return launch_move_as<FMT, 64, T>(stream, p, write);
+        if (head_dim == 256) return launch_move_as<FMT, 256, T>(stream, p, write);
+    }
+    launch_move_as<FMT, 128, T>(stream, p, write);
+}
+template <typename T> static void launch_move(yuuka_stream * stream, const MoveParams & p, bool write, int head_dim) {
+    switch (p.cache.format) {
+    case YUUKA_KV_F32: return launch_move_format<YUUKA_KV_F32, T>(stream, p, write, head_dim);
+    case YUUKA_KV_F16: return launch_move_format<YUUKA_KV_F16, T>(stream, p, write, head_dim);
+    case YUUKA_KV_Q8_0: return launch_move_format<YUUKA_KV_Q8_0, T>(stream, p, write, head_dim);
+    default: return launch_move_format<YUUKA_KV_F8, T>(stream, p, write, head_dim);
+    }
+}
+
+static yuuka_status move_rows(const char * op, bool write, yuuka_stream * stream, const yuuka_kv_cache * cache, const yuuka_kv_rows * rows,
+                              yuuka_event * completion) {
+    return guard([&] {
+        YK_REQUIRE(stream && cache && rows, YUUKA_ERR_INVALID_ARGUMENT, "%s: null argument", op);
+        const yuuka_device * dev = stream->dev;
+        MoveParams p;
+        p.cache = check_cache(op, cache, dev);
+        YK_REQUIRE(rows->rows >= 1 && rows->rows <= INT_MAX, YUUKA_ERR_INVALID_ARGUMENT, "%s: %llu rows", op, (unsigned long long)rows->rows);
+        YK_REQUIRE(rows->dtype == YUUKA_DTYPE_F32 || rows->dtype == YUUKA_DTYPE_F16 || rows->dtype == YUUKA_DTYPE_BF16, YUUKA_ERR_UNSUPPORTED,
+                   "%s: dtype %u is not F32, F16 or BF16", op, rows->dtype);
+        const uint64_t size = rows->dtype == YUUKA_DTYPE_F32 ? 4 : 2, dim = (uint64_t)cache->kv_heads * (uint64_t)cache->head_dim;
+        const uint64_t ks = rows->k_stride ? rows->k_stride : dim, vs = rows->v_stride ? rows->v_stride : dim;
+        YK_REQUIRE(ks >= dim && vs >= dim, YUUKA_ERR_INVALID_ARGUMENT, "%s: row stride below %llu elements", op, (unsigned long long)dim);
+        YK_REQUIRE(ks * size % 16 == 0 && vs * size % 16 == 0, YUUKA_ERR_INVALID_ARGUMENT, "%s: row strides must be multiples of 16 bytes", op);
+        const uint64_t kb = span_bytes(rows->rows, ks, 1, 0, dim, size), vb = span_bytes(rows->rows, vs, 1, 0, dim, size);
+        check_range(op, "k", rows->k, rows->k_offset, kb, 16, dev);
+        check_range(op, "v", rows->v, rows->v_offset, vb, 16, dev);
+        check_range(op, "pos", rows->pos, rows->pos_offset, 4 * rows->rows, 4, dev);
+        if (rows->seq) check_range(op, "seq", rows->seq, rows->seq_offset, 4 * rows->rows, 4, dev);
+        if (rows->status) check_range(op, "status", rows->status, rows->status_offset, 4, 4, dev);
+        // what is written lies over nothing that is read
+        const uint64_t pool = (uint64_t)p.cache.row_bytes * (uint64_t)cache->block_size * (uint64_t)cache->pool_blocks,
+                       tb = 4ull * (uint64_t)cache->sequences * (uint64_t)cache->table_stride;
+        struct Range {
+            const char * name;
+            const yuuka_buffer * buf;
+            uint64_t offset, bytes;
+        };
+        const Range pools[2] = {{"the K pool", cache->k, cache->k_offset, pool}, {"the V pool", cache->v, cache->v_offset, pool}};
+        const Range nums[2] = {{"k", rows->k, rows->k_offset, kb}, {"v", rows->v, rows->v_offset, vb}};
+        const Range lists[4] = {{"the block table", cache->tables, cache->tables_offset, tb},
+                                {"pos", rows->pos, rows->pos_offset, 4 * rows->rows},
+                                {"seq", rows->seq, rows->seq_offset, 4 * rows->rows},
+                                {"status", rows->status, rows->status_offset, 4}};
+        for (const Range & a : write ? pools : nums) {
+            for (const Range & b : write ? nums : pools) check_apart(op, a.name, a.buf, a.offset, a.bytes, b.name, b.buf, b.offset, b.bytes);
+            for (const Range & b : lists) check_apart(op, a.name, a.buf, a.offset, a.bytes, b.name, b.buf, b.offset, b.bytes);
+        }
+        if (!write) {
+            // (two strided arrays may lie side by side in one: the rows themselves must not meet)
+            const uint64_t k0 = (uint64_t)(uintptr_t)rows->k->ptr + rows->k_offset, v0 = (uint64_t)(uintptr_t)rows->v->ptr + rows->v_offset;
+            const uint64_t apart = v0 > k0 ? v0 - k0 : k0 - v0, stride = ks * size, row = dim * size;
+            const bool interleaved = ks == vs && apart % stride >= row && apart % stride + row <= stride;
+            if (!interleaved) check_apart(op, "k", rows->k, rows->k_offset, kb, "v", rows->v, rows->v_offset, vb);
+        }
+        p.k = (uint8_t *)rows->k->ptr + rows->k_offset;
+        p.v = (uint8_t *)rows->v->ptr + rows->v_offset;
+        p.k_stride = (int64_t)ks;
+        p.v_stride = (int64_t)vs;
+        p.pos = (const int32_t *)((const uint8_t *)rows->pos->ptr + rows->pos_offset);
+        p.seq = rows->seq ? (const int32_t *)((const uint8_t *)rows->seq->ptr + rows->seq_offset) : nullptr;
+        p.status = rows->status ? (int32_t *)((uint8_t *)rows->status->ptr + rows->status_offset) : nullptr;
+        p.rows = (int)rows->rows;
+        p.kv_dim = (int)dim;
+        p.chunks = (int)((dim + 255) / 256);
+        set_device(dev);
+        if (rows->dtype == YUUKA_DTYPE_F32) launch_move<float>(stream, p, write, cache->head_dim);
+        else if (rows->dtype == YUUKA_DTYPE_F16) launch_move<__half>(stream, p, write, cache->head_dim);
+        else launch_move<__nv_bfloat16>(stream, p, write, cache->head_dim);
+        record_completion(stream, completion);
+    });
+}
+
+}  // namespace yk
+
+extern "C" uint64_t yuuka_kv_row_bytes(int32_t format, int32_t kv_heads, int32_t head_dim) {
+    return yk::kv_row_bytes(format, kv_heads, head_dim);
+}
+
+extern "C" yuuka_status yuuka_kv_write(yuuka_stream * stream, const yuuka_kv_cache * cache, const yuuka_kv_rows * rows,
+                                       yuuka_event * completion) {
+    return yk::move_rows("kv_write", true, stream, cache, rows, completion);
+}
+
+extern "C" yuuka_status yuuka_kv_read(yuuka_stream * stream, const yuuka_kv_cache * cache, const yuuka_kv_rows * rows,
+                                      yuuka_event * completion) {
+    return yk::move_rows("kv_read", false, stream, cache, rows, completion);
+}

@@ -15,7 +15,8 @@ from . import build as _build
 
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED, ERR_DEVICE, ERR_ALLOCATION, ERR_INTERNAL = range(6)
 F32, F16, Q8_0, Q4_K, Q5_K, Q6_K, BF16 = 0, 1, 8, 12, 13, 14, 30
-KV_F32, KV_F16, KV_Q8_0 = 0, 1, 2
+KV_F32, KV_F16, KV_Q8_0, KV_F8 = 0, 1, 2, 3
+KV_STATUS_BLOCK, KV_STATUS_SEQUENCE, KV_STATUS_POSITION = 1, 2, 4
 PATH_AUTO, PATH_FP32, PATH_MMA = 0, 1, 2
 GEMM_ACCUMULATE = 1
 GEMM_TILED = 2
@@ -96,6 +97,28 @@ class VerifyBatch(C.Structure):
                 ("emitted", C.c_void_p), ("path", C.c_void_p), ("logits", C.c_void_p), ("seq_ids", C.c_void_p)]
 
 
+class KvCacheArgs(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("tables", C.c_void_p), ("k_offset", C.c_uint64), ("v_offset", C.c_uint64),
+                ("tables_offset", C.c_uint64), ("format", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("block_size", C.c_int32), ("pool_blocks", C.c_int32), ("sequences", C.c_int32), ("table_stride", C.c_int32)]
+
+
+class KvRowsArgs(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("pos", C.c_void_p), ("seq", C.c_void_p), ("status", C.c_void_p),
+                ("k_offset", C.c_uint64), ("v_offset", C.c_uint64), ("pos_offset", C.c_uint64), ("seq_offset", C.c_uint64),
+                ("status_offset", C.c_uint64), ("k_stride", C.c_uint64), ("v_stride", C.c_uint64), ("rows", C.c_uint64),
+                ("dtype", C.c_uint32)]
+
+
+class AttentionDecodeArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("gate", C.c_void_p), ("lse", C.c_void_p), ("lens", C.c_void_p),
+                ("seq_ids", C.c_void_p), ("status", C.c_void_p), ("q_offset", C.c_uint64), ("out_offset", C.c_uint64),
+                ("gate_offset", C.c_uint64), ("lse_offset", C.c_uint64), ("lens_offset", C.c_uint64),
+                ("seq_ids_offset", C.c_uint64), ("status_offset", C.c_uint64), ("q_row_stride", C.c_uint64),
+                ("q_head_stride", C.c_uint64), ("out_row_stride", C.c_uint64), ("out_head_stride", C.c_uint64),
+                ("dtype", C.c_uint32), ("batch", C.c_int32), ("heads", C.c_int32), ("window", C.c_int32), ("scale", C.c_float)]
+
+
 # name -> (restype, argtypes); the exported symbol list the ABI test checks
 _vp, _i32, _u32, _u64, _f32 = C.c_void_p, C.c_int32, C.c_uint32, C.c_uint64, C.c_float
 SIGNATURES = {
@@ -106,10 +129,12 @@ SIGNATURES = {
     "yuuka_device_info_get": (_i32, [_vp, _vp]),
     "yuuka_device_memory_get": (_i32, [_vp, _vp, _vp]),
     "yuuka_buffer_alloc": (_i32, [_vp, _u64, _vp]),
+    "yuuka_buffer_view": (_i32, [_vp, _vp, _u64, _vp]),
     "yuuka_buffer_free": (None, [_vp]),
     "yuuka_buffer_size": (_u64, [_vp]),
     "yuuka_buffer_ptr": (_vp, [_vp]),
     "yuuka_stream_create": (_i32, [_vp, _vp]),
+    "yuuka_stream_view": (_i32, [_vp, _vp, _vp]),
     "yuuka_stream_destroy": (None, [_vp]),
     "yuuka_stream_synchronize": (_i32, [_vp]),
     "yuuka_event_create": (_i32, [_vp, _vp]),
@@ -127,6 +152,12 @@ SIGNATURES = {
                                 _u32, _u32, _vp]),
     "yuuka_gemm_quant_static": (_i32, [_vp, _vp, _u64, _vp, _u64, _u32, _vp, _u64, _u32, _u64, _u64, _u64,
                                 _u32, _u32, _vp]),
+    "yuuka_kv_row_bytes": (_u64, [_i32, _i32, _i32]),
+    "yuuka_kv_write": (_i32, [_vp, _vp, _vp, _vp]),
+    "yuuka_kv_read": (_i32, [_vp, _vp, _vp, _vp]),
+    "yuuka_attention_scratch_create": (_i32, [_vp, _vp]),
+    "yuuka_attention_scratch_destroy": (None, [_vp]),
+    "yuuka_attention_decode": (_i32, [_vp, _vp, _vp, _vp, _vp]),
     "yuuka_allocator_create": (_i32, [_i32, _i32, _vp]),
     "yuuka_allocator_destroy": (None, [_vp]),
     "yuuka_allocator_acquire": (_i32, [_vp, _vp]),
@@ -244,8 +275,22 @@ class Device:
         buf.write(a)
         return buf
 
+    def view(self, device_ptr: int, nbytes: int) -> "Buffer":
+        """Device memory of another owner (a torch tensor's data_ptr(), say) as a Buffer; the owner keeps it alive."""
+        buf = Buffer.__new__(Buffer)
+        buf.dev, buf.h, buf.nbytes = self, C.c_void_p(), nbytes
+        check(lib().yuuka_buffer_view(self.h, device_ptr, nbytes, C.byref(buf.h)))
+        return buf
+
     def stream(self) -> "Stream":
         return Stream(self)
+
+    def stream_view(self, cuda_stream: int) -> "Stream":
+        """A stream of another owner (torch.cuda.current_stream().cuda_stream, say) as a Stream."""
+        s = Stream.__new__(Stream)
+        s.dev, s.h = self, C.c_void_p()
+        check(lib().yuuka_stream_view(self.h, cuda_stream, C.byref(s.h)))
+        return s
 
     def event(self) -> "Event":
         return Event(self)
@@ -343,6 +388,86 @@ def gemm_quant(stream: Stream, out: Buffer, x: Buffer, w: Buffer, n_in: int, n_o
                out_offset: int = 0, x_offset: int = 0, w_offset: int = 0, completion: Event | None = None):
     check(lib().yuuka_gemm_quant(stream.h, out.h, out_offset, x.h, x_offset, x_dtype, w.h, w_offset, w_dtype,
                                  n_in, n_out, rows, path, flags, completion.h if completion else None))
+
+
+def kv_row_bytes(fmt: int, kv_heads: int, head_dim: int) -> int:
+    return lib().yuuka_kv_row_bytes(fmt, kv_heads, head_dim)
+
+
+def _handle(x):
+    return x.h if x is not None else None
+
+
+class KvCache:
+    """yuuka_kv_cache: K and V pools and block tables in buffers of the caller. Keeps the buffers."""
+
+    def __init__(self, k: Buffer, v: Buffer, tables: Buffer, fmt: int, kv_heads: int, head_dim: int, block_size: int, pool_blocks: int,
+                 sequences: int, table_stride: int, k_offset: int = 0, v_offset: int = 0, tables_offset: int = 0):
+        self.keep = (k, v, tables)
+        self.args = KvCacheArgs(_handle(k), _handle(v), _handle(tables), k_offset, v_offset, tables_offset, fmt, kv_heads, head_dim,
+                                block_size, pool_blocks, sequences, table_stride)
+        self.ref = C.byref(self.args)
+
+
+class KvRows:
+    """yuuka_kv_rows: K and V rows of tokens, row r being position pos[r] of sequence seq[r]. Strides in elements."""
+
+    def __init__(self, k: Buffer, v: Buffer, pos: Buffer, rows: int, dtype: int = F32, seq: Buffer | None = None, k_stride: int = 0,
+                 v_stride: int = 0, k_offset: int = 0, v_offset: int = 0, pos_offset: int = 0, seq_offset: int = 0,
+                 status: Buffer | None = None, status_offset: int = 0):
+        self.keep = (k, v, pos, seq, status)
+        self.args = KvRowsArgs(_handle(k), _handle(v), _handle(pos), _handle(seq), _handle(status), k_offset, v_offset, pos_offset, seq_offset,
+                               status_offset, k_stride, v_stride, rows, dtype)
+        self.ref = C.byref(self.args)
+
+
+def kv_write(stream: Stream, cache: KvCache, rows: KvRows, completion: Event | None = None):
+    """yuuka_kv_write: the rows into the pools, in the pools' format."""
+    status = lib().yuuka_kv_write(stream.h, cache.ref, rows.ref, _handle(completion))
+    if status:
+        check(status)
+
+
+def kv_read(stream: Stream, cache: KvCache, rows: KvRows, completion: Event | None = None):
+    """yuuka_kv_read: rows of the pools as plain numbers."""
+    status = lib().yuuka_kv_read(stream.h, cache.ref, rows.ref, _handle(completion))
+    if status:
+        check(status)
+
+
+class AttentionScratch:
+    """Device memory in which attention_decode joins split sequences: one for all shapes; calls that share it are ordered."""
+
+    def __init__(self, dev: Device):
+        self.h = C.c_void_p()
+        check(lib().yuuka_attention_scratch_create(dev.h, C.byref(self.h)))
+
+    def destroy(self):
+        if self.h:
+            lib().yuuka_attention_scratch_destroy(self.h)
+            self.h = C.c_void_p()
+
+
+class DecodeArgs:
+    """yuuka_attention_decode_args: one new token's queries per sequence. Strides in elements."""
+
+    def __init__(self, q: Buffer, out: Buffer, lens: Buffer, batch: int, heads: int, dtype: int = F32, scale: float = 0.0, window: int = 0,
+                 gate: Buffer | None = None, lse: Buffer | None = None, seq_ids: Buffer | None = None, status: Buffer | None = None,
+                 q_row_stride: int = 0, q_head_stride: int = 0, out_row_stride: int = 0, out_head_stride: int = 0, q_offset: int = 0,
+                 out_offset: int = 0, gate_offset: int = 0, lse_offset: int = 0, lens_offset: int = 0, seq_ids_offset: int = 0,
+                 status_offset: int = 0):
+        self.keep = (q, out, gate, lse, lens, seq_ids, status)
+        self.args = AttentionDecodeArgs(_handle(q), _handle(out), _handle(gate), _handle(lse), _handle(lens), _handle(seq_ids), _handle(status),
+                                        q_offset, out_offset, gate_offset, lse_offset, lens_offset, seq_ids_offset, status_offset,
+                                        q_row_stride, q_head_stride, out_row_stride, out_head_stride, dtype, batch, heads, window, scale)
+        self.ref = C.byref(self.args)
+
+
+def attention_decode(stream: Stream, scratch: AttentionScratch, cache: KvCache, args: DecodeArgs, completion: Event | None = None):
+    """yuuka_attention_decode: attention of one new token per sequence over the cache."""
+    status = lib().yuuka_attention_decode(stream.h, scratch.h, cache.ref, args.ref, _handle(completion))
+    if status:
+        check(status)
 
 
 class AllocatorStats(C.Structure):
