@@ -12,9 +12,7 @@ struct yuuka_attention_scratch {
 
 namespace yk {
 
-// The largest partial of any shape: 16 columns of 256 dimensions.
-constexpr size_t DEC_PART_MAX = 16 * (256 + 2) * sizeof(float);
-static size_t scratch_joins_bytes(const yuuka_device * dev) { return ((size_t)dev->sm_count * sizeof(int4) + 255) / 256 * 256; }
+constexpr size_t DEC_COUNTER_BYTES = (DEC_COUNTERS * sizeof(int) + 255) / 256 * 256;
 
 // rows and heads of an output: either all heads of a row behind one another or all rows of a head
 static bool strides_disjoint(uint64_t rows, uint64_t row, uint64_t heads, uint64_t head, uint64_t dim) {
@@ -32,16 +30,20 @@ extern "C" yuuka_status yuuka_attention_scratch_create(yuuka_device * dev, yuuka
         YK_REQUIRE(dev, YUUKA_ERR_INVALID_ARGUMENT, "attention_scratch_create: null argument");
         set_device(dev);
         void * ptr = nullptr;
-        const size_t bytes = scratch_joins_bytes(dev) + (size_t)dev->sm_count * 2 * DEC_PART_MAX;
+        const size_t bytes = DEC_COUNTER_BYTES + DEC_CTAS * sizeof(int4) + DEC_PARTIAL_BYTES;
         const cudaError_t err = cudaMalloc(&ptr, bytes);
         if (err != cudaSuccess) {
             cudaGetLastError();
             YK_REQUIRE(false, YUUKA_ERR_ALLOCATION, "cudaMalloc(%llu) failed: %s", (unsigned long long)bytes, cudaGetErrorString(err));
         }
         auto * s = new (std::nothrow) yuuka_attention_scratch();
-        if (!s) {
+        const cudaError_t zeroed = s ? cudaMemset(ptr, 0, DEC_COUNTER_BYTES) : cudaSuccess;
+        const cudaError_t waited = s && zeroed == cudaSuccess ? cudaDeviceSynchronize() : zeroed;
+        if (!s || waited != cudaSuccess) {
             cudaFree(ptr);
-            throw std::bad_alloc();
+            delete s;
+            if (!s) throw std::bad_alloc();
+            YK_CUDA(waited);
         }
         s->dev = dev;
         s->memory = (uint8_t *)ptr;
@@ -137,12 +139,12 @@ extern "C" yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_atte
         p.dtype = (int)a->dtype;
         const double scale = a->scale != 0.0f ? (double)a->scale : 1.0 / std::sqrt((double)cache->head_dim);
         p.scale_log2 = (float)(scale * 1.4426950408889634);
-        p.joins = (int4 *)scratch->memory;
-        p.partial = (float *)(scratch->memory + scratch_joins_bytes(dev));
-        p.min_tiles = 4;
-        // tiles of a warp are counted in 32 bits
+        p.counters = (int *)scratch->memory;
+        p.joins = (int4 *)(scratch->memory + DEC_COUNTER_BYTES);
+        p.partial = (float *)(scratch->memory + DEC_COUNTER_BYTES + DEC_CTAS * sizeof(int4));
+        // tiles are counted in 31 bits
         const double tiles = (double)a->batch * cache->kv_heads * p.head_tiles * (p.cache.capacity / DEC_TILE + 1.0);
-        YK_REQUIRE(tiles / (4.0 * dev->sm_count) < 1e9, YUUKA_ERR_UNSUPPORTED, "%s: %g tiles of keys are too many for one call", op, tiles);
+        YK_REQUIRE(tiles < 2e9, YUUKA_ERR_UNSUPPORTED, "%s: %g tiles of keys are too many for one call", op, tiles);
         set_device(dev);
         switch (cache->format) {
         case YUUKA_KV_F32: launch_decode_f32(stream->s, p, cache->head_dim, cols, dev->sm_count); break;

@@ -3,7 +3,8 @@
 // Mathematics. A unit is one KV head of one row of the batch, with up to 8 NT of the query heads that share it as columns.
 // Its keys are taken 16 at a time: S^T = K Q^T (keys as the rows of the product, heads as its 8-wide columns), running
 // maximum m and sum l per head, O^T += V^T P^T. Scores live in the base-2 domain, s = (scale log2 e) q.k, and probabilities
-// carry a factor of 2^14, p = 2^(s - m + 14), so that those down to 2^-28 of the largest stay normal in f16.
+// carry a factor of 2^7, p = 2^(s - m + 7). m is the maximum when the sums were last rescaled, which they are only when a score
+// passes it by 2^8 (in the first tiles, mostly), so the largest p is 2^15 and those down to 2^-21 of 2^m stay normal in f16.
 //
 // What bounds it: the bytes of the cache, read once. The products run on mma.sync: at 148 x 23 bytes a clock (the measured
 // memory rate) they take 10 to 40 % of its issue rate, and operands go straight from the cache's own layout into fragments.
@@ -43,13 +44,20 @@ struct DecodeParams {
     int window, dtype;
     float scale_log2;  // softmax scale times log2 e
     float * partial;   // [CTAs][2][part floats]: a CTA's first and last unfinished unit
-    int4 * joins;      // [CTAs] the unit that begins in the CTA and ends in a later one: x row, y unit of the row, z last CTA (-1: none)
-    int min_tiles;     // tiles a warp takes at least
+    int4 * joins;      // units that several CTAs share: x row, y unit of the row, z first and w last CTA
+    int * counters;    // zero between calls: joins listed, CTAs of the joining kernel done
 };
 
 constexpr int DEC_TILE = 16;            // keys
-constexpr float DEC_P_LOG2 = 14.0f;     // log2 of the factor that probabilities carry
-constexpr int DEC_SMEM = 232448 - 1024; // dynamic shared memory of a CTA (the rest: the warps' records)
+#ifndef DEC_MIN_TILES
+#define DEC_MIN_TILES 1
+#endif
+constexpr int DEC_CTAS = 1024;          // at most
+constexpr size_t DEC_PARTIAL_BYTES = 8u << 20;
+enum { DEC_JOINS, DEC_DONE, DEC_COUNTERS };
+constexpr float DEC_P_LOG2 = 7.0f;      // log2 of the factor that probabilities carry
+constexpr float DEC_SLACK = 8.0f;       // log2 of what a score may pass the running maximum by before sums are rescaled
+constexpr int DEC_SMEM_SM = 233472;     // shared memory of an SM
 
 // ---- small helpers -------------------------------------------------------------------------------------------------
 
@@ -79,10 +87,14 @@ __device__ __forceinline__ float dec_exp2(float x) {
     asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-template <int BYTES> __device__ __forceinline__ void dec_copy(uint32_t dst, const uint8_t * src, bool fill) {
-    const int n = fill ? BYTES : 0;  // nothing copied: zeros
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(n), "n"(BYTES) : "memory");
+template <int BYTES> __device__ __forceinline__ void dec_copy(uint32_t dst, const uint8_t * src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+// What the tensor core's tf32 (an f32 cut off behind 10 bits of its fraction) leaves of an f32, as a tf32: rounded, since
+// the cutting alone would make all scores 2^-22 too small.
+__device__ __forceinline__ uint32_t dec_rest(uint32_t x) {
+    return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u)) + 0x1000u;
 }
 __device__ __forceinline__ void dec_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void dec_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -110,10 +122,12 @@ __device__ __forceinline__ void dec_sts(uint32_t at, uint32_t v) { asm volatile(
 __device__ __forceinline__ void dec_sts4(uint32_t at, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-// two E4M3 (the low or high half of a word) as f16 pairs
-__device__ __forceinline__ uint32_t dec_e4m3(uint32_t two) {
-    uint32_t h;
-    asm volatile("{\n\t.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\t}" : "=r"(h) : "r"(two));
+// four E4M3 as two pairs of f16
+__device__ __forceinline__ uint2 dec_e4m3(uint32_t four) {
+    uint2 h;
+    asm volatile("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
+                 : "=r"(h.x), "=r"(h.y)
+                 : "r"(four));
     return h;
 }
 // bytes 0 and 1 (PAIR 0) or 2 and 3 of x, unsigned with an offset of 128, as f16 pairs of the signed values: exact
@@ -131,7 +145,18 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     static constexpr bool IS_F32 = FMT == YUUKA_KV_F32, IS_Q8 = FMT == YUUKA_KV_Q8_0, IS_F8 = FMT == YUUKA_KV_F8;
     // lanes read what others have copied (Q8_0's words, F8's scales)
     static constexpr bool SHARED_COPIES = IS_Q8 || IS_F8;
-    static constexpr int W = HD == 256 ? 4 : 8;  // warps: 256 dimensions leave a warp 128 registers of sums and queries
+        // warps of a CTA, CTAs of an SM
+#ifndef DEC_W64
+#define DEC_W64 4
+#define DEC_R64 2
+#define DEC_W128 4
+#define DEC_R128 2
+#define DEC_W256 4
+#define DEC_R256 1
+#endif
+    static constexpr bool NARROW = NT == 2 || (IS_F32 && HD > 64);
+    static constexpr int W = NARROW ? 4 : HD == 256 ? DEC_W256 : HD == 128 ? DEC_W128 : DEC_W64;
+    static constexpr int RESIDENT = NARROW ? (HD == 256 ? 1 : 2) : HD == 256 ? DEC_R256 : HD == 128 ? DEC_R128 : DEC_R64;
     static constexpr int COLS = 8 * NT, PARTS = WIDE ? 2 : 1;
     // Q8_0: words from key to key. K: 8 or 24 modulo 32, V: 4 or 12 modulo 16, which keeps the lanes' reads on different banks
     static constexpr int Q8_K = HD == 64 ? 24 : (HD == 128 ? 40 : 88), Q8_V = HD == 64 ? 20 : (HD == 128 ? 36 : 68);
@@ -145,7 +170,7 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     // queries in registers, or in shared memory where the sums leave too few (f32: 8 heads of all dimensions, split at use)
     static constexpr bool Q_SHARED = IS_F32 || HD / 4 * NT + HD / 8 * PARTS * NT > 128;
     static constexpr int Q_BYTES = !Q_SHARED ? 0 : (IS_F32 ? 8 * HD * 4 : COLS * HD * 2 * PARTS);
-    static constexpr int WARP_BYTES = DEC_SMEM / W / 16 * 16;
+    static constexpr int WARP_BYTES = (DEC_SMEM_SM / RESIDENT - 1536) / W / 16 * 16;  // (the rest: the warps' records, what a CTA takes by itself)
     static constexpr int FIT = (WARP_BYTES - PART_BYTES - Q_BYTES) / SLOT;
     static constexpr int SLOTS = FIT > 8 ? 8 : FIT;  // K and V of a tile take one each
     static constexpr int AHEAD = SLOTS - 1;
@@ -203,37 +228,95 @@ __device__ __forceinline__ DecodeSpan decode_span(const DecodeParams & p, int b)
     return decode_span(p, b, bad);
 }
 
-// A place in the sequence of tiles.
+// A place in the sequence of tiles: the next one of unit u of row b.
 struct DecodeCursor {
-    DecodeSpan span;
-    int b, u, tile;
+    int b, u;
+    int pos, end;  // its first key; behind the unit's last key
+    int left;      // tiles of the unit from here on
+    int first, tiles, seq;  // of the row
+    __device__ __forceinline__ void row(const DecodeParams & p) {
+        const DecodeSpan s = decode_span(p, b);
+        first = s.first;
+        end = s.end;
+        tiles = s.tiles;
+        seq = s.seq;
+    }
     __device__ __forceinline__ void next(const DecodeParams & p, int units) {
-        if (++tile < span.tiles) return;
-        tile = 0;
-        if (++u < units) return;
-        u = 0;
-        if (++b < p.batch) span = decode_span(p, b);
+        pos += DEC_TILE;
+        if (--left > 0) return;
+        if (++u == units) {
+            u = 0;
+            if (++b < p.batch) row(p);
+        }
+        pos = first;
+        left = tiles;
     }
 };
 
 // ---- results -------------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ float2 dec_read2(const void * base, int64_t at, int dtype) {
-    if (dtype == YUUKA_DTYPE_F32) return *reinterpret_cast<const float2 *>(reinterpret_cast<const float *>(base) + at);
-    if (dtype == YUUKA_DTYPE_F16) return __half22float2(*reinterpret_cast<const __half2 *>(reinterpret_cast<const __half *>(base) + at));
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(reinterpret_cast<const __nv_bfloat16 *>(base) + at));
-}
-// two neighbouring values of a head's result, gated and rounded to the output's type
-__device__ __forceinline__ void dec_write2(const DecodeParams & p, int b, int head, int dim, float x, float y) {
-    if (p.gate) {
-        const float2 z = dec_read2(p.gate, b * p.q_row + head * p.q_head + dim, p.dtype);
-        x *= 1.0f / (1.0f + expf(-z.x));
-        y *= 1.0f / (1.0f + expf(-z.y));
+// N neighbouring values (2, or a multiple of 4) as words, through the read-only path: loads may be moved over stores, and no
+// branch on the type stands between them.
+template <bool WIDE, int N> struct DecodeRaw {
+    static constexpr int WORDS = WIDE ? N : N / 2;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load(const void * base, int64_t at) {
+        const uint32_t * src = reinterpret_cast<const uint32_t *>(base) + (WIDE ? at : at / 2);
+        if constexpr (WORDS == 1) w[0] = __ldg(src);
+        else if constexpr (WORDS == 2) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2 *>(src));
+            w[0] = v.x;
+            w[1] = v.y;
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src + i));
+                w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+            }
+        }
     }
+    __device__ __forceinline__ float2 pair(int i, int dtype) const {  // values 2 i and 2 i + 1
+        if constexpr (WIDE) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(w + i));
+            const float2 b = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+            return dtype == YUUKA_DTYPE_F16 ? h : b;
+        }
+    }
+};
+// the gates of N neighbouring values of a head: what the values are multiplied with
+template <bool WIDE, int N> __device__ __forceinline__ void dec_gates(const DecodeParams & p, const DecodeRaw<WIDE, N> & raw, float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) {
+        const float2 z = raw.pair(i, p.dtype);
+        // (approximate exponential and reciprocal: 2^-21 in all)
+        f[2 * i] = __fdividef(1.0f, 1.0f + __expf(-z.x));
+        f[2 * i + 1] = __fdividef(1.0f, 1.0f + __expf(-z.y));
+    }
+}
+// N neighbouring values of a head's result, rounded to the output's type
+template <bool WIDE, int N> __device__ __forceinline__ void dec_write(const DecodeParams & p, int b, int head, int dim, const float (&x)[N]) {
     const int64_t at = b * p.out_row + head * p.out_head + dim;
-    if (p.dtype == YUUKA_DTYPE_F32) *reinterpret_cast<float2 *>(reinterpret_cast<float *>(p.out) + at) = make_float2(x, y);
-    else if (p.dtype == YUUKA_DTYPE_F16) *reinterpret_cast<__half2 *>(reinterpret_cast<__half *>(p.out) + at) = __floats2half2_rn(x, y);
-    else *reinterpret_cast<__nv_bfloat162 *>(reinterpret_cast<__nv_bfloat16 *>(p.out) + at) = __floats2bfloat162_rn(x, y);
+    if constexpr (WIDE) {
+        float * dst = reinterpret_cast<float *>(p.out) + at;
+        if constexpr (N == 2) *reinterpret_cast<float2 *>(dst) = make_float2(x[0], x[1]);
+        else
+#pragma unroll
+            for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(dst + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        return;
+    }
+    uint32_t raw[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) {
+        if (p.dtype == YUUKA_DTYPE_F16) *reinterpret_cast<__half2 *>(raw + i) = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+        else *reinterpret_cast<__nv_bfloat162 *>(raw + i) = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    }
+    uint16_t * dst = reinterpret_cast<uint16_t *>(p.out) + at;
+    if constexpr (N == 2) *reinterpret_cast<uint32_t *>(dst) = raw[0];
+    else if constexpr (N == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(raw[0], raw[1]);
+    else
+#pragma unroll
+        for (int i = 0; i < N / 2; i += 4) *reinterpret_cast<uint4 *>(dst + 2 * i) = make_uint4(raw[i], raw[i + 1], raw[i + 2], raw[i + 3]);
 }
 __device__ __forceinline__ void dec_write_lse(const DecodeParams & p, int b, int head, float m, float l) {
     // (l carries the probabilities' factor)
@@ -254,13 +337,19 @@ __device__ __forceinline__ DecodeHeads decode_heads(const DecodeParams & p, int 
 
 // A chain of partials of one unit, `count` of them `stride` floats apart from `second` on, joined and written: as the unit's
 // result (final), or as one partial. Threads of a CTA take pairs of dimensions.
-template <int HD, int COLS>
+template <int HD, int COLS, bool WIDE>
 __device__ __forceinline__ void dec_join(const DecodeParams & p, const float * head, const float * second, int stride, int count, bool final,
                                          int b, int u, float * dst, int thread, int threads) {
     const DecodeHeads h = decode_heads(p, u);
     for (int i = thread; i < COLS * HD / 2; i += threads) {
         const int col = i / (HD / 2), dim = 2 * (i - col * (HD / 2));
         if (col >= h.count) continue;
+        float gate[2] = {1.0f, 1.0f};
+        if (final && p.gate) {
+            DecodeRaw<WIDE, 2> raw;
+            raw.load(p.gate, b * p.q_row + (h.first + col) * p.q_head + dim);
+            dec_gates<WIDE, 2>(p, raw, gate);
+        }
         float m = -INFINITY;
         for (int k = 0; k < count; k++) m = fmaxf(m, (k ? second + (size_t)(k - 1) * stride : head)[COLS * HD + col]);
         float l = 0.0f, x = 0.0f, y = 0.0f;
@@ -273,7 +362,7 @@ __device__ __forceinline__ void dec_join(const DecodeParams & p, const float * h
             y = fmaf(f, o.y, y);
         }
         if (final) {
-            dec_write2(p, b, h.first + col, dim, x / l, y / l);
+            dec_write<WIDE, 2>(p, b, h.first + col, dim, {x / l * gate[0], y / l * gate[1]});
             if (dim == 0) dec_write_lse(p, b, h.first + col, m, l);
         } else {
             *reinterpret_cast<float2 *>(dst + col * HD + dim) = make_float2(x, y);
@@ -288,14 +377,14 @@ __device__ __forceinline__ void dec_join(const DecodeParams & p, const float * h
 // ---- the kernel ----------------------------------------------------------------------------------------------------
 
 template <int FMT, int HD, int NT, bool WIDE>
-__global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, 1) attention_decode_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, DecodeShape<FMT, HD, NT, WIDE>::RESIDENT) attention_decode_kernel(const DecodeParams p) {
     using S = DecodeShape<FMT, HD, NT, WIDE>;
-    constexpr int W = S::W, COLS = S::COLS, SLOTS = S::SLOTS, AHEAD = S::AHEAD, CHUNKS = S::CHUNKS, DPL = S::DPL;
+    constexpr int W = S::W, COLS = S::COLS, AHEAD = S::AHEAD, CHUNKS = S::CHUNKS, DPL = S::DPL;
     extern __shared__ __align__(16) uint8_t smem[];
     // What the CTA's warps leave unfinished: a unit begun by an earlier warp (head: 1 it ends here, 2 it goes on), a unit begun
     // here (tail: 1) that goes on
-    __shared__ int head_kind[W], tail_kind[W], head_b[W], head_u[W], tail_b[W], tail_u[W];
-    __shared__ long long tail_end[W];  // tile behind the tail's unit
+    __shared__ int head_kind[W], tail_kind[W], tail_b[W], tail_u[W], head_b, head_u;
+    __shared__ unsigned tail_end[W];  // tile behind the tail's unit
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint8_t * const ring_at = smem + warp * S::RING;
     float * const head_part = reinterpret_cast<float *>(smem + W * S::RING + warp * S::PART_BYTES);
@@ -305,34 +394,32 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, 1) att
 
     // this warp's run of tiles
     const int units = p.cache.kv_heads * p.head_tiles;
-    long long total = 0;
+    unsigned total = 0;  // (below 2^31: the host has checked)
     for (int b = lane; b < p.batch; b += 32) {
         int bad;
         total += decode_span(p, b, bad).tiles;
         if (bad && p.status && blockIdx.x == 0 && warp == 0) atomicOr(p.status, bad);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= units;
-    const long long warps = (long long)gridDim.x * W;
-    const long long share = max((long long)p.min_tiles, (total + warps - 1) / warps);
-    const long long begin = ((long long)blockIdx.x * W + warp) * share;
+    total = __reduce_add_sync(0xffffffffu, total) * units;
+    const unsigned warps = gridDim.x * W;
+    const unsigned share = max((total + warps - 1) / warps, (unsigned)DEC_MIN_TILES);
+    const unsigned begin = (blockIdx.x * W + warp) * share;
     const int count = begin < total ? (int)min(share, total - begin) : 0;
+    auto scratch_at = [&](bool tail) { return p.partial + ((size_t)blockIdx.x * 2 + tail) * S::PART_FLOATS; };
 
     if (lane == 0) head_kind[warp] = tail_kind[warp] = 0;
     if (count > 0) {
         DecodeCursor use;
         {
-            long long before = 0;
-            int base = 0;
+            unsigned before = 0;
             use.b = 0;
-            for (; base < p.batch; base += 32) {  // (begin < total: some row holds it)
+            for (int base = 0; base < p.batch; base += 32) {  // (begin < total: some row holds it)
                 const int b = base + lane;
-                const long long mine = b < p.batch ? (long long)decode_span(p, b).tiles * units : 0;
-                long long sum = mine;
+                const unsigned mine = b < p.batch ? (unsigned)decode_span(p, b).tiles * units : 0;
+                unsigned sum = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+                    const unsigned v = __shfl_up_sync(0xffffffffu, sum, o);
                     if (lane >= o) sum += v;
                 }
                 const unsigned hit = __ballot_sync(0xffffffffu, before + sum > begin);
@@ -344,128 +431,134 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, 1) att
                 }
                 before += __shfl_sync(0xffffffffu, sum, 31);
             }
-            use.span = decode_span(p, use.b);
-            const long long rest = begin - before;
-            use.u = min((int)(rest / use.span.tiles), units - 1);  // (it is less, unless lengths change under the call)
-            use.tile = (int)(rest - (long long)use.u * use.span.tiles);
+            use.row(p);
+            const unsigned rest = begin - before;
+            use.u = min((int)(rest / (unsigned)use.tiles), units - 1);  // (it is less, unless lengths change under the call)
+            const int tile = min((int)rest - use.u * use.tiles, use.tiles - 1);
+            use.pos = use.first + tile * DEC_TILE;
+            use.left = use.tiles - tile;
         }
 
-        // -- copies: `ahead` is the tile whose K or V is fetched next, `slot_row` the pool row of its key lane % 16 (-1: no
-        // key there, zeros; -2: a bad block, NaN)
+        // -- copies. Keys behind the last one of a unit's last tile repeat it (their probabilities become zero), so a copy is
+        // always whole; a tile of a bad block becomes NaN, and a unit without keys copies nothing.
         DecodeCursor ahead = use;
-        int fetched = 0;  // tiles of the run whose V has been asked for
-        int slot_row = -1;
-        const int64_t head_bytes = FMT == YUUKA_KV_F32 ? HD * 4 : (FMT == YUUKA_KV_F16 ? HD * 2 : (FMT == YUUKA_KV_Q8_0 ? HD / 32 * 34 : HD));
-        int64_t head_at = 0;
+        int fetched = 0;                   // tiles of the run whose V has been asked for
+        unsigned block_of = 0, within = 0; // of key lane % 16 of the next tile
+        unsigned pool_row = 0;
+        bool copies = false;
+        const uint8_t * k_at = nullptr;    // the pools at the unit's head and this lane's piece
+        const uint8_t * v_at = nullptr;
+        const int32_t * table = nullptr;
+        const unsigned row_bytes = (unsigned)p.cache.row_bytes;
         auto look_up = [&] {
-            const int pos = ahead.span.first + ahead.tile * DEC_TILE + (lane & 15);
-            slot_row = -1;
-            if (pos < ahead.span.end) {
-                slot_row = kv_slot(p.cache, p.cache.tables + (int64_t)ahead.span.seq * p.cache.table_stride, pos);
-                if (slot_row == -2 && p.status) atomicOr(p.status, KV_BAD_BLOCK);
-            }
-            head_at = (int64_t)(ahead.u / p.head_tiles) * head_bytes;
+            if (ahead.pos >= ahead.end) return;
+            const int pos = min(ahead.pos + (lane & 15), ahead.end - 1);
+            const int page = p.cache.shift >= 0 ? pos >> p.cache.shift : pos / p.cache.block_size;
+            within = pos - page * p.cache.block_size;
+            block_of = (unsigned)__ldg(table + page);
         };
+        auto enter = [&] {  // the unit that `ahead` has come to
+            const int kv_head = ahead.u / p.head_tiles;
+            constexpr int HEAD_BYTES = FMT == YUUKA_KV_F32 ? HD * 4 : (FMT == YUUKA_KV_F16 ? HD * 2 : (FMT == YUUKA_KV_Q8_0 ? HD / 32 * 34 : HD));
+            const int64_t at = (int64_t)kv_head * HEAD_BYTES;
+            k_at = p.cache.k + at + (S::IS_Q8 ? 4 * (lane & 7) : 16 * t);
+            v_at = p.cache.v + at + (S::IS_Q8 ? 4 * (lane & 7) : (S::IS_F8 ? S::F8_V : 16) * g);
+            table = p.cache.tables + (int64_t)max(ahead.seq, 0) * p.cache.table_stride;
+        };
+        enter();
         look_up();
-        auto row_of = [&](const uint8_t * pool, int key, int & row) {
-            row = __shfl_sync(0xffffffffu, slot_row, key);
-            return pool + (int64_t)max(row, 0) * p.cache.row_bytes + head_at;
-        };
-        auto fetch = [&](auto is_v, int slot) {
+        uint32_t put = ring;  // slot that is filled next
+        auto fetch = [&](auto is_v) {
             constexpr bool V = decltype(is_v)::value;
-            const uint8_t * pool = V ? p.cache.v : p.cache.k;
-            const uint32_t base = ring + slot * S::SLOT;
             if (fetched < count) {
-                if constexpr (FMT == YUUKA_KV_Q8_0) {
-                    constexpr int WORDS = HD / 32 * 34 / 4;
-                    const int l8 = lane & 7;
-#pragma unroll
-                    for (int kg = 0; kg < 4; kg++) {
-                        const int key = 4 * kg + (lane >> 3);
-                        int row;
-                        const uint8_t * src = row_of(pool, key, row) + 4 * l8;
-                        const uint32_t dst = base + 4 * (V ? key * S::Q8_V : key * S::Q8_K + 1) + 4 * l8;
-#pragma unroll
-                        for (int i = 0; i < (WORDS + 7) / 8; i++) {
-                            const int w = 8 * i + l8;
-                            // K: one word between the pairs of blocks (17 words), so that lanes read two aligned words
-                            const int gap = V ? 0 : (w >= 17) + (w >= 34) + (w >= 51);
-                            if (w < WORDS) {
-                                if (row == -2) dec_sts(dst + 32 * i + 4 * gap, 0xffffffffu);
-                                else dec_copy<4>(dst + 32 * i + 4 * gap, src + 32 * i, row >= 0);
-                            }
+                if constexpr (!V) {
+                    copies = false;
+                    if (ahead.pos < ahead.end) {
+                        copies = !__any_sync(0xffffffffu, block_of >= (unsigned)p.cache.pool_blocks);
+                        pool_row = block_of * (unsigned)p.cache.block_size + within;
+                        if (!copies) {
+                            if (lane == 0 && p.status) atomicOr(p.status, KV_BAD_BLOCK);
+                            for (uint32_t at = put + 16 * lane; at < put + S::SLOT; at += 512) dec_sts4(at, make_uint4(~0u, ~0u, ~0u, ~0u));
                         }
                     }
-                } else if constexpr (!V) {
-                    constexpr int PIECES = S::K_BYTES / 1024;  // 16 bytes of keys g and g + 8, per lane
-                    int r0, r1;
-                    const uint8_t * s0 = row_of(pool, g, r0) + 16 * t;
-                    const uint8_t * s1 = row_of(pool, g + 8, r1) + 16 * t;
-                    const uint32_t dst = base + lane * 16;
+                }
+                if (copies) {
+                    auto row_of = [&](int key) { return (V ? v_at : k_at) + (uint64_t)__shfl_sync(0xffffffffu, pool_row, key) * row_bytes; };
+                    if constexpr (S::IS_Q8) {
+                        constexpr int WORDS = HD / 32 * 34 / 4;
+                        const int l8 = lane & 7;
 #pragma unroll
-                    for (int i = 0; i < PIECES; i++) {
-                        if (r0 != -2) dec_copy<16>(dst + 1024 * i, s0 + 64 * i, r0 >= 0);
-                        else dec_sts4(dst + 1024 * i, make_uint4(~0u, ~0u, ~0u, ~0u));
-                        if (r1 != -2) dec_copy<16>(dst + 1024 * i + 512, s1 + 64 * i, r1 >= 0);
-                        else dec_sts4(dst + 1024 * i + 512, make_uint4(~0u, ~0u, ~0u, ~0u));
-                    }
-                    if constexpr (FMT == YUUKA_KV_F8) {
-                        // scales: lanes 0-15 of K, 16-31 of V
-                        const int kv_head = ahead.u / p.head_tiles;
-                        const uint8_t * src = (lane < 16 ? p.cache.k : p.cache.v) + (int64_t)max(slot_row, 0) * p.cache.row_bytes +
-                                              (int64_t)p.cache.kv_heads * HD + 4 * kv_head;
-                        if (slot_row == -2) dec_sts(base + HD * 16 + 4 * lane, 0x7fffffffu);
-                        else dec_copy<4>(base + HD * 16 + 4 * lane, src, slot_row >= 0);
-                    }
-                } else {
-                    constexpr int PIECE = FMT == YUUKA_KV_F8 ? S::F8_V : 16;  // a lane's bytes of keys 2t, 2t + 1, 2t + 8, 2t + 9
-                    constexpr int PIECES = S::V_BYTES / (128 * PIECE);
-                    const uint32_t dst = base + lane * PIECE;
+                        for (int kg = 0; kg < 4; kg++) {
+                            const int key = 4 * kg + (lane >> 3);
+                            const uint8_t * src = row_of(key);
+                            const uint32_t dst = put + 4 * (V ? key * S::Q8_V : key * S::Q8_K + 1) + 4 * l8;
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        int row;
-                        const uint8_t * src = row_of(pool, 2 * t + (k & 1) + 8 * (k >> 1), row) + PIECE * g;
+                            for (int i = 0; i < (WORDS + 7) / 8; i++) {
+                                const int w = 8 * i + l8;
+                                // K: one word between the pairs of blocks (17 words), so that lanes read two aligned words
+                                const int gap = V ? 0 : (w >= 17) + (w >= 34) + (w >= 51);
+                                if (8 * i + 7 < WORDS || w < WORDS) dec_copy<4>(dst + 32 * i + 4 * gap, src + 32 * i);
+                            }
+                        }
+                    } else if constexpr (!V) {
+                        constexpr int PIECES = S::K_BYTES / 1024;  // 16 bytes of keys g and g + 8, per lane
+                        const uint8_t * s0 = row_of(g);
+                        const uint8_t * s1 = row_of(g + 8);
+                        const uint32_t dst = put + lane * 16;
 #pragma unroll
                         for (int i = 0; i < PIECES; i++) {
-                            const uint32_t to = dst + (i * 4 + k) * 32 * PIECE;
-                            if (row != -2) dec_copy<PIECE>(to, src + 8 * PIECE * i, row >= 0);
-                            else
-                                for (int w = 0; w < PIECE; w += 4) dec_sts(to + w, ~0u);
+                            dec_copy<16>(dst + 1024 * i, s0 + 64 * i);
+                            dec_copy<16>(dst + 1024 * i + 512, s1 + 64 * i);
+                        }
+                        if constexpr (FMT == YUUKA_KV_F8) {
+                            // scales: lanes 0-15 of K, 16-31 of V
+                            const uint8_t * src = (lane < 16 ? p.cache.k : p.cache.v) + (uint64_t)pool_row * row_bytes +
+                                                  (p.cache.kv_heads * HD + 4 * (ahead.u / p.head_tiles));
+                            dec_copy<4>(put + HD * 16 + 4 * lane, src);
+                        }
+                    } else {
+                        constexpr int PIECE = FMT == YUUKA_KV_F8 ? S::F8_V : 16;  // a lane's bytes of keys 2t, 2t + 1, 2t + 8, 2t + 9
+                        constexpr int PIECES = S::V_BYTES / (128 * PIECE);
+                        const uint32_t dst = put + lane * PIECE;
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint8_t * src = row_of(2 * t + (k & 1) + 8 * (k >> 1));
+#pragma unroll
+                            for (int i = 0; i < PIECES; i++) dec_copy<PIECE>(dst + (i * 4 + k) * 32 * PIECE, src + 8 * PIECE * i);
                         }
                     }
                 }
                 if constexpr (V) {
-                    fetched++;
-                    if (fetched < count) {
+                    if (++fetched < count) {
+                        const bool other = ahead.left == 1;
                         ahead.next(p, units);
+                        if (other) enter();
                         look_up();
                     }
                 }
             }
+            put = put + S::SLOT == ring + S::RING ? ring : put + S::SLOT;
             dec_commit();
         };
-        int put = 0;  // slot that is filled next
-        auto fetch_next = [&](auto is_v) {
-            fetch(is_v, put);
-            put = put + 1 == SLOTS ? 0 : put + 1;
-        };
-#pragma unroll
-        for (int i = 0; i < AHEAD; i++) {
-            if (i & 1) fetch_next(std::true_type());
-            else fetch_next(std::false_type());
+#pragma unroll 1
+        for (int i = 0; i < AHEAD / 2; i++) {
+            fetch(std::false_type());
+            fetch(std::true_type());
         }
+        if constexpr (AHEAD & 1) fetch(std::false_type());
 
         // -- per unit: queries, statistics and sums
         constexpr int QM = HD / 16;  // 16-bit products over the head dimension
         uint32_t q[S::Q_SHARED ? 1 : NT][S::Q_SHARED ? 1 : S::PARTS][S::Q_SHARED ? 1 : QM][2];
-        float scale[NT][2];          // of the columns' scores
+        float scale[NT][2];          // of the columns' scores, not negative: a negative scale's sign goes into the queries
         float m[NT][2], l[NT][2];    // l: of this lane's keys
         float o[NT][CHUNKS][DPL / 2][4];
         float v_scale = 1.0f;        // Q8_0, F8: o is in units of it (a power of two)
-        bool from_start = false;
+        bool from_start = false, fresh = true;
 
         auto load_queries = [&] {
             const DecodeHeads h = decode_heads(p, use.u);
+            const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 const int col = nt * 8 + g;
@@ -473,26 +566,32 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, 1) att
                 const int64_t at = use.b * p.q_row + (h.first + (has ? col : 0)) * p.q_head;
                 if constexpr (S::IS_F32) {
                     // dimensions 16 i + 4 t .. + 3 of head g
-#pragma unroll 4
+                    DecodeRaw<WIDE, 4> raw[HD / 16];
+#pragma unroll
+                    for (int i = 0; i < HD / 16; i++) raw[i].load(p.q, at + 16 * i + 4 * t);
+                    const float f = has ? sign : 0.0f;
+#pragma unroll
                     for (int i = 0; i < HD / 16; i++) {
-                        const float2 x = has ? dec_read2(p.q, at + 16 * i + 4 * t, p.dtype) : make_float2(0.f, 0.f);
-                        const float2 y = has ? dec_read2(p.q, at + 16 * i + 4 * t + 2, p.dtype) : make_float2(0.f, 0.f);
-                        dec_sts4(q_at + 512 * i, make_uint4(__float_as_uint(x.x), __float_as_uint(x.y), __float_as_uint(y.x), __float_as_uint(y.y)));
+                        const float2 x = raw[i].pair(0, p.dtype), y = raw[i].pair(1, p.dtype);
+                        dec_sts4(q_at + 512 * i, make_uint4(__float_as_uint(x.x * f), __float_as_uint(x.y * f), __float_as_uint(y.x * f), __float_as_uint(y.y * f)));
                     }
-                    scale[nt][0] = scale[nt][1] = p.scale_log2;
+                    scale[nt][0] = scale[nt][1] = fmaxf(fabsf(p.scale_log2), 1e-37f);
                 } else {
                     // scaled to a largest magnitude of 2^14 .. 2^15, so that two f16 parts hold 22 bits of what matters
+                    DecodeRaw<WIDE, 2> raw[2 * QM];
+#pragma unroll
+                    for (int i = 0; i < 2 * QM; i++) raw[i].load(p.q, at + S::q_dim(i >> 1, i & 1, t));
                     float amax = 0.0f;
-#pragma unroll 4
+#pragma unroll
                     for (int i = 0; i < 2 * QM; i++) {
-                        const float2 x = has ? dec_read2(p.q, at + S::q_dim(i >> 1, i & 1, t), p.dtype) : make_float2(0.f, 0.f);
+                        const float2 x = raw[i].pair(0, p.dtype);
                         amax = fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y)));
                     }
                     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                     const int e = min(max((int)(__float_as_uint(amax) >> 23), 15), 254);
-                    const float up = __int_as_float((268 - e) << 23);                        // 2^(14 - (e - 127))
-                    const float down = p.scale_log2 * __int_as_float((e - 14) << 23);        // scale / up
+                    const float up = has ? sign * __int_as_float((268 - e) << 23) : 0.0f;                          // 2^(14 - (e - 127))
+                    const float down = fmaxf(fabsf(p.scale_log2) * __int_as_float((e - 14) << 23), 1e-37f);        // |scale| / up
                     scale[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
                     scale[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
 #pragma unroll
@@ -500,7 +599,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, 1) att
                         uint32_t hi[2], lo[2];
 #pragma unroll
                         for (int half = 0; half < 2; half++) {
-                            float2 x = has ? dec_read2(p.q, at + S::q_dim(i, half, t), p.dtype) : make_float2(0.f, 0.f);
+                            float2 x = raw[2 * i + half].pair(0, p.dtype);
                             x.x *= up;
                             x.y *= up;
                             hi[half] = dec_pack(x.x, x.y);
@@ -568,27 +667,43 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, 1) att
                 rescale(f);
                 v_scale = v;
             }
-            return 1.0f / v_scale;
+            return __fdividef(1.0f, v_scale);  // (exact: a power of two)
+        };
+        // o += a P^T for product j of a chunk. The tensor core cuts sums off instead of rounding them: over thousands of tiles
+        // that would cost an f32 result 2^-17, so such a tile is summed on its own and added in f32
+        auto add_values = [&](float (&acc)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[S::PARTS][2]) {
+            if constexpr (WIDE) {
+                float d[4] = {0.f, 0.f, 0.f, 0.f};
+                dec_mma16(d, a0, a1, a2, a3, b[1][0], b[1][1]);
+                dec_mma16(d, a0, a1, a2, a3, b[0][0], b[0][1]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[e] += d[e];
+            } else {
+                dec_mma16(acc, a0, a1, a2, a3, b[0][0], b[0][1]);
+            }
         };
 
-        int take = 0;  // slot that is used next
+        uint32_t take = ring;  // slot that is used next
+#pragma unroll 1
         for (int it = 0; it < count; it++) {
             // ---- K: scores
             dec_wait<AHEAD - 1>();
             if constexpr (S::SHARED_COPIES) __syncwarp();
-            if constexpr (AHEAD & 1) fetch_next(std::true_type());
-            else fetch_next(std::false_type());
-            const uint32_t ks = ring + take * S::SLOT;
-            take = take + 1 == SLOTS ? 0 : take + 1;
+            if constexpr (AHEAD & 1) fetch(std::true_type());
+            else fetch(std::false_type());
+            const uint32_t ks = take;
+            take = take + S::SLOT == ring + S::RING ? ring : take + S::SLOT;
 
-            if (it == 0 || use.tile == 0) {
-                from_start = use.tile == 0;
+            if (fresh) {
+                fresh = false;
+                from_start = use.left == use.tiles;
                 load_queries();
                 v_scale = __uint_as_float(0x00800000u);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     m[nt][0] = m[nt][1] = -INFINITY;
-                    l[nt][0] = l[nt][1] = 0.0f;
+                    // (a row that is out of range has no keys and becomes NaN)
+                    l[nt][0] = l[nt][1] = use.seq < 0 ? __uint_as_float(0x7fffffffu) : 0.0f;
 #pragma unroll
                     for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
@@ -596,102 +711,112 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, 1) att
 #pragma unroll
                             for (int e = 0; e < 4; e++) o[nt][c][j][e] = 0.0f;
                 }
-                // a row that is out of range: everything becomes NaN
-                if (use.span.seq < 0)
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) l[nt][0] = l[nt][1] = __uint_as_float(0x7fffffffu);
             }
-            const int keys = min(DEC_TILE, use.span.end - use.span.first - use.tile * DEC_TILE);  // 0 for a row without any
+            const int keys = use.end - use.pos;  // of the unit from here on; 0 for a row without any
 
+            uint32_t pb[NT][S::PARTS][2];  // probabilities as fragments: keys become the dimension that is summed over
             float s[NT][4];
+            auto fragments = [&](float f0, float f1) {  // with factors of keys g and g + 8
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[nt][e] = 0.0f;
-            if constexpr (S::IS_F32) {
-                // three products of tf32 parts: hi hi, hi lo, lo hi
-                float s2[NT][4] = {};
-#pragma unroll
-                for (int c = 0; c < HD / 16; c++) {
-                    const uint4 ka = dec_lds4(ks + lane * 16 + 1024 * c), kb = dec_lds4(ks + lane * 16 + 1024 * c + 512);
-                    const uint4 f = dec_lds4(q_at + 512 * c);
-                    const uint32_t a[8] = {ka.x, kb.x, ka.y, kb.y, ka.z, kb.z, ka.w, kb.w};
-                    const uint32_t b[4] = {f.x, f.y, f.z, f.w};
-                    uint32_t ah[8], al[8], bh[4], bl[4];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        ah[i] = a[i] & 0xffffe000u;
-                        al[i] = __float_as_uint(__uint_as_float(a[i]) - __uint_as_float(ah[i]));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        bh[i] = b[i] & 0xffffe000u;
-                        bl[i] = __float_as_uint(__uint_as_float(b[i]) - __uint_as_float(bh[i]));
-                    }
-                    dec_mma8(s[0], ah[0], ah[1], ah[2], ah[3], bh[0], bh[1]);
-                    dec_mma8(s2[0], ah[4], ah[5], ah[6], ah[7], bh[2], bh[3]);
-                    dec_mma8(s[0], al[0], al[1], al[2], al[3], bh[0], bh[1]);
-                    dec_mma8(s2[0], al[4], al[5], al[6], al[7], bh[2], bh[3]);
-                    if constexpr (WIDE) {  // (16-bit queries have no second part)
-                        dec_mma8(s[0], ah[0], ah[1], ah[2], ah[3], bl[0], bl[1]);
-                        dec_mma8(s2[0], ah[4], ah[5], ah[6], ah[7], bl[2], bl[3]);
+                for (int nt = 0; nt < NT; nt++) {
+                    const float x0 = s[nt][0] * f0, x1 = s[nt][1] * f0, y0 = s[nt][2] * f1, y1 = s[nt][3] * f1;
+                    const uint32_t hx = dec_pack(x0, x1), hy = dec_pack(y0, y1);
+                    pb[nt][0][0] = dec_transpose(hx);
+                    pb[nt][0][1] = dec_transpose(hy);
+                    if constexpr (WIDE) {
+                        const float2 rx = dec_unpack(hx), ry = dec_unpack(hy);
+                        pb[nt][1][0] = dec_transpose(dec_pack(x0 - rx.x, x1 - rx.y));
+                        pb[nt][1][1] = dec_transpose(dec_pack(y0 - ry.x, y1 - ry.y));
                     }
                 }
+            };
+            if (keys > 0) {  // (uniform)
+                float s2[NT][4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[0][e] += s2[0][e];
-            } else if constexpr (S::IS_Q8) {
-                const uint32_t ka = ks + 4 * (g * S::Q8_K + 1), kb = ka + 32 * S::Q8_K;  // keys g and g + 8
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int pair = 0; pair < HD / 64; pair++) {
-                    uint32_t w[2][4];   // [key][word]: two of the even block, two of the odd one
-                    float d[2][2];      // [key][block]
+                    for (int e = 0; e < 4; e++) s[nt][e] = s2[nt][e] = 0.0f;
+                if constexpr (S::IS_F32) {
+                    // three products of tf32 parts: hi hi, hi lo, lo hi (the tensor core itself drops what a first part leaves)
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const uint32_t at = (k ? kb : ka) + 72 * pair;
-                        const uint2 even = dec_lds2(at + 4 * (1 + 2 * t)), odd = dec_lds2(at + 4 * (9 + 2 * t));
-                        const uint32_t w0 = dec_lds(at), w8 = dec_lds(at + 32);
-                        d[k][0] = __half2float(__ushort_as_half((unsigned short)w0));
-                        d[k][1] = __half2float(__ushort_as_half((unsigned short)(w8 >> 16)));
-                        w[k][0] = even.x ^ 0x80808080u;
-                        // word 8 is the block's last two values and the next scale: its first two are in word 0
-                        w[k][1] = (t == 3 ? __byte_perm(w8, w0, 0x7610) : even.y) ^ 0x80808080u;
-                        w[k][2] = odd.x ^ 0x80808080u;
-                        w[k][3] = odd.y ^ 0x80808080u;
+                    for (int c = 0; c < HD / 16; c++) {
+                        const uint4 ka = dec_lds4(ks + lane * 16 + 1024 * c), kb = dec_lds4(ks + lane * 16 + 1024 * c + 512);
+                        const uint4 f = dec_lds4(q_at + 512 * c);
+                        const uint32_t a[8] = {ka.x, kb.x, ka.y, kb.y, ka.z, kb.z, ka.w, kb.w};
+                        const uint32_t b[4] = {f.x, f.y, f.z, f.w};
+                        uint32_t al[8], bl[4];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) al[i] = dec_rest(a[i]);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) bl[i] = dec_rest(b[i]);
+                        dec_mma8(s[0], a[0], a[1], a[2], a[3], b[0], b[1]);
+                        dec_mma8(s2[0], a[4], a[5], a[6], a[7], b[2], b[3]);
+                        dec_mma8(s[0], al[0], al[1], al[2], al[3], b[0], b[1]);
+                        dec_mma8(s2[0], al[4], al[5], al[6], al[7], b[2], b[3]);
+                        if constexpr (WIDE) {  // (16-bit queries have no second part)
+                            dec_mma8(s[0], a[0], a[1], a[2], a[3], bl[0], bl[1]);
+                            dec_mma8(s2[0], a[4], a[5], a[6], a[7], bl[2], bl[3]);
+                        }
                     }
+                } else if constexpr (S::IS_Q8) {
+                    const uint32_t ka = ks + 4 * (g * S::Q8_K + 1), kb = ka + 32 * S::Q8_K;  // keys g and g + 8
 #pragma unroll
-                    for (int blk = 0; blk < 2; blk++)
+                    for (int pair = 0; pair < HD / 64; pair++) {
+                        uint32_t w[2][4];   // [key][word]: two of the even block, two of the odd one
+                        float d[2][2];      // [key][block]
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            float x[4] = {0.f, 0.f, 0.f, 0.f};
+                        for (int k = 0; k < 2; k++) {
+                            const uint32_t at = (k ? kb : ka) + 72 * pair;
+                            const uint2 even = dec_lds2(at + 4 * (1 + 2 * t)), odd = dec_lds2(at + 4 * (9 + 2 * t));
+                            const uint32_t w0 = dec_lds(at), w8 = dec_lds(at + 32);
+                            d[k][0] = __half2float(__ushort_as_half((unsigned short)w0));
+                            d[k][1] = __half2float(__ushort_as_half((unsigned short)(w8 >> 16)));
+                            w[k][0] = even.x ^ 0x80808080u;
+                            // word 8 is the block's last two values and the next scale: its first two are in word 0
+                            w[k][1] = (t == 3 ? __byte_perm(w8, w0, 0x7610) : even.y) ^ 0x80808080u;
+                            w[k][2] = odd.x ^ 0x80808080u;
+                            w[k][3] = odd.y ^ 0x80808080u;
+                        }
+#pragma unroll
+                        for (int blk = 0; blk < 2; blk++) {
+                            uint32_t a[2][4];
 #pragma unroll
                             for (int h = 0; h < 2; h++) {
                                 const uint32_t u0 = w[0][2 * blk + h], u1 = w[1][2 * blk + h];
-                                const uint32_t a0 = dec_int8<0>(u0), a1 = dec_int8<0>(u1), a2 = dec_int8<1>(u0), a3 = dec_int8<1>(u1);
-                                const uint4 f = query(nt, 4 * pair + 2 * blk + h);
-                                dec_mma16(x, a0, a1, a2, a3, f.x, f.y);
-                                if constexpr (WIDE) dec_mma16(x, a0, a1, a2, a3, f.z, f.w);
+                                a[h][0] = dec_int8<0>(u0);
+                                a[h][1] = dec_int8<0>(u1);
+                                a[h][2] = dec_int8<1>(u0);
+                                a[h][3] = dec_int8<1>(u1);
                             }
-                            s[nt][0] = fmaf(x[0], d[0][blk], s[nt][0]);
-                            s[nt][1] = fmaf(x[1], d[0][blk], s[nt][1]);
-                            s[nt][2] = fmaf(x[2], d[1][blk], s[nt][2]);
-                            s[nt][3] = fmaf(x[3], d[1][blk], s[nt][3]);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                for (int h = 0; h < 2; h++) {
+                                    const uint4 f = query(nt, 4 * pair + 2 * blk + h);
+                                    if constexpr (WIDE) dec_mma16(x, a[h][0], a[h][1], a[h][2], a[h][3], f.z, f.w);
+                                    dec_mma16(x, a[h][0], a[h][1], a[h][2], a[h][3], f.x, f.y);
+                                }
+                                s[nt][0] = fmaf(x[0], d[0][blk], s[nt][0]);
+                                s[nt][1] = fmaf(x[1], d[0][blk], s[nt][1]);
+                                s[nt][2] = fmaf(x[2], d[1][blk], s[nt][2]);
+                                s[nt][3] = fmaf(x[3], d[1][blk], s[nt][3]);
+                            }
                         }
-                }
-            } else {
-                float s2[NT][4] = {};
-                if constexpr (S::IS_F8) {
+                    }
+                } else if constexpr (S::IS_F8) {
 #pragma unroll
                     for (int c = 0; c < HD / 64; c++) {
                         const uint4 ka = dec_lds4(ks + lane * 16 + 1024 * c), kb = dec_lds4(ks + lane * 16 + 1024 * c + 512);
                         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const uint32_t a0 = dec_e4m3(wa[i]), a1 = dec_e4m3(wb[i]), a2 = dec_e4m3(wa[i] >> 16), a3 = dec_e4m3(wb[i] >> 16);
+                            const uint2 x = dec_e4m3(wa[i]), y = dec_e4m3(wb[i]);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
                                 const uint4 f = query(nt, 4 * c + i);
-                                dec_mma16((i & 1) ? s2[nt] : s[nt], a0, a1, a2, a3, f.x, f.y);
-                                if constexpr (WIDE) dec_mma16((i & 1) ? s2[nt] : s[nt], a0, a1, a2, a3, f.z, f.w);
+                                dec_mma16((i & 1) ? s2[nt] : s[nt], x.x, y.x, x.y, y.y, f.x, f.y);
+                                if constexpr (WIDE) dec_mma16((i & 1) ? s2[nt] : s[nt], x.x, y.x, x.y, y.y, f.z, f.w);
                             }
                         }
                     }
@@ -711,222 +836,208 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, 1) att
                         }
                     }
                 }
+                if constexpr (!S::IS_Q8)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[nt][e] += s2[nt][e];
-            }
-            float vd[2] = {1.0f, 1.0f};  // F8: scales of V of keys g and g + 8
-            if constexpr (S::IS_F8) {
-                const float d0 = __uint_as_float(dec_lds(ks + HD * 16 + 4 * g)), d1 = __uint_as_float(dec_lds(ks + HD * 16 + 4 * (g + 8)));
-                vd[0] = __uint_as_float(dec_lds(ks + HD * 16 + 64 + 4 * g));
-                vd[1] = __uint_as_float(dec_lds(ks + HD * 16 + 64 + 4 * (g + 8)));
+                        for (int e = 0; e < 4; e++) s[nt][e] += s2[nt][e];
+                float vd[2] = {1.0f, 1.0f};  // F8: scales of V of keys g and g + 8
+                if constexpr (S::IS_F8) {
+                    const float d0 = __uint_as_float(dec_lds(ks + HD * 16 + 4 * g)), d1 = __uint_as_float(dec_lds(ks + HD * 16 + 4 * (g + 8)));
+                    vd[0] = __uint_as_float(dec_lds(ks + HD * 16 + 64 + 4 * g));
+                    vd[1] = __uint_as_float(dec_lds(ks + HD * 16 + 64 + 4 * (g + 8)));
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    s[nt][0] *= d0;
-                    s[nt][1] *= d0;
-                    s[nt][2] *= d1;
-                    s[nt][3] *= d1;
+                    for (int nt = 0; nt < NT; nt++) {
+                        s[nt][0] *= d0;
+                        s[nt][1] *= d0;
+                        s[nt][2] *= d1;
+                        s[nt][3] *= d1;
+                    }
                 }
-            }
 
-            // ---- running maximum and sum; s becomes the probabilities of keys g (0, 1) and g + 8 (2, 3), columns 2t and 2t + 1
-            if (keys > 0) {  // (uniform)
-                float corr[NT][2];
+                // ---- running maximum and sum; s becomes the probabilities of keys g (0, 1) and g + 8 (2, 3), columns 2t and 2t + 1
+                if (keys < DEC_TILE) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (g + 8 * (e >> 1) >= keys) s[nt][e] = -INFINITY;
+                }
+                float top[NT][2];
                 bool moved = false;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[nt][e] = (g + 8 * (e >> 1) < keys) ? s[nt][e] * scale[nt][e & 1] : -INFINITY;
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         float mx = fmaxf(s[nt][c], s[nt][c + 2]);
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float top = fmaxf(m[nt][c], mx);
-                        corr[nt][c] = dec_exp2(m[nt][c] - top);
-                        moved |= top > m[nt][c];
-                        m[nt][c] = top;
-                        s[nt][c] = dec_exp2(s[nt][c] - top + DEC_P_LOG2);
-                        s[nt][c + 2] = dec_exp2(s[nt][c + 2] - top + DEC_P_LOG2);
-                        l[nt][c] = fmaf(l[nt][c], corr[nt][c], s[nt][c] + s[nt][c + 2]);
+                        top[nt][c] = fmaxf(m[nt][c], mx * scale[nt][c]);
+                        moved |= top[nt][c] > m[nt][c] + DEC_SLACK;
                     }
+                if (__any_sync(0xffffffffu, moved)) {
+                    float corr[NT][2];
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            corr[nt][c] = dec_exp2(m[nt][c] - top[nt][c]);
+                            l[nt][c] *= corr[nt][c];
+                            m[nt][c] = top[nt][c];
+                        }
+                    rescale(corr);
                 }
-                if (__any_sync(0xffffffffu, moved)) rescale(corr);
-            } else {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) s[nt][e] = 0.0f;
-            }
-            // probabilities as fragments: keys become the dimension that is summed over
-            uint32_t pb[NT][S::PARTS][2];
-            auto fragments = [&](float f0, float f1) {  // with factors of keys g and g + 8
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const float x0 = s[nt][0] * f0, x1 = s[nt][1] * f0, y0 = s[nt][2] * f1, y1 = s[nt][3] * f1;
-                    const uint32_t hx = dec_pack(x0, x1), hy = dec_pack(y0, y1);
-                    pb[nt][0][0] = dec_transpose(hx);
-                    pb[nt][0][1] = dec_transpose(hy);
-                    if constexpr (WIDE) {
-                        const float2 rx = dec_unpack(hx), ry = dec_unpack(hy);
-                        pb[nt][1][0] = dec_transpose(dec_pack(x0 - rx.x, x1 - rx.y));
-                        pb[nt][1][1] = dec_transpose(dec_pack(y0 - ry.x, y1 - ry.y));
+                    for (int c = 0; c < 2; c++) {
+                        const float base = DEC_P_LOG2 - m[nt][c];
+                        s[nt][c] = dec_exp2(fmaf(s[nt][c], scale[nt][c], base));
+                        s[nt][c + 2] = dec_exp2(fmaf(s[nt][c + 2], scale[nt][c], base));
+                        l[nt][c] += s[nt][c] + s[nt][c + 2];
                     }
+                if constexpr (FMT == YUUKA_KV_F16) fragments(1.0f, 1.0f);
+                else if constexpr (S::IS_F8) {
+                    const float inv = take_v_scale(max(__float_as_uint(fabsf(vd[0])), __float_as_uint(fabsf(vd[1]))));
+                    fragments(vd[0] * inv, vd[1] * inv);
                 }
-            };
-            if constexpr (FMT == YUUKA_KV_F16) fragments(1.0f, 1.0f);
-            else if constexpr (S::IS_F8) {
-                const float inv = take_v_scale(max(__float_as_uint(fabsf(vd[0])), __float_as_uint(fabsf(vd[1]))));
-                fragments(vd[0] * inv, vd[1] * inv);
             }
 
             // ---- V: sums
             dec_wait<AHEAD - 1>();
             if constexpr (S::SHARED_COPIES) __syncwarp();
-            if constexpr (AHEAD & 1) fetch_next(std::false_type());
-            else fetch_next(std::true_type());
-            const uint32_t vs = ring + take * S::SLOT;
-            take = take + 1 == SLOTS ? 0 : take + 1;
+            if constexpr (AHEAD & 1) fetch(std::false_type());
+            else fetch(std::true_type());
+            const uint32_t vs = take;
+            take = take + S::SLOT == ring + S::RING ? ring : take + S::SLOT;
 
-            if constexpr (S::IS_F32) {
-                // probabilities in f32 change hands as two 16-bit halves; lane (g, t) then has keys 2t, 2t + 1 (and + 8) of column g
-                float pk[4];
+            if (keys > 0) {
+                if constexpr (S::IS_F32) {
+                    // probabilities in f32 change hands as two 16-bit halves; lane (g, t) then has keys 2t, 2t + 1 (and + 8) of column g
+                    uint32_t pk[4], pl[4];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t x = __float_as_uint(s[0][2 * h]), y = __float_as_uint(s[0][2 * h + 1]);
-                    const uint32_t low = dec_transpose(__byte_perm(x, y, 0x5410)), high = dec_transpose(__byte_perm(x, y, 0x7632));
-                    pk[2 * h] = __uint_as_float(__byte_perm(low, high, 0x5410));
-                    pk[2 * h + 1] = __uint_as_float(__byte_perm(low, high, 0x7632));
-                }
-                uint32_t ph[4], pl[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    ph[i] = __float_as_uint(pk[i]) & 0xffffe000u;
-                    pl[i] = __float_as_uint(pk[i] - __uint_as_float(ph[i]));
-                }
-#pragma unroll
-                for (int c = 0; c < CHUNKS; c++) {
-                    uint32_t v[4][4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint4 r = dec_lds4(vs + lane * 16 + (c * 4 + k) * 512);
-                        v[k][0] = r.x; v[k][1] = r.y; v[k][2] = r.z; v[k][3] = r.w;
+                    for (int h = 0; h < 2; h++) {
+                        const uint32_t x = __float_as_uint(s[0][2 * h]), y = __float_as_uint(s[0][2 * h + 1]);
+                        const uint32_t low = dec_transpose(__byte_perm(x, y, 0x5410)), high = dec_transpose(__byte_perm(x, y, 0x7632));
+                        pk[2 * h] = __byte_perm(low, high, 0x5410);
+                        pk[2 * h + 1] = __byte_perm(low, high, 0x7632);
                     }
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
+                    for (int i = 0; i < 4; i++) pl[i] = dec_rest(pk[i]);
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const uint32_t a[4] = {v[2 * h][2 * j], v[2 * h][2 * j + 1], v[2 * h + 1][2 * j], v[2 * h + 1][2 * j + 1]};
-                            uint32_t ah[4], al[4];
+                    for (int c = 0; c < CHUNKS; c++) {
+                        uint32_t v[4][4];
 #pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                ah[i] = a[i] & 0xffffe000u;
-                                al[i] = __float_as_uint(__uint_as_float(a[i]) - __uint_as_float(ah[i]));
-                            }
-                            dec_mma8(o[0][c][j], ah[0], ah[1], ah[2], ah[3], ph[2 * h], ph[2 * h + 1]);
-                            dec_mma8(o[0][c][j], al[0], al[1], al[2], al[3], ph[2 * h], ph[2 * h + 1]);
-                            dec_mma8(o[0][c][j], ah[0], ah[1], ah[2], ah[3], pl[2 * h], pl[2 * h + 1]);
-                        }
-                }
-            } else if constexpr (S::IS_Q8) {
-                // scales of V: of keys g and g + 8, block by block, into the probabilities
-                const uint32_t va = vs + 4 * g * S::Q8_V, vb = va + 32 * S::Q8_V;
-                float d[2][HD / 32];
-                uint32_t top = 0;
-#pragma unroll
-                for (int blk = 0; blk < HD / 32; blk++) {
-                    const uint32_t x = dec_lds_u16(va + 34 * blk), y = dec_lds_u16(vb + 34 * blk);
-                    d[0][blk] = __half2float(__ushort_as_half((unsigned short)x));
-                    d[1][blk] = __half2float(__ushort_as_half((unsigned short)y));
-                    top = max(top, max(__float_as_uint(fabsf(d[0][blk])), __float_as_uint(fabsf(d[1][blk]))));
-                }
-                const float inv = take_v_scale(top);
-#pragma unroll
-                for (int c = 0; c < CHUNKS; c++) {
-                    fragments(d[0][c] * inv, d[1][c] * inv);
-                    uint32_t w[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t at = vs + 4 * (2 * t + (k & 1) + 8 * (k >> 1)) * S::Q8_V + 68 * (c >> 1);
-                        if (c & 1) w[k] = dec_lds(at + 4 * (9 + g));
-                        else {
-                            const uint32_t x = dec_lds(at + 4 * (1 + g)), w0 = dec_lds(at);
-                            w[k] = g == 7 ? __byte_perm(x, w0, 0x7610) : x;
-                        }
-                        w[k] ^= 0x80808080u;
-                    }
-                    const uint32_t x01 = __byte_perm(w[0], w[1], 0x5140), x23 = __byte_perm(w[0], w[1], 0x7362);
-                    const uint32_t y01 = __byte_perm(w[2], w[3], 0x5140), y23 = __byte_perm(w[2], w[3], 0x7362);
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const uint32_t x = j ? x23 : x01, y = j ? y23 : y01;
-                        const uint32_t a0 = dec_int8<0>(x), a1 = dec_int8<1>(x), a2 = dec_int8<0>(y), a3 = dec_int8<1>(y);
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            dec_mma16(o[nt][c][j], a0, a1, a2, a3, pb[nt][0][0], pb[nt][0][1]);
-                            if constexpr (WIDE) dec_mma16(o[nt][c][j], a0, a1, a2, a3, pb[nt][1][0], pb[nt][1][1]);
-                        }
-                    }
-                }
-            } else if constexpr (S::IS_F8) {
-                constexpr int WORDS = S::F8_V / 4;
-#pragma unroll
-                for (int c = 0; c < CHUNKS; c++) {
-                    uint32_t v[4][WORDS];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t at = vs + lane * S::F8_V + (c * 4 + k) * 32 * S::F8_V;
-                        if constexpr (WORDS == 4) {
-                            const uint4 r = dec_lds4(at);
+                        for (int k = 0; k < 4; k++) {
+                            const uint4 r = dec_lds4(vs + lane * 16 + (c * 4 + k) * 512);
                             v[k][0] = r.x; v[k][1] = r.y; v[k][2] = r.z; v[k][3] = r.w;
-                        } else {
-                            const uint2 r = dec_lds2(at);
-                            v[k][0] = r.x; v[k][1] = r.y;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            float d[4] = {0.f, 0.f, 0.f, 0.f};  // (summed on its own, as in add_values)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const uint32_t a[4] = {v[2 * h][2 * j], v[2 * h][2 * j + 1], v[2 * h + 1][2 * j], v[2 * h + 1][2 * j + 1]};
+                                uint32_t al[4];
+#pragma unroll
+                                for (int i = 0; i < 4; i++) al[i] = dec_rest(a[i]);
+                                dec_mma8(d, al[0], al[1], al[2], al[3], pk[2 * h], pk[2 * h + 1]);
+                                dec_mma8(d, a[0], a[1], a[2], a[3], pl[2 * h], pl[2 * h + 1]);
+                                dec_mma8(d, a[0], a[1], a[2], a[3], pk[2 * h], pk[2 * h + 1]);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[0][c][j][e] += d[e];
                         }
                     }
+                } else if constexpr (S::IS_Q8) {
+                    // scales of V: of keys g and g + 8, block by block, into the probabilities
+                    const uint32_t va = vs + 4 * g * S::Q8_V, vb = va + 32 * S::Q8_V;
+                    float d[2][HD / 32];
+                    uint32_t top = 0;
 #pragma unroll
-                    for (int w = 0; w < WORDS; w++) {
-                        // bytes of two keys next to one another: values of one dimension
-                        const uint32_t x01 = __byte_perm(v[0][w], v[1][w], 0x5140), x23 = __byte_perm(v[0][w], v[1][w], 0x7362);
-                        const uint32_t y01 = __byte_perm(v[2][w], v[3][w], 0x5140), y23 = __byte_perm(v[2][w], v[3][w], 0x7362);
+                    for (int blk = 0; blk < HD / 32; blk++) {
+                        const uint32_t x = dec_lds_u16(va + 34 * blk), y = dec_lds_u16(vb + 34 * blk);
+                        d[0][blk] = __half2float(__ushort_as_half((unsigned short)x));
+                        d[1][blk] = __half2float(__ushort_as_half((unsigned short)y));
+                        top = max(top, max(__float_as_uint(fabsf(d[0][blk])), __float_as_uint(fabsf(d[1][blk]))));
+                    }
+                    const float inv = take_v_scale(top);
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; c++) {
+                        fragments(d[0][c] * inv, d[1][c] * inv);
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t at = vs + 4 * (2 * t + (k & 1) + 8 * (k >> 1)) * S::Q8_V + 68 * (c >> 1);
+                            if (c & 1) w[k] = dec_lds(at + 4 * (9 + g));
+                            else {
+                                const uint32_t x = dec_lds(at + 4 * (1 + g)), w0 = dec_lds(at);
+                                w[k] = g == 7 ? __byte_perm(x, w0, 0x7610) : x;
+                            }
+                            w[k] ^= 0x80808080u;
+                        }
+                        const uint32_t x01 = __byte_perm(w[0], w[1], 0x5140), x23 = __byte_perm(w[0], w[1], 0x7362);
+                        const uint32_t y01 = __byte_perm(w[2], w[3], 0x5140), y23 = __byte_perm(w[2], w[3], 0x7362);
 #pragma unroll
                         for (int j = 0; j < 2; j++) {
                             const uint32_t x = j ? x23 : x01, y = j ? y23 : y01;
-                            const uint32_t a0 = dec_e4m3(x), a1 = dec_e4m3(x >> 16), a2 = dec_e4m3(y), a3 = dec_e4m3(y >> 16);
+                            const uint32_t a0 = dec_int8<0>(x), a1 = dec_int8<1>(x), a2 = dec_int8<0>(y), a3 = dec_int8<1>(y);
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                dec_mma16(o[nt][c][2 * w + j], a0, a1, a2, a3, pb[nt][0][0], pb[nt][0][1]);
-                                if constexpr (WIDE) dec_mma16(o[nt][c][2 * w + j], a0, a1, a2, a3, pb[nt][1][0], pb[nt][1][1]);
+                            for (int nt = 0; nt < NT; nt++) add_values(o[nt][c][j], a0, a1, a2, a3, pb[nt]);
+                        }
+                    }
+                } else if constexpr (S::IS_F8) {
+                    constexpr int WORDS = S::F8_V / 4;
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; c++) {
+                        uint32_t v[4][WORDS];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t at = vs + lane * S::F8_V + (c * 4 + k) * 32 * S::F8_V;
+                            if constexpr (WORDS == 4) {
+                                const uint4 r = dec_lds4(at);
+                                v[k][0] = r.x; v[k][1] = r.y; v[k][2] = r.z; v[k][3] = r.w;
+                            } else {
+                                const uint2 r = dec_lds2(at);
+                                v[k][0] = r.x; v[k][1] = r.y;
+                            }
+                        }
+#pragma unroll
+                        for (int w = 0; w < WORDS; w++) {
+                            // bytes of two keys next to one another: values of one dimension
+                            const uint32_t x01 = __byte_perm(v[0][w], v[1][w], 0x5140), x23 = __byte_perm(v[0][w], v[1][w], 0x7362);
+                            const uint32_t y01 = __byte_perm(v[2][w], v[3][w], 0x5140), y23 = __byte_perm(v[2][w], v[3][w], 0x7362);
+#pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                const uint2 x = dec_e4m3(j ? x23 : x01), y = dec_e4m3(j ? y23 : y01);
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++) add_values(o[nt][c][2 * w + j], x.x, x.y, y.x, y.y, pb[nt]);
                             }
                         }
                     }
-                }
-            } else {
+                } else {
 #pragma unroll
-                for (int c = 0; c < CHUNKS; c++) {
-                    uint32_t v[4][4];
+                    for (int c = 0; c < CHUNKS; c++) {
+                        uint32_t v[4][4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint4 r = dec_lds4(vs + lane * 16 + (c * 4 + k) * 512);
-                        v[k][0] = r.x; v[k][1] = r.y; v[k][2] = r.z; v[k][3] = r.w;
-                    }
+                        for (int k = 0; k < 4; k++) {
+                            const uint4 r = dec_lds4(vs + lane * 16 + (c * 4 + k) * 512);
+                            v[k][0] = r.x; v[k][1] = r.y; v[k][2] = r.z; v[k][3] = r.w;
+                        }
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t a0 = __byte_perm(v[0][j], v[1][j], 0x5410), a1 = __byte_perm(v[0][j], v[1][j], 0x7632);
-                        const uint32_t a2 = __byte_perm(v[2][j], v[3][j], 0x5410), a3 = __byte_perm(v[2][j], v[3][j], 0x7632);
+                        for (int j = 0; j < 4; j++) {
+                            const uint32_t a0 = __byte_perm(v[0][j], v[1][j], 0x5410), a1 = __byte_perm(v[0][j], v[1][j], 0x7632);
+                            const uint32_t a2 = __byte_perm(v[2][j], v[3][j], 0x5410), a3 = __byte_perm(v[2][j], v[3][j], 0x7632);
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            dec_mma16(o[nt][c][j], a0, a1, a2, a3, pb[nt][0][0], pb[nt][0][1]);
-                            if constexpr (WIDE) dec_mma16(o[nt][c][j], a0, a1, a2, a3, pb[nt][1][0], pb[nt][1][1]);
+                            for (int nt = 0; nt < NT; nt++) add_values(o[nt][c][j], a0, a1, a2, a3, pb[nt]);
                         }
                     }
                 }
             }
 
             // ---- the end of the unit or of the run
-            const bool ends = use.tile + 1 == use.span.tiles;
+            const bool ends = use.left == 1;
             if (ends || it + 1 == count) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -946,11 +1057,29 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, 1) att
                             const int col = nt * 8 + 2 * t + e;
                             if (col >= h.count) continue;
                             const float inv = l[nt][e] == 0.0f ? 0.0f : v_scale / l[nt][e];
+                            // a lane's dimensions of a chunk are neighbours (two and two of Q8_0's even blocks)
+                            constexpr int RUN = S::IS_Q8 ? 2 : DPL;
+                            DecodeRaw<WIDE, RUN> gates[CHUNKS * DPL / RUN];
+                            if (p.gate) {
+                                const int64_t at = use.b * p.q_row + (h.first + col) * p.q_head;
 #pragma unroll
-                            for (int c = 0; c < CHUNKS; c++)
+                                for (int i = 0; i < CHUNKS * DPL / RUN; i++)
+                                    gates[i].load(p.gate, at + S::out_dim(i * RUN / DPL, i * RUN % DPL / 2, g));
+                            }
 #pragma unroll
-                                for (int j = 0; j < DPL / 2; j++)
-                                    dec_write2(p, use.b, h.first + col, S::out_dim(c, j, g), o[nt][c][j][e] * inv, o[nt][c][j][e + 2] * inv);
+                            for (int i = 0; i < CHUNKS * DPL / RUN; i++) {
+                                const int c = i * RUN / DPL, j0 = i * RUN % DPL / 2;
+                                float x[RUN];
+#pragma unroll
+                                for (int j = 0; j < RUN; j++) x[j] = o[nt][c][j0 + j / 2][e + 2 * (j & 1)] * inv;
+                                if (p.gate) {
+                                    float f[RUN];
+                                    dec_gates<WIDE, RUN>(p, gates[i], f);
+#pragma unroll
+                                    for (int j = 0; j < RUN; j++) x[j] *= f[j];
+                                }
+                                dec_write<WIDE, RUN>(p, use.b, h.first + col, S::out_dim(c, j0, g), x);
+                            }
                             if (g == 0) dec_write_lse(p, use.b, h.first + col, m[nt][e], l[nt][e]);
                         }
                 } else {
@@ -983,100 +1112,157 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, 1) att
                             tail_kind[warp] = 1;
                             tail_b[warp] = use.b;
                             tail_u[warp] = use.u;
-                            tail_end[warp] = begin + it + (use.span.tiles - use.tile);
+                            tail_end[warp] = begin + it + use.left;
                         } else {
                             head_kind[warp] = ends ? 1 : 2;
-                            head_b[warp] = use.b;
-                            head_u[warp] = use.u;
+                            if (warp == 0) {
+                                head_b = use.b;
+                                head_u = use.u;
+                            }
                         }
                     }
                 }
+                fresh = true;
             }
             use.next(p, units);
         }
         dec_wait<0>();
     }
-
-    // ---- joining the warps' partials, in the order of the keys
+#ifdef DEC_TRIG
+    pdl_trigger_late();
+#endif
+    // ---- joining the warps' partials, in the order of the keys: first what an earlier CTA began, then what a warp here
+    // began (warp 0 of CTA 0 never begins inside a unit)
     __syncthreads();
-    auto head_of = [&](int w) { return reinterpret_cast<float *>(smem + W * S::RING + w * S::PART_BYTES); };
-    float * const cta_head = p.partial + (size_t)blockIdx.x * 2 * S::PART_FLOATS;
-    float * const cta_tail = cta_head + S::PART_FLOATS;
-    int join_b = 0, join_u = 0, join_last = -1;
-    if (head_kind[0]) {
+    auto head_of = [&](int w) { return reinterpret_cast<const float *>(smem + W * S::RING + w * S::PART_BYTES); };
+#pragma unroll 1
+    for (int w = -1; w < W; w++) {
+        const bool tail = w >= 0;
+        if (!(tail ? tail_kind[w] : head_kind[0])) continue;
         int n = 1;
-        bool ends = head_kind[0] == 1;
-        while (!ends && n < W && head_kind[n]) ends = head_kind[n++] == 1;
-        // (warp 0 of CTA 0 never begins inside a unit)
-        dec_join<HD, COLS>(p, head_of(0), head_of(1), S::PART_BYTES / 4, n, false, head_b[0], head_u[0], cta_head, threadIdx.x, W * 32);
+        bool ends = !tail && head_kind[0] == 1;
+        const int second = tail ? w + 1 : 1;
+        while (!ends && second + n - 1 < W && head_kind[second + n - 1]) ends = head_kind[second + n++ - 1] == 1;
+        const int b = tail ? tail_b[w] : head_b, u = tail ? tail_u[w] : head_u;
+        dec_join<HD, COLS, WIDE>(p, tail ? reinterpret_cast<const float *>(smem + w * S::RING) : head_of(0), head_of(min(second, W - 1)),
+                                 S::PART_BYTES / 4, n, ends && tail, b, u, scratch_at(tail), threadIdx.x, W * 32);
+        if (tail && !ends && threadIdx.x == 0)
+            p.joins[atomicAdd(p.counters + DEC_JOINS, 1)] = make_int4(b, u, (int)blockIdx.x, (int)((tail_end[w] - 1) / (share * W)));
     }
-    for (int w = 0; w < W; w++) {
-        if (!tail_kind[w]) continue;
-        int n = 1;
-        bool ends = false;
-        while (!ends && w + n < W && head_kind[w + n]) ends = head_kind[w + n++] == 1;
-        dec_join<HD, COLS>(p, reinterpret_cast<const float *>(smem + w * S::RING), w + 1 < W ? head_of(w + 1) : nullptr, S::PART_BYTES / 4, n, ends,
-                           tail_b[w], tail_u[w], cta_tail, threadIdx.x, W * 32);
-        if (!ends) {
-            join_b = tail_b[w];
-            join_u = tail_u[w];
-            join_last = (int)((tail_end[w] - 1) / (share * W));
-        }
-    }
-    if (threadIdx.x == 0) p.joins[blockIdx.x] = make_int4(join_b, join_u, join_last, 0);
 }
 
-// The units that several CTAs share: a CTA per (CTA in which such a unit begins, column).
-template <int HD, int COLS> __global__ void __launch_bounds__(HD / 2) attention_decode_join_kernel(const DecodeParams p) {
-    constexpr int PART = COLS * (HD + 2);
+// The units that several CTAs share. A CTA takes a column of one at a time; groups of threads take every JOIN_GROUPS-th
+// partial, so that many loads are in flight, and are added in their order.
+constexpr int JOIN_THREADS = 256, JOIN_CTAS_SM = 4;
+template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_THREADS) attention_decode_join_kernel(const DecodeParams p) {
+    constexpr int PART = COLS * (HD + 2), LANES = HD / 4, GROUPS = JOIN_THREADS / LANES, EACH = DEC_CTAS / JOIN_THREADS;
+    __shared__ float factor[DEC_CTAS], reduce[2][JOIN_THREADS / 32];
+    __shared__ float4 sums[GROUPS][LANES];
     pdl_entry();
-    const int c = blockIdx.x, col = blockIdx.y;
-    const int4 join = p.joins[c];
-    if (join.z < 0) return;
-    const DecodeHeads h = decode_heads(p, join.y);
-    if (col >= h.count) return;
-    const int n = join.z - c + 1;  // partials: the tail of CTA c and the heads of the following ones
-    const float * tail = p.partial + ((size_t)c * 2 + 1) * PART;
-    const float * heads = p.partial + (size_t)(c + 1) * 2 * PART;
-    auto part = [&](int k) { return k ? heads + (size_t)(k - 1) * 2 * PART : tail; };
-    float m = -INFINITY;
-    for (int k = 0; k < n; k++) m = fmaxf(m, part(k)[COLS * HD + col]);
-    float l = 0.0f, x = 0.0f, y = 0.0f;
-    const int dim = 2 * threadIdx.x;
-#pragma unroll 8
-    for (int k = 0; k < n; k++) {
-        const float * q = part(k);
-        const float f = exp2f(q[COLS * HD + col] - m);
-        const float2 o = *reinterpret_cast<const float2 *>(q + col * HD + dim);
-        l = fmaf(f, q[COLS * HD + COLS + col], l);
-        x = fmaf(f, o.x, x);
-        y = fmaf(f, o.y, y);
+    const int tid = threadIdx.x, dim = 4 * (tid % LANES), group = tid / LANES;
+    const int jobs = p.counters[DEC_JOINS] * COLS;
+#pragma unroll 1
+    for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
+        const int4 join = p.joins[job / COLS];
+        const int col = job % COLS;
+        const DecodeHeads h = decode_heads(p, join.y);
+        if (col >= h.count) continue;
+        const int n = join.w - join.z + 1;  // partials: the tail of the first CTA and the heads of the following ones
+        const float * tail = p.partial + ((size_t)join.z * 2 + 1) * PART;
+        const float * heads = p.partial + (size_t)(join.z + 1) * 2 * PART;
+        auto part = [&](int k) { return k ? heads + (size_t)(k - 1) * 2 * PART : tail; };
+        float gate[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+        if (p.gate && group == 0) {
+            DecodeRaw<WIDE, 4> raw;
+            raw.load(p.gate, join.x * p.q_row + (h.first + col) * p.q_head + dim);
+            dec_gates<WIDE, 4>(p, raw, gate);
+        }
+        float ms[EACH], ls[EACH], m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int k = tid + i * JOIN_THREADS;
+            ms[i] = k < n ? part(k)[COLS * HD + col] : -INFINITY;
+            ls[i] = k < n ? part(k)[COLS * HD + COLS + col] : 0.0f;
+            m = fmaxf(m, ms[i]);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if ((tid & 31) == 0) reduce[0][tid >> 5] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < JOIN_THREADS / 32; w++) m = fmaxf(m, reduce[0][w]);
+        float l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int k = tid + i * JOIN_THREADS;
+            if (k < n) {
+                const float f = exp2f(ms[i] - m);
+                factor[k] = f;
+                l = fmaf(f, ls[i], l);
+            }
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if ((tid & 31) == 0) reduce[1][tid >> 5] = l;
+        __syncthreads();
+        l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < JOIN_THREADS / 32; w++) l += reduce[1][w];
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int k = group; k < n; k += GROUPS) {
+            const float f = factor[k];
+            const float4 o = *reinterpret_cast<const float4 *>(part(k) + col * HD + dim);
+            x.x = fmaf(f, o.x, x.x);
+            x.y = fmaf(f, o.y, x.y);
+            x.z = fmaf(f, o.z, x.z);
+            x.w = fmaf(f, o.w, x.w);
+        }
+        sums[group][tid % LANES] = x;
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+            for (int i = 1; i < GROUPS; i++) {
+                const float4 o = sums[i][tid];
+                x.x += o.x;
+                x.y += o.y;
+                x.z += o.z;
+                x.w += o.w;
+            }
+            dec_write<WIDE, 4>(p, join.x, h.first + col, dim, {x.x / l * gate[0], x.y / l * gate[1], x.z / l * gate[2], x.w / l * gate[3]});
+            if (tid == 0) dec_write_lse(p, join.x, h.first + col, m, l);
+        }
+        __syncthreads();
     }
-    dec_write2(p, join.x, h.first + col, dim, x / l, y / l);
-    if (dim == 0) dec_write_lse(p, join.x, h.first + col, m, l);
+    // the last CTA leaves the counters as the call found them (every CTA has read its own above)
+    if (tid == 0 && atomicAdd(p.counters + DEC_DONE, 1) == (int)gridDim.x - 1)
+        p.counters[DEC_JOINS] = p.counters[DEC_DONE] = 0;
 }
 
-// Launches for one format; `ctas` CTAs. Returns the kernels launched.
-void launch_decode_f32(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int ctas);
-void launch_decode_f16(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int ctas);
-void launch_decode_q8_0(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int ctas);
-void launch_decode_f8(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int ctas);
+// Launches for one format on a device with `sms` multiprocessors.
+void launch_decode_f32(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int sms);
+void launch_decode_f16(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int sms);
+void launch_decode_q8_0(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int sms);
+void launch_decode_f8(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int sms);
 
-template <int FMT, int HD, int NT, bool WIDE> void launch_decode_as(cudaStream_t s, const DecodeParams & p, int ctas) {
+template <int FMT, int HD, int NT, bool WIDE> void launch_decode_as(cudaStream_t s, DecodeParams p, int sms) {
     using S = DecodeShape<FMT, HD, NT, WIDE>;
+    const int ctas = sms * S::RESIDENT;
+    YK_REQUIRE(ctas <= DEC_CTAS && ctas * 2 * S::PART_FLOATS * sizeof(float) <= DEC_PARTIAL_BYTES, YUUKA_ERR_UNSUPPORTED,
+               "attention_decode: %d multiprocessors", sms);
     auto kern = attention_decode_kernel<FMT, HD, NT, WIDE>;
     YK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::LAYOUT_BYTES));
     launch_k(kern, (unsigned)ctas, S::W * 32, S::LAYOUT_BYTES, s, p);
-    launch_k(attention_decode_join_kernel<HD, S::COLS>, dim3((unsigned)ctas, S::COLS), HD / 2, 0, s, p);
+    launch_k(attention_decode_join_kernel<HD, S::COLS, WIDE>, (unsigned)(sms * JOIN_CTAS_SM), JOIN_THREADS, 0, s, p);
 }
-template <int FMT, int HD, int NT> void launch_decode_tiles(cudaStream_t s, const DecodeParams & p, int ctas) {
-    if (p.dtype == YUUKA_DTYPE_F32) launch_decode_as<FMT, HD, NT, true>(s, p, ctas);
-    else launch_decode_as<FMT, HD, NT, false>(s, p, ctas);
+template <int FMT, int HD, int NT> void launch_decode_tiles(cudaStream_t s, const DecodeParams & p, int sms) {
+    if (p.dtype == YUUKA_DTYPE_F32) launch_decode_as<FMT, HD, NT, true>(s, p, sms);
+    else launch_decode_as<FMT, HD, NT, false>(s, p, sms);
 }
-template <int FMT, int NT> void launch_decode_dims(cudaStream_t s, const DecodeParams & p, int head_dim, int ctas) {
-    if (head_dim == 64) launch_decode_tiles<FMT, 64, NT>(s, p, ctas);
-    else if (head_dim == 128) launch_decode_tiles<FMT, 128, NT>(s, p, ctas);
-    else launch_decode_tiles<FMT, 256, NT>(s, p, ctas);
+template <int FMT, int NT> void launch_decode_dims(cudaStream_t s, const DecodeParams & p, int head_dim, int sms) {
+    if (head_dim == 64) launch_decode_tiles<FMT, 64, NT>(s, p, sms);
+    else if (head_dim == 128) launch_decode_tiles<FMT, 128, NT>(s, p, sms);
+    else launch_decode_tiles<FMT, 256, NT>(s, p, sms);
 }
 
 }  // namespace yk

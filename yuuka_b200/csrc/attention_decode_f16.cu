@@ -3,9 +3,9 @@
 
 namespace yk {
 
-void launch_decode_f16(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int ctas) {
-    if (cols == 8) launch_decode_dims<YUUKA_KV_F16, 1>(s, p, head_dim, ctas);
-    else launch_decode_dims<YUUKA_KV_F16, 2>(s, p, head_dim, ctas);
+void launch_decode_f16(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int sms) {
+    if (cols == 8) launch_decode_dims<YUUKA_KV_F16, 1>(s, p, head_dim, sms);
+    else launch_decode_dims<YUUKA_KV_F16, 2>(s, p, head_dim, sms);
 }
 
 }  // namespace yk

@@ -3,9 +3,9 @@
 
 namespace yk {
 
-void launch_decode_q8_0(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int ctas) {
-    if (cols == 8) launch_decode_dims<YUUKA_KV_Q8_0, 1>(s, p, head_dim, ctas);
-    else launch_decode_dims<YUUKA_KV_Q8_0, 2>(s, p, head_dim, ctas);
+void launch_decode_q8_0(cudaStream_t s, const DecodeParams & p, int head_dim, int cols, int sms) {
+    if (cols == 8) launch_decode_dims<YUUKA_KV_Q8_0, 1>(s, p, head_dim, sms);
+    else launch_decode_dims<YUUKA_KV_Q8_0, 2>(s, p, head_dim, sms);
 }
 
 }  // namespace yk
