@@ -30,7 +30,7 @@ extern "C" yuuka_status yuuka_attention_scratch_create(yuuka_device * dev, yuuka
         YK_REQUIRE(dev, YUUKA_ERR_INVALID_ARGUMENT, "attention_scratch_create: null argument");
         set_device(dev);
         void * ptr = nullptr;
-        const size_t bytes = DEC_COUNTER_BYTES + DEC_CTAS * sizeof(int4) + DEC_PARTIAL_BYTES;
+        const size_t bytes = DEC_COUNTER_BYTES + 2 * DEC_WARPS * sizeof(int4) + DEC_PARTIAL_BYTES;
         const cudaError_t err = cudaMalloc(&ptr, bytes);
         if (err != cudaSuccess) {
             cudaGetLastError();
@@ -141,7 +141,7 @@ extern "C" yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_atte
         p.scale_log2 = (float)(scale * 1.4426950408889634);
         p.counters = (int *)scratch->memory;
         p.joins = (int4 *)(scratch->memory + DEC_COUNTER_BYTES);
-        p.partial = (float *)(scratch->memory + DEC_COUNTER_BYTES + DEC_CTAS * sizeof(int4));
+        p.partial = (float *)(scratch->memory + DEC_COUNTER_BYTES + 2 * DEC_WARPS * sizeof(int4));
         // tiles are counted in 31 bits
         const double tiles = (double)a->batch * cache->kv_heads * p.head_tiles * (p.cache.capacity / DEC_TILE + 1.0);
         YK_REQUIRE(tiles < 2e9, YUUKA_ERR_UNSUPPORTED, "%s: %g tiles of keys are too many for one call", op, tiles);

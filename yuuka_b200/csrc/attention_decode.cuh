@@ -13,11 +13,12 @@
 // halves one byte permutation pairs up: no lane reads what another has copied, no barrier, no bank conflict. (Q8_0's blocks of
 // 34 bytes are copied by words, and the word at which a lane starts is chosen so that its two words are never misaligned.)
 //
-// Work is cut at the granularity of warps: all tiles of 16 keys of all units form one sequence, every warp of the grid takes
-// an equal run of it, wherever that begins and ends, with its copies running ahead across units. So batches of any mixture of
-// lengths load the machine evenly, and the grid does not depend on the lengths, which only the device knows. A run that ends
-// inside a unit leaves a partial (O, m, l); those of a CTA's warps are joined in shared memory, those of several CTAs in
-// scratch memory, always in the order of the keys, so results do not depend on timing.
+// Work is cut at the granularity of warps. A team of as many warps as a row has units (KV heads) takes a run of tiles, each
+// warp one head of the same keys, so that the heads of a token, which lie side by side in the pool, are read at about the same
+// time. The rows' tiles form one sequence that the teams share evenly, wherever a run begins and ends, with its copies running
+// ahead across rows. So batches of any mixture of lengths load the machine evenly, and the grid does not depend on the lengths,
+// which only the device knows. A run that ends inside a row leaves a partial (O, m, l) in scratch memory, and a second kernel
+// joins those of a row, always in the order of the keys, so results do not depend on timing.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -43,18 +44,19 @@ struct DecodeParams {
     int batch, heads, group, head_tiles, tile_heads;  // group: query heads per KV head; tiles of them, heads per tile
     int window, dtype;
     float scale_log2;  // softmax scale times log2 e
-    float * partial;   // [CTAs][2][part floats]: a CTA's first and last unfinished unit
-    int4 * joins;      // units that several CTAs share: x row, y unit of the row, z first and w last CTA
-    int * counters;    // zero between calls: joins listed, CTAs of the joining kernel done
+    float * partial;   // [teams][units][2][part floats]: what a run leaves of its first row (0) and of its last one (1)
+    int4 * joins;      // [2][DEC_WARPS] units that several teams share, few and many: x row, y unit of the row, z first and w last team
+    int * counters;    // zero between calls: joins of both lists, CTAs of the joining kernel done
 };
 
 constexpr int DEC_TILE = 16;            // keys
 #ifndef DEC_MIN_TILES
 #define DEC_MIN_TILES 1
 #endif
-constexpr int DEC_CTAS = 1024;          // at most
-constexpr size_t DEC_PARTIAL_BYTES = 8u << 20;
-enum { DEC_JOINS, DEC_DONE, DEC_COUNTERS };
+constexpr int DEC_WARPS = 4096;         // of a grid, at most
+constexpr size_t DEC_PARTIAL_BYTES = 24u << 20;
+enum { DEC_SHORT, DEC_LONG, DEC_DONE, DEC_COUNTERS };
+constexpr int DEC_SHORT_MOST = 32;      // partials that a warp joins
 constexpr float DEC_P_LOG2 = 7.0f;      // log2 of the factor that probabilities carry
 constexpr float DEC_SLACK = 8.0f;       // log2 of what a score may pass the running maximum by before sums are rescaled
 constexpr int DEC_SMEM_SM = 233472;     // shared memory of an SM
@@ -143,8 +145,6 @@ template <int PAIR> __device__ __forceinline__ uint32_t dec_int8(uint32_t x) {
 // the products as two parts (22 bits); otherwise f16 or bf16 and one part (11 bits, no less than such an output can tell).
 template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     static constexpr bool IS_F32 = FMT == YUUKA_KV_F32, IS_Q8 = FMT == YUUKA_KV_Q8_0, IS_F8 = FMT == YUUKA_KV_F8;
-    // lanes read what others have copied (Q8_0's words, F8's scales)
-    static constexpr bool SHARED_COPIES = IS_Q8 || IS_F8;
         // warps of a CTA, CTAs of an SM
 #ifndef DEC_W64
 #define DEC_W64 4
@@ -164,19 +164,27 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     static constexpr int F8_V = HD == 64 ? 8 : 16;
     static constexpr int K_BYTES = IS_F32 ? HD * 64 : (IS_Q8 ? 64 * Q8_K : (IS_F8 ? HD * 16 + 128 : HD * 32));
     static constexpr int V_BYTES = IS_F32 ? HD * 64 : (IS_Q8 ? 64 * Q8_V : (IS_F8 ? HD * 16 : HD * 32));
+    // K of the other formats: a key's row, its 16-byte pieces copied by lines of 128 bytes, eight lanes to a line (one request
+    // to memory instead of two: 239 -> 227 us for 8 sequences of 32768, 8 KV heads of 128). In odd keys the halves of a line
+    // trade places, so that the eight lanes that read four pieces of two keys find them on different banks.
+    static constexpr int K_ROW = IS_Q8 ? 0 : IS_F32 ? HD * 4 : IS_F8 ? HD : HD * 2;
+    static constexpr bool K_LINES = K_ROW >= 128;
+    // where piece q (16 bytes) of a key's row lies
+    __device__ static __forceinline__ uint32_t k_piece(int key, int q) {
+        return key * K_ROW + 16 * (K_LINES ? q ^ ((key & 1) << 2) : q);
+    }
     static constexpr int SLOT = (K_BYTES > V_BYTES ? K_BYTES : V_BYTES);
     static constexpr int PART_FLOATS = COLS * (HD + 2);
-    static constexpr int PART_BYTES = (PART_FLOATS * 4 + 15) / 16 * 16;
     // queries in registers, or in shared memory where the sums leave too few (f32: 8 heads of all dimensions, split at use)
     static constexpr bool Q_SHARED = IS_F32 || HD / 4 * NT + HD / 8 * PARTS * NT > 128;
     static constexpr int Q_BYTES = !Q_SHARED ? 0 : (IS_F32 ? 8 * HD * 4 : COLS * HD * 2 * PARTS);
     static constexpr int WARP_BYTES = (DEC_SMEM_SM / RESIDENT - 1536) / W / 16 * 16;  // (the rest: the warps' records, what a CTA takes by itself)
-    static constexpr int FIT = (WARP_BYTES - PART_BYTES - Q_BYTES) / SLOT;
+    static constexpr int FIT = (WARP_BYTES - Q_BYTES) / SLOT;
     static constexpr int SLOTS = FIT > 8 ? 8 : FIT;  // K and V of a tile take one each
     static constexpr int AHEAD = SLOTS - 1;
     static constexpr int RING = SLOTS * SLOT;
-    static_assert(SLOTS >= 2 && RING >= PART_BYTES, "a warp's shared memory");
-    static constexpr int LAYOUT_BYTES = W * (RING + PART_BYTES + Q_BYTES);
+    static_assert(SLOTS >= 2, "a warp's shared memory");
+    static constexpr int LAYOUT_BYTES = W * (RING + Q_BYTES);
     // accumulators: chunks of dimensions, DPL of them per lane
     static constexpr int DPL = (IS_F32 || IS_Q8) ? 4 : (IS_F8 ? F8_V : 8);
     static constexpr int CHUNKS = HD / (8 * DPL);
@@ -228,11 +236,11 @@ __device__ __forceinline__ DecodeSpan decode_span(const DecodeParams & p, int b)
     return decode_span(p, b, bad);
 }
 
-// A place in the sequence of tiles: the next one of unit u of row b.
+// A place in the sequence of tiles: the next one of row b.
 struct DecodeCursor {
-    int b, u;
-    int pos, end;  // its first key; behind the unit's last key
-    int left;      // tiles of the unit from here on
+    int b;
+    int pos, end;           // its first key; behind the row's last key
+    int left;               // tiles of the row from here on
     int first, tiles, seq;  // of the row
     __device__ __forceinline__ void row(const DecodeParams & p) {
         const DecodeSpan s = decode_span(p, b);
@@ -241,13 +249,10 @@ struct DecodeCursor {
         tiles = s.tiles;
         seq = s.seq;
     }
-    __device__ __forceinline__ void next(const DecodeParams & p, int units) {
+    __device__ __forceinline__ void next(const DecodeParams & p) {
         pos += DEC_TILE;
         if (--left > 0) return;
-        if (++u == units) {
-            u = 0;
-            if (++b < p.batch) row(p);
-        }
+        if (++b < p.batch) row(p);
         pos = first;
         left = tiles;
     }
@@ -260,6 +265,14 @@ struct DecodeCursor {
 template <bool WIDE, int N> struct DecodeRaw {
     static constexpr int WORDS = WIDE ? N : N / 2;
     uint32_t w[WORDS];
+    __device__ __forceinline__ void fetch(const float * from) {  // scratch memory: not through the read-only path
+        static_assert(WIDE, "f32");
+#pragma unroll
+        for (int i = 0; i < WORDS; i += N == 2 ? 2 : 4) {
+            if constexpr (N == 2) *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(from);
+            else *reinterpret_cast<uint4 *>(w + i) = *reinterpret_cast<const uint4 *>(from + i);
+        }
+    }
     __device__ __forceinline__ void load(const void * base, int64_t at) {
         const uint32_t * src = reinterpret_cast<const uint32_t *>(base) + (WIDE ? at : at / 2);
         if constexpr (WORDS == 1) w[0] = __ldg(src);
@@ -335,45 +348,6 @@ __device__ __forceinline__ DecodeHeads decode_heads(const DecodeParams & p, int 
     return h;
 }
 
-// A chain of partials of one unit, `count` of them `stride` floats apart from `second` on, joined and written: as the unit's
-// result (final), or as one partial. Threads of a CTA take pairs of dimensions.
-template <int HD, int COLS, bool WIDE>
-__device__ __forceinline__ void dec_join(const DecodeParams & p, const float * head, const float * second, int stride, int count, bool final,
-                                         int b, int u, float * dst, int thread, int threads) {
-    const DecodeHeads h = decode_heads(p, u);
-    for (int i = thread; i < COLS * HD / 2; i += threads) {
-        const int col = i / (HD / 2), dim = 2 * (i - col * (HD / 2));
-        if (col >= h.count) continue;
-        float gate[2] = {1.0f, 1.0f};
-        if (final && p.gate) {
-            DecodeRaw<WIDE, 2> raw;
-            raw.load(p.gate, b * p.q_row + (h.first + col) * p.q_head + dim);
-            dec_gates<WIDE, 2>(p, raw, gate);
-        }
-        float m = -INFINITY;
-        for (int k = 0; k < count; k++) m = fmaxf(m, (k ? second + (size_t)(k - 1) * stride : head)[COLS * HD + col]);
-        float l = 0.0f, x = 0.0f, y = 0.0f;
-        for (int k = 0; k < count; k++) {
-            const float * part = k ? second + (size_t)(k - 1) * stride : head;
-            const float f = exp2f(part[COLS * HD + col] - m);
-            const float2 o = *reinterpret_cast<const float2 *>(part + col * HD + dim);
-            l = fmaf(f, part[COLS * HD + COLS + col], l);
-            x = fmaf(f, o.x, x);
-            y = fmaf(f, o.y, y);
-        }
-        if (final) {
-            dec_write<WIDE, 2>(p, b, h.first + col, dim, {x / l * gate[0], y / l * gate[1]});
-            if (dim == 0) dec_write_lse(p, b, h.first + col, m, l);
-        } else {
-            *reinterpret_cast<float2 *>(dst + col * HD + dim) = make_float2(x, y);
-            if (dim == 0) {
-                dst[COLS * HD + col] = m;
-                dst[COLS * HD + COLS + col] = l;
-            }
-        }
-    }
-}
-
 // ---- the kernel ----------------------------------------------------------------------------------------------------
 
 template <int FMT, int HD, int NT, bool WIDE>
@@ -381,41 +355,35 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
     using S = DecodeShape<FMT, HD, NT, WIDE>;
     constexpr int W = S::W, COLS = S::COLS, AHEAD = S::AHEAD, CHUNKS = S::CHUNKS, DPL = S::DPL;
     extern __shared__ __align__(16) uint8_t smem[];
-    // What the CTA's warps leave unfinished: a unit begun by an earlier warp (head: 1 it ends here, 2 it goes on), a unit begun
-    // here (tail: 1) that goes on
-    __shared__ int head_kind[W], tail_kind[W], tail_b[W], tail_u[W], head_b, head_u;
-    __shared__ unsigned tail_end[W];  // tile behind the tail's unit
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    uint8_t * const ring_at = smem + warp * S::RING;
-    float * const head_part = reinterpret_cast<float *>(smem + W * S::RING + warp * S::PART_BYTES);
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(ring_at);
-    const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(smem + W * (S::RING + S::PART_BYTES) + warp * S::Q_BYTES) + lane * 16;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * S::RING);
+    const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(smem + W * S::RING + warp * S::Q_BYTES) + lane * 16;
     pdl_entry();
 
-    // this warp's run of tiles
-    const int units = p.cache.kv_heads * p.head_tiles;
+    // this warp's unit and its team's run of tiles
     unsigned total = 0;  // (below 2^31: the host has checked)
     for (int b = lane; b < p.batch; b += 32) {
         int bad;
         total += decode_span(p, b, bad).tiles;
         if (bad && p.status && blockIdx.x == 0 && warp == 0) atomicOr(p.status, bad);
     }
-    total = __reduce_add_sync(0xffffffffu, total) * units;
-    const unsigned warps = gridDim.x * W;
-    const unsigned share = max((total + warps - 1) / warps, (unsigned)DEC_MIN_TILES);
-    const unsigned begin = (blockIdx.x * W + warp) * share;
-    const int count = begin < total ? (int)min(share, total - begin) : 0;
-    auto scratch_at = [&](bool tail) { return p.partial + ((size_t)blockIdx.x * 2 + tail) * S::PART_FLOATS; };
-
-    if (lane == 0) head_kind[warp] = tail_kind[warp] = 0;
-    if (count > 0) {
+    total = __reduce_add_sync(0xffffffffu, total);
+    const unsigned units = p.cache.kv_heads * p.head_tiles, warps = gridDim.x * W, self = blockIdx.x * W + warp;
+    const unsigned teams = max(warps / units, 1u), team = min(self / units, units > warps ? 0u : ~0u);
+    const unsigned share = max((total + teams - 1) / teams, (unsigned)DEC_MIN_TILES);
+    const unsigned begin = team * share;
+    const int count = team < teams && begin < total ? (int)min(share, total - begin) : 0;
+#pragma unroll 1
+    for (unsigned unit = units > warps ? self : self - team * units; unit < units; unit += warps) {
+    if (count == 0) break;
+    {
         DecodeCursor use;
         {
             unsigned before = 0;
             use.b = 0;
             for (int base = 0; base < p.batch; base += 32) {  // (begin < total: some row holds it)
                 const int b = base + lane;
-                const unsigned mine = b < p.batch ? (unsigned)decode_span(p, b).tiles * units : 0;
+                const unsigned mine = b < p.batch ? (unsigned)decode_span(p, b).tiles : 0;
                 unsigned sum = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -432,9 +400,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 before += __shfl_sync(0xffffffffu, sum, 31);
             }
             use.row(p);
-            const unsigned rest = begin - before;
-            use.u = min((int)(rest / (unsigned)use.tiles), units - 1);  // (it is less, unless lengths change under the call)
-            const int tile = min((int)rest - use.u * use.tiles, use.tiles - 1);
+            const int tile = min((int)(begin - before), use.tiles - 1);  // (it is less, unless lengths change under the call)
             use.pos = use.first + tile * DEC_TILE;
             use.left = use.tiles - tile;
         }
@@ -446,8 +412,11 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
         unsigned block_of = 0, within = 0; // of key lane % 16 of the next tile
         unsigned pool_row = 0;
         bool copies = false;
-        const uint8_t * k_at = nullptr;    // the pools at the unit's head and this lane's piece
-        const uint8_t * v_at = nullptr;
+        // the pools at the unit's head and this lane's piece
+        constexpr int HEAD_BYTES = FMT == YUUKA_KV_F32 ? HD * 4 : (FMT == YUUKA_KV_F16 ? HD * 2 : (FMT == YUUKA_KV_Q8_0 ? HD / 32 * 34 : HD));
+        const int kv_head = unit / p.head_tiles;
+        const uint8_t * const k_at = p.cache.k + (int64_t)kv_head * HEAD_BYTES + (S::IS_Q8 ? 4 * (lane & 7) : 16 * (S::K_LINES ? lane & 7 : t));
+        const uint8_t * const v_at = p.cache.v + (int64_t)kv_head * HEAD_BYTES + (S::IS_Q8 ? 4 * (lane & 7) : (S::IS_F8 ? S::F8_V : 16) * g);
         const int32_t * table = nullptr;
         const unsigned row_bytes = (unsigned)p.cache.row_bytes;
         auto look_up = [&] {
@@ -457,12 +426,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
             within = pos - page * p.cache.block_size;
             block_of = (unsigned)__ldg(table + page);
         };
-        auto enter = [&] {  // the unit that `ahead` has come to
-            const int kv_head = ahead.u / p.head_tiles;
-            constexpr int HEAD_BYTES = FMT == YUUKA_KV_F32 ? HD * 4 : (FMT == YUUKA_KV_F16 ? HD * 2 : (FMT == YUUKA_KV_Q8_0 ? HD / 32 * 34 : HD));
-            const int64_t at = (int64_t)kv_head * HEAD_BYTES;
-            k_at = p.cache.k + at + (S::IS_Q8 ? 4 * (lane & 7) : 16 * t);
-            v_at = p.cache.v + at + (S::IS_Q8 ? 4 * (lane & 7) : (S::IS_F8 ? S::F8_V : 16) * g);
+        auto enter = [&] {  // the row that `ahead` has come to
             table = p.cache.tables + (int64_t)max(ahead.seq, 0) * p.cache.table_stride;
         };
         enter();
@@ -501,19 +465,22 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                             }
                         }
                     } else if constexpr (!V) {
-                        constexpr int PIECES = S::K_BYTES / 1024;  // 16 bytes of keys g and g + 8, per lane
-                        const uint8_t * s0 = row_of(g);
-                        const uint8_t * s1 = row_of(g + 8);
-                        const uint32_t dst = put + lane * 16;
+                        if constexpr (S::K_LINES) {
 #pragma unroll
-                        for (int i = 0; i < PIECES; i++) {
-                            dec_copy<16>(dst + 1024 * i, s0 + 64 * i);
-                            dec_copy<16>(dst + 1024 * i + 512, s1 + 64 * i);
+                            for (int k = 0; k < 4; k++) {
+                                const int key = 4 * k + (lane >> 3);
+                                const uint8_t * src = row_of(key);
+#pragma unroll
+                                for (int i = 0; i < S::K_ROW / 128; i++) dec_copy<16>(put + S::k_piece(key, lane & 7) + 128 * i, src + 128 * i);
+                            }
+                        } else {
+                            dec_copy<16>(put + S::k_piece(g, t), row_of(g));
+                            dec_copy<16>(put + S::k_piece(g + 8, t), row_of(g + 8));
                         }
                         if constexpr (FMT == YUUKA_KV_F8) {
                             // scales: lanes 0-15 of K, 16-31 of V
                             const uint8_t * src = (lane < 16 ? p.cache.k : p.cache.v) + (uint64_t)pool_row * row_bytes +
-                                                  (p.cache.kv_heads * HD + 4 * (ahead.u / p.head_tiles));
+                                                  (p.cache.kv_heads * HD + 4 * kv_head);
                             dec_copy<4>(put + HD * 16 + 4 * lane, src);
                         }
                     } else {
@@ -531,7 +498,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 if constexpr (V) {
                     if (++fetched < count) {
                         const bool other = ahead.left == 1;
-                        ahead.next(p, units);
+                        ahead.next(p);
                         if (other) enter();
                         look_up();
                     }
@@ -557,7 +524,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
         bool from_start = false, fresh = true;
 
         auto load_queries = [&] {
-            const DecodeHeads h = decode_heads(p, use.u);
+            const DecodeHeads h = decode_heads(p, unit);
             const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
@@ -688,7 +655,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
         for (int it = 0; it < count; it++) {
             // ---- K: scores
             dec_wait<AHEAD - 1>();
-            if constexpr (S::SHARED_COPIES) __syncwarp();
+            __syncwarp();  // (lanes read what others have copied, and copy over what others have read)
             if constexpr (AHEAD & 1) fetch(std::true_type());
             else fetch(std::false_type());
             const uint32_t ks = take;
@@ -740,7 +707,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                     // three products of tf32 parts: hi hi, hi lo, lo hi (the tensor core itself drops what a first part leaves)
 #pragma unroll
                     for (int c = 0; c < HD / 16; c++) {
-                        const uint4 ka = dec_lds4(ks + lane * 16 + 1024 * c), kb = dec_lds4(ks + lane * 16 + 1024 * c + 512);
+                        const uint4 ka = dec_lds4(ks + S::k_piece(g, 4 * c + t)), kb = dec_lds4(ks + S::k_piece(g + 8, 4 * c + t));
                         const uint4 f = dec_lds4(q_at + 512 * c);
                         const uint32_t a[8] = {ka.x, kb.x, ka.y, kb.y, ka.z, kb.z, ka.w, kb.w};
                         const uint32_t b[4] = {f.x, f.y, f.z, f.w};
@@ -807,7 +774,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 } else if constexpr (S::IS_F8) {
 #pragma unroll
                     for (int c = 0; c < HD / 64; c++) {
-                        const uint4 ka = dec_lds4(ks + lane * 16 + 1024 * c), kb = dec_lds4(ks + lane * 16 + 1024 * c + 512);
+                        const uint4 ka = dec_lds4(ks + S::k_piece(g, 4 * c + t)), kb = dec_lds4(ks + S::k_piece(g + 8, 4 * c + t));
                         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
@@ -823,7 +790,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 } else {
 #pragma unroll
                     for (int c = 0; c < HD / 32; c++) {
-                        const uint4 ka = dec_lds4(ks + lane * 16 + 1024 * c), kb = dec_lds4(ks + lane * 16 + 1024 * c + 512);
+                        const uint4 ka = dec_lds4(ks + S::k_piece(g, 4 * c + t)), kb = dec_lds4(ks + S::k_piece(g + 8, 4 * c + t));
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             const uint4 f = query(nt, 2 * c), f2 = query(nt, 2 * c + 1);
@@ -906,7 +873,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 
             // ---- V: sums
             dec_wait<AHEAD - 1>();
-            if constexpr (S::SHARED_COPIES) __syncwarp();
+            __syncwarp();  // (lanes read what others have copied, and copy over what others have read)
             if constexpr (AHEAD & 1) fetch(std::false_type());
             else fetch(std::true_type());
             const uint32_t vs = take;
@@ -1048,8 +1015,8 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 16);
                     }
                 if constexpr (!S::IS_Q8 && !S::IS_F8) v_scale = 1.0f;
+                const DecodeHeads h = decode_heads(p, unit);
                 if (ends && from_start) {
-                    const DecodeHeads h = decode_heads(p, use.u);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -1083,19 +1050,14 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                             if (g == 0) dec_write_lse(p, use.b, h.first + col, m[nt][e], l[nt][e]);
                         }
                 } else {
-                    // a unit begun earlier goes to its own place; one begun here is the run's last, and its ring is done with
-                    // once every lane has used its copies
-                    float * part = head_part;
-                    if (from_start) {
-                        dec_wait<0>();
-                        __syncwarp();
-                        part = reinterpret_cast<float *>(ring_at);
-                    }
+                    // what other teams share: a row begun earlier (head), or one begun here that goes on (tail)
+                    float * const part = p.partial + (((size_t)team * units + unit) * 2 + from_start) * S::PART_FLOATS;
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             const int col = nt * 8 + 2 * t + e;
+                            if (col >= h.count) continue;
 #pragma unroll
                             for (int c = 0; c < CHUNKS; c++)
 #pragma unroll
@@ -1107,136 +1069,162 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                                 part[COLS * HD + COLS + col] = l[nt][e];
                             }
                         }
-                    if (lane == 0) {
-                        if (from_start) {
-                            tail_kind[warp] = 1;
-                            tail_b[warp] = use.b;
-                            tail_u[warp] = use.u;
-                            tail_end[warp] = begin + it + use.left;
-                        } else {
-                            head_kind[warp] = ends ? 1 : 2;
-                            if (warp == 0) {
-                                head_b = use.b;
-                                head_u = use.u;
-                            }
-                        }
+                    if (from_start && lane == 0) {
+                        const int last = (int)((begin + it + use.left - 1) / share);
+                        const int list = last - (int)team < DEC_SHORT_MOST ? DEC_SHORT : DEC_LONG;
+                        p.joins[list * DEC_WARPS + atomicAdd(p.counters + list, 1)] = make_int4(use.b, (int)unit, (int)team, last);
                     }
                 }
                 fresh = true;
             }
-            use.next(p, units);
+            use.next(p);
         }
         dec_wait<0>();
     }
-#ifdef DEC_TRIG
-    pdl_trigger_late();
-#endif
-    // ---- joining the warps' partials, in the order of the keys: first what an earlier CTA began, then what a warp here
-    // began (warp 0 of CTA 0 never begins inside a unit)
-    __syncthreads();
-    auto head_of = [&](int w) { return reinterpret_cast<const float *>(smem + W * S::RING + w * S::PART_BYTES); };
-#pragma unroll 1
-    for (int w = -1; w < W; w++) {
-        const bool tail = w >= 0;
-        if (!(tail ? tail_kind[w] : head_kind[0])) continue;
-        int n = 1;
-        bool ends = !tail && head_kind[0] == 1;
-        const int second = tail ? w + 1 : 1;
-        while (!ends && second + n - 1 < W && head_kind[second + n - 1]) ends = head_kind[second + n++ - 1] == 1;
-        const int b = tail ? tail_b[w] : head_b, u = tail ? tail_u[w] : head_u;
-        dec_join<HD, COLS, WIDE>(p, tail ? reinterpret_cast<const float *>(smem + w * S::RING) : head_of(0), head_of(min(second, W - 1)),
-                                 S::PART_BYTES / 4, n, ends && tail, b, u, scratch_at(tail), threadIdx.x, W * 32);
-        if (tail && !ends && threadIdx.x == 0)
-            p.joins[atomicAdd(p.counters + DEC_JOINS, 1)] = make_int4(b, u, (int)blockIdx.x, (int)((tail_end[w] - 1) / (share * W)));
     }
 }
 
-// The units that several CTAs share. A CTA takes a column of one at a time; groups of threads take every JOIN_GROUPS-th
-// partial, so that many loads are in flight, and are added in their order.
-constexpr int JOIN_THREADS = 256, JOIN_CTAS_SM = 4;
+// The units that several teams share. Few partials: a CTA takes a unit, a warp a column, a lane HD / 32 dimensions. Many: a CTA
+// takes 64 dimensions of a column at a time; groups of 16 threads take every 16th partial, so that many loads are in flight, and
+// are added in their order.
+constexpr int JOIN_THREADS = 256, JOIN_CTAS_SM = 4, JOIN_LANES = 16, JOIN_GROUPS = JOIN_THREADS / JOIN_LANES;
 template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_THREADS) attention_decode_join_kernel(const DecodeParams p) {
-    constexpr int PART = COLS * (HD + 2), LANES = HD / 4, GROUPS = JOIN_THREADS / LANES, EACH = DEC_CTAS / JOIN_THREADS;
-    __shared__ float factor[DEC_CTAS], reduce[2][JOIN_THREADS / 32];
-    __shared__ float4 sums[GROUPS][LANES];
+    constexpr int PART = COLS * (HD + 2), SLICES = HD / (4 * JOIN_LANES), DIMS = HD / 32;
+    __shared__ float factor[DEC_WARPS], reduce[2][JOIN_THREADS / 32];
+    __shared__ float4 sums[JOIN_GROUPS][JOIN_LANES];
     pdl_entry();
-    const int tid = threadIdx.x, dim = 4 * (tid % LANES), group = tid / LANES;
-    const int jobs = p.counters[DEC_JOINS] * COLS;
+    const int tid = threadIdx.x, units = p.cache.kv_heads * p.head_tiles, group = tid / JOIN_LANES;
+    const int few = p.counters[DEC_SHORT], jobs = p.counters[DEC_LONG] * COLS * SLICES;
+#pragma unroll 1
+    for (int job = blockIdx.x; job < few; job += gridDim.x) {
+        const int4 join = p.joins[job];
+        const DecodeHeads h = decode_heads(p, join.y);
+        const int n = join.w - join.z + 1, lane = tid & 31, dim = lane * DIMS;
+        const float * first = p.partial + ((size_t)join.z * units + join.y) * 2 * PART;
+        const int64_t stride = (int64_t)units * 2 * PART;
+        for (int col = tid >> 5; col < h.count; col += JOIN_THREADS / 32) {
+            const float * mine = first + lane * stride + (lane ? 0 : PART) + COLS * HD + col;
+            const float ms = lane < n ? mine[0] : -INFINITY, ls = lane < n ? mine[COLS] : 0.0f;
+            DecodeRaw<WIDE, DIMS> raw;
+            if (p.gate) raw.load(p.gate, join.x * p.q_row + (h.first + col) * p.q_head + dim);
+            float m = ms, x[DIMS];
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+            const float f = lane < n ? exp2f(ms - m) : 0.0f;
+            float l = f * ls;
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+#pragma unroll
+            for (int i = 0; i < DIMS; i++) x[i] = 0.0f;
+            constexpr int FLIGHT = 32 / DIMS;  // partials whose loads are in flight
+#pragma unroll 1
+            for (int k0 = 0; k0 < n; k0 += FLIGHT) {
+                DecodeRaw<true, DIMS> o[FLIGHT];
+#pragma unroll
+                for (int i = 0; i < FLIGHT; i++) {
+                    const int k = min(k0 + i, n - 1);
+                    o[i].fetch(first + k * stride + (k ? 0 : PART) + col * HD + dim);
+                }
+#pragma unroll
+                for (int i = 0; i < FLIGHT; i++) {
+                    const float fk = k0 + i < n ? __shfl_sync(0xffffffffu, f, k0 + i) : 0.0f;
+                    if (k0 + i < n)
+#pragma unroll
+                        for (int d = 0; d < DIMS; d++) x[d] = fmaf(fk, __uint_as_float(o[i].w[d]), x[d]);
+                }
+            }
+            float gates[DIMS];
+            if (p.gate) dec_gates<WIDE, DIMS>(p, raw, gates);
+#pragma unroll
+            for (int d = 0; d < DIMS; d++) x[d] = x[d] / l * (p.gate ? gates[d] : 1.0f);
+            dec_write<WIDE, DIMS>(p, join.x, h.first + col, dim, x);
+            if (lane == 0) dec_write_lse(p, join.x, h.first + col, m, l);
+        }
+    }
 #pragma unroll 1
     for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
-        const int4 join = p.joins[job / COLS];
-        const int col = job % COLS;
+        const int4 join = p.joins[DEC_WARPS + job / (COLS * SLICES)];
+        const int col = job / SLICES % COLS, dim = 4 * (job % SLICES * JOIN_LANES + tid % JOIN_LANES);
         const DecodeHeads h = decode_heads(p, join.y);
         if (col >= h.count) continue;
-        const int n = join.w - join.z + 1;  // partials: the tail of the first CTA and the heads of the following ones
-        const float * tail = p.partial + ((size_t)join.z * 2 + 1) * PART;
-        const float * heads = p.partial + (size_t)(join.z + 1) * 2 * PART;
-        auto part = [&](int k) { return k ? heads + (size_t)(k - 1) * 2 * PART : tail; };
+        const int n = join.w - join.z + 1;  // partials: the tail of the first team and the heads of the following ones
+        const float * first = p.partial + ((size_t)join.z * units + join.y) * 2 * PART;
+        const int64_t stride = (int64_t)units * 2 * PART;
+        auto part = [&](int k) { return first + k * stride + (k ? 0 : PART); };
         float gate[4] = {1.0f, 1.0f, 1.0f, 1.0f};
         if (p.gate && group == 0) {
             DecodeRaw<WIDE, 4> raw;
             raw.load(p.gate, join.x * p.q_row + (h.first + col) * p.q_head + dim);
             dec_gates<WIDE, 4>(p, raw, gate);
         }
-        float ms[EACH], ls[EACH], m = -INFINITY;
+        // the first loads of sums are on their way while the statistics are made
+        float4 o[4];
 #pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const int k = tid + i * JOIN_THREADS;
-            ms[i] = k < n ? part(k)[COLS * HD + col] : -INFINITY;
-            ls[i] = k < n ? part(k)[COLS * HD + COLS + col] : 0.0f;
-            m = fmaxf(m, ms[i]);
+        for (int i = 0; i < 4; i++) {
+            const int k = group + i * JOIN_GROUPS;
+            o[i] = k < n ? *reinterpret_cast<const float4 *>(part(k) + col * HD + dim) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
+        float m = -INFINITY;
+        for (int k = tid; k < n; k += JOIN_THREADS) m = fmaxf(m, part(k)[COLS * HD + col]);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
         if ((tid & 31) == 0) reduce[0][tid >> 5] = m;
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < JOIN_THREADS / 32; w++) m = fmaxf(m, reduce[0][w]);
         float l = 0.0f;
-#pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const int k = tid + i * JOIN_THREADS;
-            if (k < n) {
-                const float f = exp2f(ms[i] - m);
-                factor[k] = f;
-                l = fmaf(f, ls[i], l);
-            }
+        for (int k = tid; k < n; k += JOIN_THREADS) {
+            const float f = exp2f(part(k)[COLS * HD + col] - m);
+            factor[k] = f;
+            l = fmaf(f, part(k)[COLS * HD + COLS + col], l);
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
         if ((tid & 31) == 0) reduce[1][tid >> 5] = l;
         __syncthreads();
         l = 0.0f;
 #pragma unroll
         for (int w = 0; w < JOIN_THREADS / 32; w++) l += reduce[1][w];
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int k = group; k < n; k += GROUPS) {
-            const float f = factor[k];
-            const float4 o = *reinterpret_cast<const float4 *>(part(k) + col * HD + dim);
-            x.x = fmaf(f, o.x, x.x);
-            x.y = fmaf(f, o.y, x.y);
-            x.z = fmaf(f, o.z, x.z);
-            x.w = fmaf(f, o.w, x.w);
+#pragma unroll 1
+        for (int k0 = group; k0 < n; k0 += 4 * JOIN_GROUPS) {
+            if (k0 != group) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int k = k0 + i * JOIN_GROUPS;
+                    o[i] = k < n ? *reinterpret_cast<const float4 *>(part(k) + col * HD + dim) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int k = k0 + i * JOIN_GROUPS;
+                if (k >= n) continue;
+                const float f = factor[k];
+                x.x = fmaf(f, o[i].x, x.x);
+                x.y = fmaf(f, o[i].y, x.y);
+                x.z = fmaf(f, o[i].z, x.z);
+                x.w = fmaf(f, o[i].w, x.w);
+            }
         }
-        sums[group][tid % LANES] = x;
+        sums[group][tid % JOIN_LANES] = x;
         __syncthreads();
         if (group == 0) {
 #pragma unroll
-            for (int i = 1; i < GROUPS; i++) {
-                const float4 o = sums[i][tid];
-                x.x += o.x;
-                x.y += o.y;
-                x.z += o.z;
-                x.w += o.w;
+            for (int i = 1; i < JOIN_GROUPS; i++) {
+                const float4 y = sums[i][tid];
+                x.x += y.x;
+                x.y += y.y;
+                x.z += y.z;
+                x.w += y.w;
             }
             dec_write<WIDE, 4>(p, join.x, h.first + col, dim, {x.x / l * gate[0], x.y / l * gate[1], x.z / l * gate[2], x.w / l * gate[3]});
-            if (tid == 0) dec_write_lse(p, join.x, h.first + col, m, l);
+            if (dim == 0) dec_write_lse(p, join.x, h.first + col, m, l);
         }
         __syncthreads();
     }
-    // the last CTA leaves the counters as the call found them (every CTA has read its own above)
-    if (tid == 0 && atomicAdd(p.counters + DEC_DONE, 1) == (int)gridDim.x - 1)
-        p.counters[DEC_JOINS] = p.counters[DEC_DONE] = 0;
+    // the last CTA leaves the counters as the call found them
+    __syncthreads();
+    if (tid == 0 && atomicAdd(p.counters + DEC_DONE, 1) == (int)gridDim.x - 1) p.counters[DEC_SHORT] = p.counters[DEC_LONG] = p.counters[DEC_DONE] = 0;
 }
 
 // Launches for one format on a device with `sms` multiprocessors.
@@ -1248,7 +1236,7 @@ void launch_decode_f8(cudaStream_t s, const DecodeParams & p, int head_dim, int 
 template <int FMT, int HD, int NT, bool WIDE> void launch_decode_as(cudaStream_t s, DecodeParams p, int sms) {
     using S = DecodeShape<FMT, HD, NT, WIDE>;
     const int ctas = sms * S::RESIDENT;
-    YK_REQUIRE(ctas <= DEC_CTAS && ctas * 2 * S::PART_FLOATS * sizeof(float) <= DEC_PARTIAL_BYTES, YUUKA_ERR_UNSUPPORTED,
+    YK_REQUIRE(ctas * S::W <= DEC_WARPS && ctas * S::W * 2 * S::PART_FLOATS * sizeof(float) <= DEC_PARTIAL_BYTES, YUUKA_ERR_UNSUPPORTED,
                "attention_decode: %d multiprocessors", sms);
     auto kern = attention_decode_kernel<FMT, HD, NT, WIDE>;
     YK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::LAYOUT_BYTES));
