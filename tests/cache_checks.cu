@@ -210,25 +210,25 @@ int main() {
     p.lens = lens;
     p.seq_ids = seqs;
     p.batch = 6;
-    DecodeSpan s = decode_span(p, 0, bad);
+    DecodeSpan s = decode_span(p, 0, 16, bad);
     expect(s.tiles == 1 && s.end == 0 && s.seq == 0 && !bad, "a row without keys has a tile");
-    s = decode_span(p, 1, bad);
+    s = decode_span(p, 1, 16, bad);
     expect(s.tiles == 1 && s.first == 0 && s.end == 12 && s.seq == 1 && !bad, "a full table");
-    s = decode_span(p, 2, bad);
+    s = decode_span(p, 2, 16, bad);
     expect(s.tiles == 1 && s.end == 0 && s.seq == -1 && bad == YUUKA_KV_STATUS_POSITION, "a length beyond the table");
-    s = decode_span(p, 3, bad);
+    s = decode_span(p, 3, 16, bad);
     expect(s.tiles == 1 && s.end == 0 && s.seq == -1 && bad == YUUKA_KV_STATUS_POSITION, "a length below zero");
-    s = decode_span(p, 4, bad);
+    s = decode_span(p, 4, 16, bad);
     expect(s.tiles == 1 && s.seq == -1 && bad == YUUKA_KV_STATUS_SEQUENCE, "a sequence beyond the tables");
-    s = decode_span(p, 5, bad);
+    s = decode_span(p, 5, 16, bad);
     expect(s.tiles == 1 && s.seq == -1 && bad == YUUKA_KV_STATUS_SEQUENCE, "a sequence below the tables");
     p.window = 5;
-    s = decode_span(p, 1, bad);
+    s = decode_span(p, 1, 16, bad);
     expect(s.tiles == 1 && s.first == 7 && s.end == 12, "a window");
     p.cache.capacity = INT_MAX;
     lens[1] = INT_MAX;
     p.window = 0;
-    s = decode_span(p, 1, bad);
+    s = decode_span(p, 1, 16, bad);
     expect(s.tiles == 1 << 27 && s.end == INT_MAX && !bad, "the longest sequence");
 
     expect(yuuka_kv_row_bytes(YUUKA_KV_F32, 3, 64) == 768 && yuuka_kv_row_bytes(YUUKA_KV_F16, 3, 64) == 384 &&

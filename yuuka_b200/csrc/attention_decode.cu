@@ -143,7 +143,7 @@ extern "C" yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_atte
         p.joins = (int4 *)(scratch->memory + DEC_COUNTER_BYTES);
         p.partial = (float *)(scratch->memory + DEC_COUNTER_BYTES + 2 * DEC_WARPS * sizeof(int4));
         // tiles are counted in 31 bits
-        const double tiles = (double)a->batch * cache->kv_heads * p.head_tiles * (p.cache.capacity / DEC_TILE + 1.0);
+        const double tiles = (double)a->batch * cache->kv_heads * p.head_tiles * (p.cache.capacity / 16 + 1.0);
         YK_REQUIRE(tiles < 2e9, YUUKA_ERR_UNSUPPORTED, "%s: %g tiles of keys are too many for one call", op, tiles);
         set_device(dev);
         switch (cache->format) {

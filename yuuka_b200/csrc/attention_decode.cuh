@@ -49,7 +49,6 @@ struct DecodeParams {
     int * counters;    // zero between calls: joins of both lists, CTAs of the joining kernel done
 };
 
-constexpr int DEC_TILE = 16;            // keys
 #ifndef DEC_MIN_TILES
 #define DEC_MIN_TILES 1
 #endif
@@ -157,13 +156,21 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     static constexpr bool NARROW = NT == 2 || (IS_F32 && HD > 64);
     static constexpr int W = NARROW ? 4 : HD == 256 ? DEC_W256 : HD == 128 ? DEC_W128 : DEC_W64;
     static constexpr int RESIDENT = NARROW ? (HD == 256 ? 1 : 2) : HD == 256 ? DEC_R256 : HD == 128 ? DEC_R128 : DEC_R64;
+#ifndef DEC_K256
+#define DEC_K256 1
+#define DEC_K128 2
+#define DEC_K64 2
+#endif
+    // keys of a tile: sixteen make one row tile of the products
+    static constexpr int HALVES = IS_F32 && HD > 64 ? 1 : HD == 256 ? DEC_K256 : HD == 128 ? DEC_K128 : DEC_K64, KEYS = 16 * HALVES;
     static constexpr int COLS = 8 * NT, PARTS = WIDE ? 2 : 1;
     // Q8_0: words from key to key. K: 8 or 24 modulo 32, V: 4 or 12 modulo 16, which keeps the lanes' reads on different banks
     static constexpr int Q8_K = HD == 64 ? 24 : (HD == 128 ? 40 : 88), Q8_V = HD == 64 ? 20 : (HD == 128 ? 36 : 68);
     // F8: a lane's piece of V, 16 dimensions of 128 or 8 of 64; the scales of the tile's K and V lie behind K
     static constexpr int F8_V = HD == 64 ? 8 : 16;
-    static constexpr int K_BYTES = IS_F32 ? HD * 64 : (IS_Q8 ? 64 * Q8_K : (IS_F8 ? HD * 16 + 128 : HD * 32));
-    static constexpr int V_BYTES = IS_F32 ? HD * 64 : (IS_Q8 ? 64 * Q8_V : (IS_F8 ? HD * 16 : HD * 32));
+    static constexpr int K16 = IS_F32 ? HD * 64 : (IS_Q8 ? 64 * Q8_K : (IS_F8 ? HD * 16 : HD * 32));  // bytes of sixteen keys
+    static constexpr int V16 = IS_F32 ? HD * 64 : (IS_Q8 ? 64 * Q8_V : (IS_F8 ? HD * 16 : HD * 32));
+    static constexpr int K_BYTES = K16 * HALVES + (IS_F8 ? 8 * KEYS : 0), V_BYTES = V16 * HALVES;
     // K of the other formats: a key's row, its 16-byte pieces copied by lines of 128 bytes, eight lanes to a line (one request
     // to memory instead of two: 239 -> 227 us for 8 sequences of 32768, 8 KV heads of 128). In odd keys the halves of a line
     // trade places, so that the eight lanes that read four pieces of two keys find them on different banks.
@@ -218,7 +225,7 @@ struct DecodeSpan {
     int tiles;       // at least one, so that a row without keys is written too
     int seq;         // its sequence; -1: out of range
 };
-__host__ __device__ __forceinline__ DecodeSpan decode_span(const DecodeParams & p, int b, int & bad) {
+__host__ __device__ __forceinline__ DecodeSpan decode_span(const DecodeParams & p, int b, int keys, int & bad) {  // keys of a tile
     DecodeSpan s;
     const int n = kv_load(p.lens + b);
     s.seq = p.seq_ids ? kv_load(p.seq_ids + b) : b;
@@ -227,30 +234,30 @@ __host__ __device__ __forceinline__ DecodeSpan decode_span(const DecodeParams & 
     else if (n < 0 || n > p.cache.capacity) bad = KV_BAD_POSITION;
     s.end = bad ? 0 : n;
     s.first = p.window > 0 && s.end > p.window ? s.end - p.window : 0;
-    s.tiles = s.end > s.first ? (s.end - s.first - 1) / DEC_TILE + 1 : 1;
+    s.tiles = s.end > s.first ? (s.end - s.first - 1) / keys + 1 : 1;
     if (bad) s.seq = -1;
     return s;
 }
-__device__ __forceinline__ DecodeSpan decode_span(const DecodeParams & p, int b) {
+__device__ __forceinline__ DecodeSpan decode_span(const DecodeParams & p, int b, int keys) {
     int bad;
-    return decode_span(p, b, bad);
+    return decode_span(p, b, keys, bad);
 }
 
 // A place in the sequence of tiles: the next one of row b.
-struct DecodeCursor {
+template <int KEYS> struct DecodeCursor {
     int b;
     int pos, end;           // its first key; behind the row's last key
     int left;               // tiles of the row from here on
     int first, tiles, seq;  // of the row
     __device__ __forceinline__ void row(const DecodeParams & p) {
-        const DecodeSpan s = decode_span(p, b);
+        const DecodeSpan s = decode_span(p, b, KEYS);
         first = s.first;
         end = s.end;
         tiles = s.tiles;
         seq = s.seq;
     }
     __device__ __forceinline__ void next(const DecodeParams & p) {
-        pos += DEC_TILE;
+        pos += KEYS;
         if (--left > 0) return;
         if (++b < p.batch) row(p);
         pos = first;
@@ -353,7 +360,7 @@ __device__ __forceinline__ DecodeHeads decode_heads(const DecodeParams & p, int 
 template <int FMT, int HD, int NT, bool WIDE>
 __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, DecodeShape<FMT, HD, NT, WIDE>::RESIDENT) attention_decode_kernel(const DecodeParams p) {
     using S = DecodeShape<FMT, HD, NT, WIDE>;
-    constexpr int W = S::W, COLS = S::COLS, AHEAD = S::AHEAD, CHUNKS = S::CHUNKS, DPL = S::DPL;
+    constexpr int W = S::W, COLS = S::COLS, AHEAD = S::AHEAD, CHUNKS = S::CHUNKS, DPL = S::DPL, HALVES = S::HALVES, KEYS = S::KEYS;
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * S::RING);
@@ -364,7 +371,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
     unsigned total = 0;  // (below 2^31: the host has checked)
     for (int b = lane; b < p.batch; b += 32) {
         int bad;
-        total += decode_span(p, b, bad).tiles;
+        total += decode_span(p, b, KEYS, bad).tiles;
         if (bad && p.status && blockIdx.x == 0 && warp == 0) atomicOr(p.status, bad);
     }
     total = __reduce_add_sync(0xffffffffu, total);
@@ -377,13 +384,13 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
     for (unsigned unit = units > warps ? self : self - team * units; unit < units; unit += warps) {
     if (count == 0) break;
     {
-        DecodeCursor use;
+        DecodeCursor<KEYS> use;
         {
             unsigned before = 0;
             use.b = 0;
             for (int base = 0; base < p.batch; base += 32) {  // (begin < total: some row holds it)
                 const int b = base + lane;
-                const unsigned mine = b < p.batch ? (unsigned)decode_span(p, b).tiles : 0;
+                const unsigned mine = b < p.batch ? (unsigned)decode_span(p, b, KEYS).tiles : 0;
                 unsigned sum = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -401,15 +408,15 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
             }
             use.row(p);
             const int tile = min((int)(begin - before), use.tiles - 1);  // (it is less, unless lengths change under the call)
-            use.pos = use.first + tile * DEC_TILE;
+            use.pos = use.first + tile * KEYS;
             use.left = use.tiles - tile;
         }
 
         // -- copies. Keys behind the last one of a unit's last tile repeat it (their probabilities become zero), so a copy is
         // always whole; a tile of a bad block becomes NaN, and a unit without keys copies nothing.
-        DecodeCursor ahead = use;
+        DecodeCursor<KEYS> ahead = use;
         int fetched = 0;                   // tiles of the run whose V has been asked for
-        unsigned block_of = 0, within = 0; // of key lane % 16 of the next tile
+        unsigned block_of = 0, within = 0; // of key lane % KEYS of the next tile
         unsigned pool_row = 0;
         bool copies = false;
         // the pools at the unit's head and this lane's piece
@@ -421,7 +428,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
         const unsigned row_bytes = (unsigned)p.cache.row_bytes;
         auto look_up = [&] {
             if (ahead.pos >= ahead.end) return;
-            const int pos = min(ahead.pos + (lane & 15), ahead.end - 1);
+            const int pos = min(ahead.pos + (lane & (KEYS - 1)), ahead.end - 1);
             const int page = p.cache.shift >= 0 ? pos >> p.cache.shift : pos / p.cache.block_size;
             within = pos - page * p.cache.block_size;
             block_of = (unsigned)__ldg(table + page);
@@ -452,7 +459,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         constexpr int WORDS = HD / 32 * 34 / 4;
                         const int l8 = lane & 7;
 #pragma unroll
-                        for (int kg = 0; kg < 4; kg++) {
+                        for (int kg = 0; kg < KEYS / 4; kg++) {
                             const int key = 4 * kg + (lane >> 3);
                             const uint8_t * src = row_of(key);
                             const uint32_t dst = put + 4 * (V ? key * S::Q8_V : key * S::Q8_K + 1) + 4 * l8;
@@ -467,32 +474,39 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                     } else if constexpr (!V) {
                         if constexpr (S::K_LINES) {
 #pragma unroll
-                            for (int k = 0; k < 4; k++) {
+                            for (int k = 0; k < KEYS / 4; k++) {
                                 const int key = 4 * k + (lane >> 3);
                                 const uint8_t * src = row_of(key);
 #pragma unroll
                                 for (int i = 0; i < S::K_ROW / 128; i++) dec_copy<16>(put + S::k_piece(key, lane & 7) + 128 * i, src + 128 * i);
                             }
                         } else {
-                            dec_copy<16>(put + S::k_piece(g, t), row_of(g));
-                            dec_copy<16>(put + S::k_piece(g + 8, t), row_of(g + 8));
+#pragma unroll
+                            for (int k = 0; k < KEYS / 8; k++) dec_copy<16>(put + S::k_piece(g + 8 * k, t), row_of(g + 8 * k));
                         }
                         if constexpr (FMT == YUUKA_KV_F8) {
-                            // scales: lanes 0-15 of K, 16-31 of V
-                            const uint8_t * src = (lane < 16 ? p.cache.k : p.cache.v) + (uint64_t)pool_row * row_bytes +
-                                                  (p.cache.kv_heads * HD + 4 * kv_head);
-                            dec_copy<4>(put + HD * 16 + 4 * lane, src);
+                            // scales of K and behind them of V
+                            const uint64_t at = (uint64_t)pool_row * row_bytes + (p.cache.kv_heads * HD + 4 * kv_head);
+                            const uint32_t dst = put + S::K16 * HALVES + 4 * lane;
+                            if constexpr (HALVES == 2) {
+                                dec_copy<4>(dst, p.cache.k + at);
+                                dec_copy<4>(dst + 128, p.cache.v + at);
+                            } else {
+                                dec_copy<4>(dst, (lane < 16 ? p.cache.k : p.cache.v) + at);
+                            }
                         }
                     } else {
                         constexpr int PIECE = FMT == YUUKA_KV_F8 ? S::F8_V : 16;  // a lane's bytes of keys 2t, 2t + 1, 2t + 8, 2t + 9
-                        constexpr int PIECES = S::V_BYTES / (128 * PIECE);
-                        const uint32_t dst = put + lane * PIECE;
+                        constexpr int PIECES = S::V16 / (128 * PIECE);
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint8_t * src = row_of(2 * t + (k & 1) + 8 * (k >> 1));
+                        for (int h = 0; h < HALVES; h++)
 #pragma unroll
-                            for (int i = 0; i < PIECES; i++) dec_copy<PIECE>(dst + (i * 4 + k) * 32 * PIECE, src + 8 * PIECE * i);
-                        }
+                            for (int k = 0; k < 4; k++) {
+                                const uint8_t * src = row_of(16 * h + 2 * t + (k & 1) + 8 * (k >> 1));
+                                const uint32_t dst = put + S::V16 * h + lane * PIECE + k * 32 * PIECE;
+#pragma unroll
+                                for (int i = 0; i < PIECES; i++) dec_copy<PIECE>(dst + i * 128 * PIECE, src + 8 * PIECE * i);
+                            }
                     }
                 }
                 if constexpr (V) {
@@ -634,19 +648,22 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 rescale(f);
                 v_scale = v;
             }
-            return __fdividef(1.0f, v_scale);  // (exact: a power of two)
+            return v_scale < 1.7e38f ? __uint_as_float(0x7f000000u - __float_as_uint(v_scale)) : 1.0f / v_scale;  // (a power of two)
         };
         // o += a P^T for product j of a chunk. The tensor core cuts sums off instead of rounding them: over thousands of tiles
         // that would cost an f32 result 2^-17, so such a tile is summed on its own and added in f32
-        auto add_values = [&](float (&acc)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[S::PARTS][2]) {
+        auto add_values = [&](float (&acc)[4], int nt, const uint32_t (&a)[HALVES][4], const uint32_t (&b)[HALVES][NT][S::PARTS][2]) {
             if constexpr (WIDE) {
                 float d[4] = {0.f, 0.f, 0.f, 0.f};
-                dec_mma16(d, a0, a1, a2, a3, b[1][0], b[1][1]);
-                dec_mma16(d, a0, a1, a2, a3, b[0][0], b[0][1]);
+#pragma unroll
+                for (int h = 0; h < HALVES; h++) dec_mma16(d, a[h][0], a[h][1], a[h][2], a[h][3], b[h][nt][S::PARTS - 1][0], b[h][nt][S::PARTS - 1][1]);
+#pragma unroll
+                for (int h = 0; h < HALVES; h++) dec_mma16(d, a[h][0], a[h][1], a[h][2], a[h][3], b[h][nt][0][0], b[h][nt][0][1]);
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[e] += d[e];
             } else {
-                dec_mma16(acc, a0, a1, a2, a3, b[0][0], b[0][1]);
+#pragma unroll
+                for (int h = 0; h < HALVES; h++) dec_mma16(acc, a[h][0], a[h][1], a[h][2], a[h][3], b[h][nt][0][0], b[h][nt][0][1]);
             }
         };
 
@@ -681,23 +698,29 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
             }
             const int keys = use.end - use.pos;  // of the unit from here on; 0 for a row without any
 
-            uint32_t pb[NT][S::PARTS][2];  // probabilities as fragments: keys become the dimension that is summed over
-            float s[NT][4];
-            auto fragments = [&](float f0, float f1) {  // with factors of keys g and g + 8
+            // probabilities as fragments: keys become the dimension that is summed over
+            uint32_t pb[HALVES][NT][S::PARTS][2];
+            float sh[HALVES][NT][4];
+            auto fragments = [&](int h, float f0, float f1) {  // of the h-th sixteen keys, with factors of keys g and g + 8
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    const float x0 = s[nt][0] * f0, x1 = s[nt][1] * f0, y0 = s[nt][2] * f1, y1 = s[nt][3] * f1;
+                    const float x0 = sh[h][nt][0] * f0, x1 = sh[h][nt][1] * f0, y0 = sh[h][nt][2] * f1, y1 = sh[h][nt][3] * f1;
                     const uint32_t hx = dec_pack(x0, x1), hy = dec_pack(y0, y1);
-                    pb[nt][0][0] = dec_transpose(hx);
-                    pb[nt][0][1] = dec_transpose(hy);
+                    pb[h][nt][0][0] = dec_transpose(hx);
+                    pb[h][nt][0][1] = dec_transpose(hy);
                     if constexpr (WIDE) {
                         const float2 rx = dec_unpack(hx), ry = dec_unpack(hy);
-                        pb[nt][1][0] = dec_transpose(dec_pack(x0 - rx.x, x1 - rx.y));
-                        pb[nt][1][1] = dec_transpose(dec_pack(y0 - ry.x, y1 - ry.y));
+                        pb[h][nt][1][0] = dec_transpose(dec_pack(x0 - rx.x, x1 - rx.y));
+                        pb[h][nt][1][1] = dec_transpose(dec_pack(y0 - ry.x, y1 - ry.y));
                     }
                 }
             };
             if (keys > 0) {  // (uniform)
+                float vd[HALVES][2];  // F8: scales of V of keys g and g + 8
+#pragma unroll
+                for (int half = 0; half < HALVES; half++) {
+                float (&s)[NT][4] = sh[half];
+                const uint32_t kh = ks + half * S::K16;
                 float s2[NT][4];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -707,7 +730,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                     // three products of tf32 parts: hi hi, hi lo, lo hi (the tensor core itself drops what a first part leaves)
 #pragma unroll
                     for (int c = 0; c < HD / 16; c++) {
-                        const uint4 ka = dec_lds4(ks + S::k_piece(g, 4 * c + t)), kb = dec_lds4(ks + S::k_piece(g + 8, 4 * c + t));
+                        const uint4 ka = dec_lds4(kh + S::k_piece(g, 4 * c + t)), kb = dec_lds4(kh + S::k_piece(g + 8, 4 * c + t));
                         const uint4 f = dec_lds4(q_at + 512 * c);
                         const uint32_t a[8] = {ka.x, kb.x, ka.y, kb.y, ka.z, kb.z, ka.w, kb.w};
                         const uint32_t b[4] = {f.x, f.y, f.z, f.w};
@@ -726,7 +749,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         }
                     }
                 } else if constexpr (S::IS_Q8) {
-                    const uint32_t ka = ks + 4 * (g * S::Q8_K + 1), kb = ka + 32 * S::Q8_K;  // keys g and g + 8
+                    const uint32_t ka = kh + 4 * (g * S::Q8_K + 1), kb = ka + 32 * S::Q8_K;  // keys g and g + 8
 #pragma unroll
                     for (int pair = 0; pair < HD / 64; pair++) {
                         uint32_t w[2][4];   // [key][word]: two of the even block, two of the odd one
@@ -774,7 +797,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 } else if constexpr (S::IS_F8) {
 #pragma unroll
                     for (int c = 0; c < HD / 64; c++) {
-                        const uint4 ka = dec_lds4(ks + S::k_piece(g, 4 * c + t)), kb = dec_lds4(ks + S::k_piece(g + 8, 4 * c + t));
+                        const uint4 ka = dec_lds4(kh + S::k_piece(g, 4 * c + t)), kb = dec_lds4(kh + S::k_piece(g + 8, 4 * c + t));
                         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
@@ -790,7 +813,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 } else {
 #pragma unroll
                     for (int c = 0; c < HD / 32; c++) {
-                        const uint4 ka = dec_lds4(ks + S::k_piece(g, 4 * c + t)), kb = dec_lds4(ks + S::k_piece(g + 8, 4 * c + t));
+                        const uint4 ka = dec_lds4(kh + S::k_piece(g, 4 * c + t)), kb = dec_lds4(kh + S::k_piece(g + 8, 4 * c + t));
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             const uint4 f = query(nt, 2 * c), f2 = query(nt, 2 * c + 1);
@@ -808,11 +831,11 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int e = 0; e < 4; e++) s[nt][e] += s2[nt][e];
-                float vd[2] = {1.0f, 1.0f};  // F8: scales of V of keys g and g + 8
                 if constexpr (S::IS_F8) {
-                    const float d0 = __uint_as_float(dec_lds(ks + HD * 16 + 4 * g)), d1 = __uint_as_float(dec_lds(ks + HD * 16 + 4 * (g + 8)));
-                    vd[0] = __uint_as_float(dec_lds(ks + HD * 16 + 64 + 4 * g));
-                    vd[1] = __uint_as_float(dec_lds(ks + HD * 16 + 64 + 4 * (g + 8)));
+                    const uint32_t at = ks + S::K16 * HALVES + 64 * half + 4 * g;
+                    const float d0 = __uint_as_float(dec_lds(at)), d1 = __uint_as_float(dec_lds(at + 32));
+                    vd[half][0] = __uint_as_float(dec_lds(at + 4 * KEYS));
+                    vd[half][1] = __uint_as_float(dec_lds(at + 4 * KEYS + 32));
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
                         s[nt][0] *= d0;
@@ -821,14 +844,17 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         s[nt][3] *= d1;
                     }
                 }
+                }
 
                 // ---- running maximum and sum; s becomes the probabilities of keys g (0, 1) and g + 8 (2, 3), columns 2t and 2t + 1
-                if (keys < DEC_TILE) {
+                if (keys < KEYS) {
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
+                    for (int h = 0; h < HALVES; h++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (g + 8 * (e >> 1) >= keys) s[nt][e] = -INFINITY;
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (16 * h + g + 8 * (e >> 1) >= keys) sh[h][nt][e] = -INFINITY;
                 }
                 float top[NT][2];
                 bool moved = false;
@@ -836,7 +862,8 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        float mx = fmaxf(s[nt][c], s[nt][c + 2]);
+                        float mx = fmaxf(sh[0][nt][c], sh[0][nt][c + 2]);
+                        if constexpr (HALVES == 2) mx = fmaxf(mx, fmaxf(sh[1][nt][c], sh[1][nt][c + 2]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -860,14 +887,23 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
                         const float base = DEC_P_LOG2 - m[nt][c];
-                        s[nt][c] = dec_exp2(fmaf(s[nt][c], scale[nt][c], base));
-                        s[nt][c + 2] = dec_exp2(fmaf(s[nt][c + 2], scale[nt][c], base));
-                        l[nt][c] += s[nt][c] + s[nt][c + 2];
+#pragma unroll
+                        for (int h = 0; h < HALVES; h++) {
+                            sh[h][nt][c] = dec_exp2(fmaf(sh[h][nt][c], scale[nt][c], base));
+                            sh[h][nt][c + 2] = dec_exp2(fmaf(sh[h][nt][c + 2], scale[nt][c], base));
+                            l[nt][c] += sh[h][nt][c] + sh[h][nt][c + 2];
+                        }
                     }
-                if constexpr (FMT == YUUKA_KV_F16) fragments(1.0f, 1.0f);
-                else if constexpr (S::IS_F8) {
-                    const float inv = take_v_scale(max(__float_as_uint(fabsf(vd[0])), __float_as_uint(fabsf(vd[1]))));
-                    fragments(vd[0] * inv, vd[1] * inv);
+                if constexpr (FMT == YUUKA_KV_F16) {
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++) fragments(h, 1.0f, 1.0f);
+                } else if constexpr (S::IS_F8) {
+                    uint32_t largest = 0;
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++) largest = max(largest, max(__float_as_uint(fabsf(vd[h][0])), __float_as_uint(fabsf(vd[h][1]))));
+                    const float inv = take_v_scale(largest);
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++) fragments(h, vd[h][0] * inv, vd[h][1] * inv);
                 }
             }
 
@@ -881,123 +917,145 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 
             if (keys > 0) {
                 if constexpr (S::IS_F32) {
-                    // probabilities in f32 change hands as two 16-bit halves; lane (g, t) then has keys 2t, 2t + 1 (and + 8) of column g
-                    uint32_t pk[4], pl[4];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t x = __float_as_uint(s[0][2 * h]), y = __float_as_uint(s[0][2 * h + 1]);
-                        const uint32_t low = dec_transpose(__byte_perm(x, y, 0x5410)), high = dec_transpose(__byte_perm(x, y, 0x7632));
-                        pk[2 * h] = __byte_perm(low, high, 0x5410);
-                        pk[2 * h + 1] = __byte_perm(low, high, 0x7632);
-                    }
+                    for (int half = 0; half < HALVES; half++) {
+                        // probabilities in f32 change hands as two 16-bit halves; lane (g, t) then has keys 2t, 2t + 1 (and + 8) of column g
+                        uint32_t pk[4], pl[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) pl[i] = dec_rest(pk[i]);
-#pragma unroll
-                    for (int c = 0; c < CHUNKS; c++) {
-                        uint32_t v[4][4];
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint4 r = dec_lds4(vs + lane * 16 + (c * 4 + k) * 512);
-                            v[k][0] = r.x; v[k][1] = r.y; v[k][2] = r.z; v[k][3] = r.w;
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t x = __float_as_uint(sh[half][0][2 * h]), y = __float_as_uint(sh[half][0][2 * h + 1]);
+                            const uint32_t low = dec_transpose(__byte_perm(x, y, 0x5410)), high = dec_transpose(__byte_perm(x, y, 0x7632));
+                            pk[2 * h] = __byte_perm(low, high, 0x5410);
+                            pk[2 * h + 1] = __byte_perm(low, high, 0x7632);
                         }
 #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            float d[4] = {0.f, 0.f, 0.f, 0.f};  // (summed on its own, as in add_values)
+                        for (int i = 0; i < 4; i++) pl[i] = dec_rest(pk[i]);
 #pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                const uint32_t a[4] = {v[2 * h][2 * j], v[2 * h][2 * j + 1], v[2 * h + 1][2 * j], v[2 * h + 1][2 * j + 1]};
-                                uint32_t al[4];
+                        for (int c = 0; c < CHUNKS; c++) {
+                            uint32_t v[4][4];
 #pragma unroll
-                                for (int i = 0; i < 4; i++) al[i] = dec_rest(a[i]);
-                                dec_mma8(d, al[0], al[1], al[2], al[3], pk[2 * h], pk[2 * h + 1]);
-                                dec_mma8(d, a[0], a[1], a[2], a[3], pl[2 * h], pl[2 * h + 1]);
-                                dec_mma8(d, a[0], a[1], a[2], a[3], pk[2 * h], pk[2 * h + 1]);
+                            for (int k = 0; k < 4; k++) {
+                                const uint4 r = dec_lds4(vs + half * S::V16 + lane * 16 + (c * 4 + k) * 512);
+                                v[k][0] = r.x; v[k][1] = r.y; v[k][2] = r.z; v[k][3] = r.w;
                             }
 #pragma unroll
-                            for (int e = 0; e < 4; e++) o[0][c][j][e] += d[e];
+                            for (int j = 0; j < 2; j++) {
+                                float d[4] = {0.f, 0.f, 0.f, 0.f};  // (summed on its own, as in add_values)
+#pragma unroll
+                                for (int h = 0; h < 2; h++) {
+                                    const uint32_t a[4] = {v[2 * h][2 * j], v[2 * h][2 * j + 1], v[2 * h + 1][2 * j], v[2 * h + 1][2 * j + 1]};
+                                    uint32_t al[4];
+#pragma unroll
+                                    for (int i = 0; i < 4; i++) al[i] = dec_rest(a[i]);
+                                    dec_mma8(d, al[0], al[1], al[2], al[3], pk[2 * h], pk[2 * h + 1]);
+                                    dec_mma8(d, a[0], a[1], a[2], a[3], pl[2 * h], pl[2 * h + 1]);
+                                    dec_mma8(d, a[0], a[1], a[2], a[3], pk[2 * h], pk[2 * h + 1]);
+                                }
+#pragma unroll
+                                for (int e = 0; e < 4; e++) o[0][c][j][e] += d[e];
+                            }
                         }
                     }
                 } else if constexpr (S::IS_Q8) {
                     // scales of V: of keys g and g + 8, block by block, into the probabilities
-                    const uint32_t va = vs + 4 * g * S::Q8_V, vb = va + 32 * S::Q8_V;
-                    float d[2][HD / 32];
-                    uint32_t top = 0;
+                    float d[HALVES][2][HD / 32];
+                    uint32_t largest = 0;
 #pragma unroll
-                    for (int blk = 0; blk < HD / 32; blk++) {
-                        const uint32_t x = dec_lds_u16(va + 34 * blk), y = dec_lds_u16(vb + 34 * blk);
-                        d[0][blk] = __half2float(__ushort_as_half((unsigned short)x));
-                        d[1][blk] = __half2float(__ushort_as_half((unsigned short)y));
-                        top = max(top, max(__float_as_uint(fabsf(d[0][blk])), __float_as_uint(fabsf(d[1][blk]))));
-                    }
-                    const float inv = take_v_scale(top);
+                    for (int h = 0; h < HALVES; h++)
+#pragma unroll
+                        for (int k = 0; k < 2; k++)
+#pragma unroll
+                            for (int blk = 0; blk < HD / 32; blk++) {
+                                d[h][k][blk] = __half2float(__ushort_as_half((unsigned short)dec_lds_u16(vs + h * S::V16 + 4 * (g + 8 * k) * S::Q8_V + 34 * blk)));
+                                largest = max(largest, __float_as_uint(fabsf(d[h][k][blk])));
+                            }
+                    const float inv = take_v_scale(largest);
 #pragma unroll
                     for (int c = 0; c < CHUNKS; c++) {
-                        fragments(d[0][c] * inv, d[1][c] * inv);
-                        uint32_t w[4];
+                        uint32_t a[2][HALVES][4];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint32_t at = vs + 4 * (2 * t + (k & 1) + 8 * (k >> 1)) * S::Q8_V + 68 * (c >> 1);
-                            if (c & 1) w[k] = dec_lds(at + 4 * (9 + g));
-                            else {
-                                const uint32_t x = dec_lds(at + 4 * (1 + g)), w0 = dec_lds(at);
-                                w[k] = g == 7 ? __byte_perm(x, w0, 0x7610) : x;
+                        for (int h = 0; h < HALVES; h++) {
+                            fragments(h, d[h][0][c] * inv, d[h][1][c] * inv);
+                            uint32_t w[4];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const uint32_t at = vs + h * S::V16 + 4 * (2 * t + (k & 1) + 8 * (k >> 1)) * S::Q8_V + 68 * (c >> 1);
+                                if (c & 1) w[k] = dec_lds(at + 4 * (9 + g));
+                                else {
+                                    const uint32_t x = dec_lds(at + 4 * (1 + g)), w0 = dec_lds(at);
+                                    w[k] = g == 7 ? __byte_perm(x, w0, 0x7610) : x;
+                                }
+                                w[k] ^= 0x80808080u;
                             }
-                            w[k] ^= 0x80808080u;
-                        }
-                        const uint32_t x01 = __byte_perm(w[0], w[1], 0x5140), x23 = __byte_perm(w[0], w[1], 0x7362);
-                        const uint32_t y01 = __byte_perm(w[2], w[3], 0x5140), y23 = __byte_perm(w[2], w[3], 0x7362);
+                            const uint32_t x01 = __byte_perm(w[0], w[1], 0x5140), x23 = __byte_perm(w[0], w[1], 0x7362);
+                            const uint32_t y01 = __byte_perm(w[2], w[3], 0x5140), y23 = __byte_perm(w[2], w[3], 0x7362);
 #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const uint32_t x = j ? x23 : x01, y = j ? y23 : y01;
-                            const uint32_t a0 = dec_int8<0>(x), a1 = dec_int8<1>(x), a2 = dec_int8<0>(y), a3 = dec_int8<1>(y);
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) add_values(o[nt][c][j], a0, a1, a2, a3, pb[nt]);
+                            for (int j = 0; j < 2; j++) {
+                                a[j][h][0] = dec_int8<0>(j ? x23 : x01);
+                                a[j][h][1] = dec_int8<1>(j ? x23 : x01);
+                                a[j][h][2] = dec_int8<0>(j ? y23 : y01);
+                                a[j][h][3] = dec_int8<1>(j ? y23 : y01);
+                            }
                         }
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) add_values(o[nt][c][j], nt, a[j], pb);
                     }
                 } else if constexpr (S::IS_F8) {
                     constexpr int WORDS = S::F8_V / 4;
 #pragma unroll
                     for (int c = 0; c < CHUNKS; c++) {
-                        uint32_t v[4][WORDS];
+                        uint32_t v[HALVES][4][WORDS];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint32_t at = vs + lane * S::F8_V + (c * 4 + k) * 32 * S::F8_V;
-                            if constexpr (WORDS == 4) {
-                                const uint4 r = dec_lds4(at);
-                                v[k][0] = r.x; v[k][1] = r.y; v[k][2] = r.z; v[k][3] = r.w;
-                            } else {
-                                const uint2 r = dec_lds2(at);
-                                v[k][0] = r.x; v[k][1] = r.y;
+                        for (int h = 0; h < HALVES; h++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const uint32_t at = vs + h * S::V16 + lane * S::F8_V + (c * 4 + k) * 32 * S::F8_V;
+                                if constexpr (WORDS == 4) {
+                                    const uint4 r = dec_lds4(at);
+                                    v[h][k][0] = r.x; v[h][k][1] = r.y; v[h][k][2] = r.z; v[h][k][3] = r.w;
+                                } else {
+                                    const uint2 r = dec_lds2(at);
+                                    v[h][k][0] = r.x; v[h][k][1] = r.y;
+                                }
                             }
-                        }
 #pragma unroll
-                        for (int w = 0; w < WORDS; w++) {
-                            // bytes of two keys next to one another: values of one dimension
-                            const uint32_t x01 = __byte_perm(v[0][w], v[1][w], 0x5140), x23 = __byte_perm(v[0][w], v[1][w], 0x7362);
-                            const uint32_t y01 = __byte_perm(v[2][w], v[3][w], 0x5140), y23 = __byte_perm(v[2][w], v[3][w], 0x7362);
+                        for (int w = 0; w < WORDS; w++)
 #pragma unroll
                             for (int j = 0; j < 2; j++) {
-                                const uint2 x = dec_e4m3(j ? x23 : x01), y = dec_e4m3(j ? y23 : y01);
+                                uint32_t a[HALVES][4];
 #pragma unroll
-                                for (int nt = 0; nt < NT; nt++) add_values(o[nt][c][2 * w + j], x.x, x.y, y.x, y.y, pb[nt]);
+                                for (int h = 0; h < HALVES; h++) {
+                                    // bytes of two keys next to one another: values of one dimension
+                                    const uint2 x = dec_e4m3(__byte_perm(v[h][0][w], v[h][1][w], j ? 0x7362 : 0x5140));
+                                    const uint2 y = dec_e4m3(__byte_perm(v[h][2][w], v[h][3][w], j ? 0x7362 : 0x5140));
+                                    a[h][0] = x.x; a[h][1] = x.y; a[h][2] = y.x; a[h][3] = y.y;
+                                }
+#pragma unroll
+                                for (int nt = 0; nt < NT; nt++) add_values(o[nt][c][2 * w + j], nt, a, pb);
                             }
-                        }
                     }
                 } else {
 #pragma unroll
                     for (int c = 0; c < CHUNKS; c++) {
-                        uint32_t v[4][4];
+                        uint32_t v[HALVES][4][4];
 #pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const uint4 r = dec_lds4(vs + lane * 16 + (c * 4 + k) * 512);
-                            v[k][0] = r.x; v[k][1] = r.y; v[k][2] = r.z; v[k][3] = r.w;
-                        }
+                        for (int h = 0; h < HALVES; h++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++) {
+                                const uint4 r = dec_lds4(vs + h * S::V16 + lane * 16 + (c * 4 + k) * 512);
+                                v[h][k][0] = r.x; v[h][k][1] = r.y; v[h][k][2] = r.z; v[h][k][3] = r.w;
+                            }
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            const uint32_t a0 = __byte_perm(v[0][j], v[1][j], 0x5410), a1 = __byte_perm(v[0][j], v[1][j], 0x7632);
-                            const uint32_t a2 = __byte_perm(v[2][j], v[3][j], 0x5410), a3 = __byte_perm(v[2][j], v[3][j], 0x7632);
+                            uint32_t a[HALVES][4];
 #pragma unroll
-                            for (int nt = 0; nt < NT; nt++) add_values(o[nt][c][j], a0, a1, a2, a3, pb[nt]);
+                            for (int h = 0; h < HALVES; h++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++) a[h][i] = __byte_perm(v[h][i & 2][j], v[h][(i & 2) + 1][j], i & 1 ? 0x7632 : 0x5410);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) add_values(o[nt][c][j], nt, a, pb);
                         }
                     }
                 }
