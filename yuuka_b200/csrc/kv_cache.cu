@@ -1,8 +1,10 @@
 // Rows of a paged key-value cache: written in the cache's format, read back as plain numbers (yuuka_kv_write, yuuka_kv_read).
 //
 // Both move a row once and compute little, so what bounds them is memory: rows * 2 * (numbers + pool row) bytes. A warp takes
-// 256 values of a row (eight per lane, one 16- or 32-byte load), which holds whole Q8_0 blocks (four lanes each) and whole
-// heads (8, 16 or 32 lanes each), so the maxima that the scales come from need shuffles alone.
+// up to 1024 values of a K or V row, 256 at a time (eight per lane, one 16- or 32-byte load), all of its loads in flight before
+// the first is used and the row's place looked up once: with 256 values a warp and a loop over a grid of resident CTAs 30,000
+// rows of 8 x 128 bf16 took 83 us into F8. 256 values hold whole Q8_0 blocks (four lanes each) and whole heads (8, 16 or 32
+// lanes each), so the maxima that the scales come from need shuffles alone.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -100,7 +102,7 @@ struct MoveParams {
     const int32_t * pos;
     const int32_t * seq;
     int32_t * status;
-    int rows, kv_dim, chunks;  // chunks of 256 values in a row
+    int rows, kv_dim, groups;  // groups of 1024 values in a row
 };
 
 template <typename T> __device__ __forceinline__ void load8(const T * src, float (&x)[8]) {
@@ -144,50 +146,85 @@ __device__ __forceinline__ int quantize_q8(float v, float scale, float inv) {
 
 // Where row r's token lies: the pool row, -1 for a row without a token, -2 for one out of range.
 __device__ __forceinline__ int move_slot(const MoveParams & p, int r) {
-    const int pos = __ldg(p.pos + r);
+    const int pos = __ldg(p.pos + r), seq = p.seq ? __ldg(p.seq + r) : r;
     int bad;
-    const int slot = kv_token_slot(p.cache, p.seq && pos >= 0 ? __ldg(p.seq + r) : r, pos, bad);
+    const int slot = kv_token_slot(p.cache, seq, pos, bad);
     if (bad && p.status && (threadIdx.x & 31) == 0) atomicOr(p.status, bad);
     return slot;
 }
 
-constexpr int MOVE_WARPS = 8;
+constexpr int MOVE_WARPS = 8, MOVE_CHUNKS = 4;
 constexpr int Q8_CHUNK = 272;  // bytes of 256 values in Q8_0
 
-// The pool is aligned to 16 bytes, a row of Q8_0 to 4: rows are put together in shared memory and stored by words.
+// A warp's part: row, K or V, values first .. (of up to MOVE_CHUNKS chunks of 256).
+struct MoveUnit {
+    int r, first, chunks;
+    bool is_v;
+    __device__ __forceinline__ MoveUnit(const MoveParams & p) {
+        const unsigned unit = blockIdx.x * MOVE_WARPS + (threadIdx.x >> 5), parts = 2 * p.groups;
+        r = (int)(unit / parts);
+        const int rest = (int)(unit - (unsigned)r * parts);
+        is_v = rest >= p.groups;
+        first = (is_v ? rest - p.groups : rest) * 256 * MOVE_CHUNKS;
+        chunks = r < p.rows ? min(MOVE_CHUNKS, (p.kv_dim - first + 255) / 256) : 0;
+    }
+};
+
+// Words of a chunk of Q8_0 between shared memory and a pool row: rows that are a multiple of 16 bytes long by 16 bytes.
+template <bool STORE> __device__ __forceinline__ void move_q8_chunk(uint8_t * stage, uint8_t * row, int values, bool wide) {
+    const int lane = threadIdx.x & 31;
+    if (wide && values >= 256) {
+        if (lane < Q8_CHUNK / 16) {
+            if constexpr (STORE) reinterpret_cast<uint4 *>(row)[lane] = reinterpret_cast<const uint4 *>(stage)[lane];
+            else reinterpret_cast<uint4 *>(stage)[lane] = __ldg(reinterpret_cast<const uint4 *>(row) + lane);
+        }
+        return;
+    }
+    const int words = min(values, 256) / 32 * 34 / 4;
+    for (int w = lane; w < words; w += 32) {
+        if constexpr (STORE) reinterpret_cast<uint32_t *>(row)[w] = reinterpret_cast<const uint32_t *>(stage)[w];
+        else reinterpret_cast<uint32_t *>(stage)[w] = __ldg(reinterpret_cast<const uint32_t *>(row) + w);
+    }
+}
+
+// The pool is aligned to 16 bytes, a row of Q8_0 to 4: its blocks of 34 bytes are put together in shared memory.
 template <int FMT, int HD, typename T>
 __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MoveParams p) {
-    __shared__ __align__(16) uint8_t stage_all[FMT == YUUKA_KV_Q8_0 ? MOVE_WARPS * Q8_CHUNK : 16];
+    __shared__ __align__(16) uint8_t stage_all[FMT == YUUKA_KV_Q8_0 ? MOVE_WARPS * MOVE_CHUNKS * Q8_CHUNK : 16];
     pdl_entry();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t units = (int64_t)p.rows * 2 * p.chunks;
-    for (int64_t unit = (int64_t)blockIdx.x * MOVE_WARPS + warp; unit < units; unit += (int64_t)gridDim.x * MOVE_WARPS) {
-        const int r = (int)(unit / (2 * p.chunks)), rest = (int)(unit - (int64_t)r * 2 * p.chunks);
-        const bool is_v = rest >= p.chunks;
-        const int chunk = is_v ? rest - p.chunks : rest, first = chunk * 256 + lane * 8;
-        const bool live = first < p.kv_dim;
-        float x[8];
+    const MoveUnit u(p);
+    if (u.chunks == 0) return;
+    float x[MOVE_CHUNKS][8];
+    const T * src = reinterpret_cast<const T *>(u.is_v ? p.v : p.k) + (int64_t)u.r * (u.is_v ? p.v_stride : p.k_stride) + u.first + lane * 8;
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = 0.0f;
-        const T * src = reinterpret_cast<const T *>(is_v ? p.v : p.k) + (int64_t)r * (is_v ? p.v_stride : p.k_stride) + first;
-        if (live) load8(src, x);
-        const int slot = move_slot(p, r);
-        if (slot < 0) continue;  // (the whole warp: one row)
-        uint8_t * row = (is_v ? p.cache.v : p.cache.k) + (int64_t)slot * p.cache.row_bytes;
+    for (int c = 0; c < MOVE_CHUNKS; c++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[c][i] = 0.0f;
+        if (u.first + c * 256 + lane * 8 < p.kv_dim) load8(src + c * 256, x[c]);
+    }
+    const int slot = move_slot(p, u.r);
+    if (slot < 0) return;  // (the whole warp: one row)
+    uint8_t * row = (u.is_v ? p.cache.v : p.cache.k) + (int64_t)slot * p.cache.row_bytes;
+#pragma unroll
+    for (int c = 0; c < MOVE_CHUNKS; c++) {
+        if (c >= u.chunks) break;
+        const int first = u.first + c * 256 + lane * 8;
+        const bool live = first < p.kv_dim;
         if constexpr (FMT == YUUKA_KV_F32) {
-            if (live) store8(reinterpret_cast<float *>(row) + first, x);
+            if (live) store8(reinterpret_cast<float *>(row) + first, x[c]);
         } else if constexpr (FMT == YUUKA_KV_F16) {
             if (live) {
                 uint4 raw;
                 uint16_t * e = reinterpret_cast<uint16_t *>(&raw);
 #pragma unroll
-                for (int i = 0; i < 8; i++) e[i] = half_up(x[i]);
+                for (int i = 0; i < 8; i++) e[i] = half_up(x[c][i]);
                 *reinterpret_cast<uint4 *>(row + 2 * first) = raw;
             }
         } else if constexpr (FMT == YUUKA_KV_Q8_0) {
             float amax = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));
+            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[c][i]));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             const float scale = amax / 127.0f, inv = 1.0f / scale;
@@ -197,25 +234,19 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MovePar
                 for (int i = 0; i < 8; i++) q[i] = 0;
             } else if (inv <= 3.0e38f) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) q[i] = quantize_q8(x[i], scale, inv);
+                for (int i = 0; i < 8; i++) q[i] = quantize_q8(x[c][i], scale, inv);
             } else {  // (a scale whose inverse is no finite number)
 #pragma unroll
-                for (int i = 0; i < 8; i++) q[i] = (int)round((double)(x[i] / scale));
+                for (int i = 0; i < 8; i++) q[i] = (int)round((double)(x[c][i] / scale));
             }
-            uint8_t * stage = stage_all + warp * Q8_CHUNK;
-            uint16_t * blk = reinterpret_cast<uint16_t *>(stage + (lane >> 2) * 34);
-            __syncwarp();  // (the words of the unit before have been read)
+            uint16_t * blk = reinterpret_cast<uint16_t *>(stage_all + (warp * MOVE_CHUNKS + c) * Q8_CHUNK + (lane >> 2) * 34);
             if ((lane & 3) == 0) blk[0] = half_up(scale);
 #pragma unroll
             for (int i = 0; i < 4; i++) blk[1 + (lane & 3) * 4 + i] = (uint16_t)((q[2 * i] & 0xff) | (q[2 * i + 1] << 8));
-            __syncwarp();
-            const int words = min(256, p.kv_dim - chunk * 256) / 32 * 34 / 4;
-            uint32_t * dst = reinterpret_cast<uint32_t *>(row + chunk * Q8_CHUNK);
-            for (int w = lane; w < words; w += 32) dst[w] = reinterpret_cast<const uint32_t *>(stage)[w];
         } else {
             float amax = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));
+            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[c][i]));
 #pragma unroll
             for (int o = HD / 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
             const bool none = !(448.0f / amax <= 3.0e38f);  // (nothing but zeros, or too small for a finite factor)
@@ -224,7 +255,7 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MovePar
             __nv_fp8x2_storage_t * e = reinterpret_cast<__nv_fp8x2_storage_t *>(&raw);
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                e[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i] * inv, x[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                e[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[c][2 * i] * inv, x[c][2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
             if (live) {
                 *reinterpret_cast<uint2 *>(row + first) = raw;
                 if (first % HD == 0) *reinterpret_cast<float *>(row + p.kv_dim + first / HD * 4) = none ? 0.0f : amax / 448.0f;
@@ -234,68 +265,75 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MovePar
             }
         }
     }
+    if constexpr (FMT == YUUKA_KV_Q8_0) {
+        __syncwarp();
+        for (int c = 0; c < u.chunks; c++)
+            move_q8_chunk<true>(stage_all + (warp * MOVE_CHUNKS + c) * Q8_CHUNK, row + (u.first / 256 + c) * Q8_CHUNK, p.kv_dim - u.first - c * 256,
+                                p.cache.row_bytes % 16 == 0);
+    }
 }
 
 template <int FMT, int HD, typename T>
 __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_read_kernel(const MoveParams p) {
-    __shared__ __align__(16) uint8_t stage_all[FMT == YUUKA_KV_Q8_0 ? MOVE_WARPS * Q8_CHUNK : 16];
+    __shared__ __align__(16) uint8_t stage_all[FMT == YUUKA_KV_Q8_0 ? MOVE_WARPS * MOVE_CHUNKS * Q8_CHUNK : 16];
     pdl_entry();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t units = (int64_t)p.rows * 2 * p.chunks;
-    for (int64_t unit = (int64_t)blockIdx.x * MOVE_WARPS + warp; unit < units; unit += (int64_t)gridDim.x * MOVE_WARPS) {
-        const int r = (int)(unit / (2 * p.chunks)), rest = (int)(unit - (int64_t)r * 2 * p.chunks);
-        const bool is_v = rest >= p.chunks;
-        const int chunk = is_v ? rest - p.chunks : rest, first = chunk * 256 + lane * 8;
-        const int slot = move_slot(p, r);
-        if (slot == -1) continue;
-        const bool live = first < p.kv_dim;
-        const uint8_t * row = (is_v ? p.cache.v : p.cache.k) + (int64_t)max(slot, 0) * p.cache.row_bytes;
-        float x[8];
+    const MoveUnit u(p);
+    if (u.chunks == 0) return;
+    const int slot = move_slot(p, u.r);
+    if (slot == -1) return;
+    uint8_t * row = (u.is_v ? p.cache.v : p.cache.k) + (int64_t)max(slot, 0) * p.cache.row_bytes;
+    float x[MOVE_CHUNKS][8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = __uint_as_float(0x7fffffffu);
-        if (slot >= 0) {
-            if constexpr (FMT == YUUKA_KV_F32) {
-                if (live) load8(reinterpret_cast<const float *>(row) + first, x);
-            } else if constexpr (FMT == YUUKA_KV_F16) {
-                if (live) load8(reinterpret_cast<const __half *>(row) + first, x);
-            } else if constexpr (FMT == YUUKA_KV_Q8_0) {
-                uint8_t * stage = stage_all + warp * Q8_CHUNK;
-                const int words = min(256, p.kv_dim - chunk * 256) / 32 * 34 / 4;
-                const uint32_t * src = reinterpret_cast<const uint32_t *>(row + chunk * Q8_CHUNK);
-                __syncwarp();
-                for (int w = lane; w < words; w += 32) reinterpret_cast<uint32_t *>(stage)[w] = __ldg(src + w);
-                __syncwarp();
-                if (live) {
-                    const uint16_t * blk = reinterpret_cast<const uint16_t *>(stage + (lane >> 2) * 34);
-                    const float d = __half2float(__ushort_as_half(blk[0]));
+    for (int c = 0; c < MOVE_CHUNKS; c++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint16_t q = blk[1 + (lane & 3) * 4 + i];
-                        x[2 * i] = d * (float)(int8_t)(q & 0xff);
-                        x[2 * i + 1] = d * (float)(int8_t)(q >> 8);
-                    }
+        for (int i = 0; i < 8; i++) x[c][i] = __uint_as_float(0x7fffffffu);
+    if (slot >= 0) {
+        if constexpr (FMT == YUUKA_KV_Q8_0) {
+#pragma unroll
+            for (int c = 0; c < MOVE_CHUNKS; c++)
+                if (c < u.chunks)
+                    move_q8_chunk<false>(stage_all + (warp * MOVE_CHUNKS + c) * Q8_CHUNK, row + (u.first / 256 + c) * Q8_CHUNK,
+                                         p.kv_dim - u.first - c * 256, p.cache.row_bytes % 16 == 0);
+            __syncwarp();
+        }
+#pragma unroll
+        for (int c = 0; c < MOVE_CHUNKS; c++) {
+            const int first = u.first + c * 256 + lane * 8;
+            if (first >= p.kv_dim) continue;
+            if constexpr (FMT == YUUKA_KV_F32) load8(reinterpret_cast<const float *>(row) + first, x[c]);
+            else if constexpr (FMT == YUUKA_KV_F16) load8(reinterpret_cast<const __half *>(row) + first, x[c]);
+            else if constexpr (FMT == YUUKA_KV_Q8_0) {
+                const uint16_t * blk = reinterpret_cast<const uint16_t *>(stage_all + (warp * MOVE_CHUNKS + c) * Q8_CHUNK + (lane >> 2) * 34);
+                const float d = __half2float(__ushort_as_half(blk[0]));
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint16_t q = blk[1 + (lane & 3) * 4 + i];
+                    x[c][2 * i] = d * (float)(int8_t)(q & 0xff);
+                    x[c][2 * i + 1] = d * (float)(int8_t)(q >> 8);
                 }
-            } else if (live) {
+            } else {
                 const uint2 raw = __ldg(reinterpret_cast<const uint2 *>(row + first));
                 const float d = __ldg(reinterpret_cast<const float *>(row + p.kv_dim) + first / HD);
                 const __nv_fp8x2_storage_t * e = reinterpret_cast<const __nv_fp8x2_storage_t *>(&raw);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float2 v = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(e[i], __NV_E4M3)));
-                    x[2 * i] = d * v.x;
-                    x[2 * i + 1] = d * v.y;
+                    x[c][2 * i] = d * v.x;
+                    x[c][2 * i + 1] = d * v.y;
                 }
             }
         }
-        if (live) store8(reinterpret_cast<T *>(is_v ? p.v : p.k) + (int64_t)r * (is_v ? p.v_stride : p.k_stride) + first, x);
     }
+    T * dst = reinterpret_cast<T *>(u.is_v ? p.v : p.k) + (int64_t)u.r * (u.is_v ? p.v_stride : p.k_stride) + u.first + lane * 8;
+#pragma unroll
+    for (int c = 0; c < MOVE_CHUNKS; c++)
+        if (u.first + c * 256 + lane * 8 < p.kv_dim) store8(dst + c * 256, x[c]);
 }
 
 template <int FMT, int HD, typename T>
 static void launch_move_as(yuuka_stream * stream, const MoveParams & p, bool write) {
-    const int64_t units = (int64_t)p.rows * 2 * p.chunks;
-    // eight CTAs of eight warps fill an SM
-    const int64_t grid = std::min<int64_t>((units + MOVE_WARPS - 1) / MOVE_WARPS, (int64_t)stream->dev->sm_count * 8);
+    const int64_t grid = ((int64_t)p.rows * 2 * p.groups + MOVE_WARPS - 1) / MOVE_WARPS;
     launch_k(write ? kv_write_kernel<FMT, HD, T> : kv_read_kernel<FMT, HD, T>, (unsigned)grid, MOVE_WARPS * 32, 0, stream->s, p);
 }
 template <int FMT, typename T> static void launch_move_format(yuuka_stream * stream, const MoveParams & p, bool write, int head_dim) {
@@ -368,7 +406,10 @@ static yuuka_status move_rows(const char * op, bool write, yuuka_stream * stream
         p.status = rows->status ? (int32_t *)((uint8_t *)rows->status->ptr + rows->status_offset) : nullptr;
         p.rows = (int)rows->rows;
         p.kv_dim = (int)dim;
-        p.chunks = (int)((dim + 255) / 256);
+        p.groups = (int)((dim + 256 * MOVE_CHUNKS - 1) / (256 * MOVE_CHUNKS));
+        // (warps are counted in 32 bits)
+        YK_REQUIRE(rows->rows * 2 * (uint64_t)p.groups < (1ull << 32) - MOVE_WARPS, YUUKA_ERR_UNSUPPORTED, "%s: %llu rows of %llu values", op,
+                   (unsigned long long)rows->rows, (unsigned long long)dim);
         set_device(dev);
         if (rows->dtype == YUUKA_DTYPE_F32) launch_move<float>(stream, p, write, cache->head_dim);
         else if (rows->dtype == YUUKA_DTYPE_F16) launch_move<__half>(stream, p, write, cache->head_dim);
