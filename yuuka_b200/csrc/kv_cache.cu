@@ -11,6 +11,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "kv_cache.cuh"
 #include "quant.cuh"
@@ -105,17 +106,37 @@ struct MoveParams {
     int rows, kv_dim, groups;  // groups of 1024 values in a row
 };
 
-template <typename T> __device__ __forceinline__ void load8(const T * src, float (&x)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(src)), b = __ldg(reinterpret_cast<const float4 *>(src) + 1);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(src));
-        const T * e = reinterpret_cast<const T *>(&raw);
+// Eight neighbouring values as they come from memory.
+template <typename T> struct Eight {
+    uint4 raw[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const void * src) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[i] = __ldg(reinterpret_cast<const uint4 *>(src) + i);
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const T * e = reinterpret_cast<const T *>(raw);
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = (float)e[i];
     }
-}
+    __device__ __forceinline__ float largest() const {  // magnitude; a NaN does not count
+        if constexpr (sizeof(T) == 4) {
+            const float * e = reinterpret_cast<const float *>(raw);
+            float m = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(e[i]));
+            return m;
+        } else {
+            using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+            const Pair * e = reinterpret_cast<const Pair *>(raw);
+            const Pair m = __hmax2(__hmax2(__habs2(e[0]), __habs2(e[1])), __hmax2(__habs2(e[2]), __habs2(e[3])));
+            return fmaxf(fmaxf((float)m.x, (float)m.y), 0.0f);
+        }
+    }
+};
 template <typename T> __device__ __forceinline__ void store8(T * dst, const float (&x)[8]) {
     if constexpr (sizeof(T) == 4) {
         reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -136,12 +157,25 @@ __device__ __forceinline__ uint16_t half_up(float f) {
     if (a >= 0x38800000u && a < 0x477ff000u) return __half_as_ushort(__float2half_rz(__uint_as_float(b + 0x1000u)));
     return f32_to_f16_ref(f);
 }
-// The nearest integer to v / scale, halves away from zero, of the f32 quotient. The product with 1 / scale is within 2^-22
-// of the quotient (relative; at most 127.5 in magnitude, so 2^-15 in all): away from a half it rounds to the same integer.
-__device__ __forceinline__ int quantize_q8(float v, float scale, float inv) {
-    const float y = v * inv, t = truncf(y), d = fabsf(y - t);
-    if (fabsf(d - 0.5f) > 1e-4f) return (int)t + (d > 0.5f ? (v < 0.0f ? -1 : 1) : 0);
-    return (int)round((double)(v / scale));
+// The nearest integers to v / scale, halves away from zero, of the f32 quotients, as bytes. The product with 1 / scale is within
+// 2^-22 of the quotient (relative; at most 127.5 in magnitude, so 2^-15 in all): where it is not within 1e-4 of a half it rounds
+// to the same integer, which adding 1.5 * 2^23 leaves in the low byte. Others, and NaN, take the quotient itself.
+__device__ __forceinline__ uint2 quantize_q8(const float (&v)[8], float scale, float inv) {
+    constexpr float MAGIC = 12582912.0f;
+    uint32_t q[8];
+    bool sure = inv <= 3.0e38f;  // (a scale whose inverse is no finite number)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float r = fmaf(v[i], inv, MAGIC);
+        q[i] = __float_as_uint(r);
+        sure &= fabsf(fmaf(v[i], inv, MAGIC - r)) <= 0.4999f;
+    }
+    if (!sure) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) q[i] = scale != 0.0f ? (uint32_t)(int)round((double)(v[i] / scale)) : 0u;
+    }
+    return make_uint2(__byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410));
 }
 
 // Where row r's token lies: the pool row, -1 for a row without a token, -2 for one out of range.
@@ -195,70 +229,91 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MovePar
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const MoveUnit u(p);
     if (u.chunks == 0) return;
-    float x[MOVE_CHUNKS][8];
+    Eight<T> x[MOVE_CHUNKS];
     const T * src = reinterpret_cast<const T *>(u.is_v ? p.v : p.k) + (int64_t)u.r * (u.is_v ? p.v_stride : p.k_stride) + u.first + lane * 8;
 #pragma unroll
     for (int c = 0; c < MOVE_CHUNKS; c++) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[c][i] = 0.0f;
-        if (u.first + c * 256 + lane * 8 < p.kv_dim) load8(src + c * 256, x[c]);
+        x[c].zero();
+        if (u.first + c * 256 + lane * 8 < p.kv_dim) x[c].load(src + c * 256);
     }
     const int slot = move_slot(p, u.r);
     if (slot < 0) return;  // (the whole warp: one row)
     uint8_t * row = (u.is_v ? p.cache.v : p.cache.k) + (int64_t)slot * p.cache.row_bytes;
+
+    // Scales: every division is made once, by one lane, for all chunks at a time, and handed to the lanes that need it.
+    float scale[MOVE_CHUNKS], inv[MOVE_CHUNKS];
+    uint32_t half_scale = 0;  // Q8_0: of block lane (eight of a chunk)
+    if constexpr (FMT == YUUKA_KV_Q8_0 || FMT == YUUKA_KV_F8) {
+        constexpr int LANES = FMT == YUUKA_KV_Q8_0 ? 4 : HD / 8;  // that share a scale
+        static_assert(MOVE_CHUNKS == 4, "the divisions' lanes");
+        float amax[MOVE_CHUNKS];
+#pragma unroll
+        for (int c = 0; c < MOVE_CHUNKS; c++) {
+            amax[c] = x[c].largest();
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) amax[c] = fmaxf(amax[c], __shfl_xor_sync(0xffffffffu, amax[c], o));
+        }
+        if constexpr (FMT == YUUKA_KV_Q8_0) {
+            float mine = 0.0f;
+#pragma unroll
+            for (int c = 0; c < MOVE_CHUNKS; c++) {
+                const float a = __shfl_sync(0xffffffffu, amax[c], 4 * (lane & 7));
+                if (lane >> 3 == c) mine = a;
+            }
+            const float s = mine / 127.0f, r = 1.0f / s;
+            half_scale = half_up(s);
+#pragma unroll
+            for (int c = 0; c < MOVE_CHUNKS; c++) {
+                scale[c] = __shfl_sync(0xffffffffu, s, 8 * c + (lane >> 2));
+                inv[c] = __shfl_sync(0xffffffffu, r, 8 * c + (lane >> 2));
+            }
+        } else {
+            const int at = lane & (LANES - 1);
+            const float mine = (at & 2) ? ((at & 1) ? amax[3] : amax[2]) : ((at & 1) ? amax[1] : amax[0]);
+            const float r = (at & 4) ? mine / 448.0f : 448.0f / mine;
+#pragma unroll
+            for (int c = 0; c < MOVE_CHUNKS; c++) {
+                inv[c] = __shfl_sync(0xffffffffu, r, lane - at + c);
+                scale[c] = __shfl_sync(0xffffffffu, r, lane - at + 4 + c);
+                // (nothing but zeros, or too small for a finite factor; 0 keeps a NaN)
+                if (!(inv[c] <= 3.0e38f)) inv[c] = scale[c] = 0.0f;
+            }
+        }
+    }
 #pragma unroll
     for (int c = 0; c < MOVE_CHUNKS; c++) {
         if (c >= u.chunks) break;
         const int first = u.first + c * 256 + lane * 8;
         const bool live = first < p.kv_dim;
+        float f[8];
+        x[c].get(f);
         if constexpr (FMT == YUUKA_KV_F32) {
-            if (live) store8(reinterpret_cast<float *>(row) + first, x[c]);
+            if (live) store8(reinterpret_cast<float *>(row) + first, f);
         } else if constexpr (FMT == YUUKA_KV_F16) {
             if (live) {
                 uint4 raw;
                 uint16_t * e = reinterpret_cast<uint16_t *>(&raw);
 #pragma unroll
-                for (int i = 0; i < 8; i++) e[i] = half_up(x[c][i]);
+                for (int i = 0; i < 8; i++) e[i] = half_up(f[i]);
                 *reinterpret_cast<uint4 *>(row + 2 * first) = raw;
             }
         } else if constexpr (FMT == YUUKA_KV_Q8_0) {
-            float amax = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[c][i]));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            const float scale = amax / 127.0f, inv = 1.0f / scale;
-            int q[8];
-            if (scale == 0.0f) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) q[i] = 0;
-            } else if (inv <= 3.0e38f) {
-#pragma unroll
-                for (int i = 0; i < 8; i++) q[i] = quantize_q8(x[c][i], scale, inv);
-            } else {  // (a scale whose inverse is no finite number)
-#pragma unroll
-                for (int i = 0; i < 8; i++) q[i] = (int)round((double)(x[c][i] / scale));
-            }
-            uint16_t * blk = reinterpret_cast<uint16_t *>(stage_all + (warp * MOVE_CHUNKS + c) * Q8_CHUNK + (lane >> 2) * 34);
-            if ((lane & 3) == 0) blk[0] = half_up(scale);
-#pragma unroll
-            for (int i = 0; i < 4; i++) blk[1 + (lane & 3) * 4 + i] = (uint16_t)((q[2 * i] & 0xff) | (q[2 * i + 1] << 8));
+            const uint2 q = quantize_q8(f, scale[c], inv[c]);
+            uint16_t * chunk = reinterpret_cast<uint16_t *>(stage_all + (warp * MOVE_CHUNKS + c) * Q8_CHUNK);
+            uint16_t * blk = chunk + (lane >> 2) * 17 + 1 + (lane & 3) * 4;
+            blk[0] = (uint16_t)q.x;
+            blk[1] = (uint16_t)(q.x >> 16);
+            blk[2] = (uint16_t)q.y;
+            blk[3] = (uint16_t)(q.y >> 16);
+            if (lane >> 3 == c) chunk[(lane & 7) * 17] = (uint16_t)half_scale;
         } else {
-            float amax = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[c][i]));
-#pragma unroll
-            for (int o = HD / 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            const bool none = !(448.0f / amax <= 3.0e38f);  // (nothing but zeros, or too small for a finite factor)
-            const float inv = none ? 0.0f : 448.0f / amax;  // (0 keeps a NaN)
             uint2 raw;
             __nv_fp8x2_storage_t * e = reinterpret_cast<__nv_fp8x2_storage_t *>(&raw);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                e[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[c][2 * i] * inv, x[c][2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+            for (int i = 0; i < 4; i++) e[i] = __nv_cvt_float2_to_fp8x2(make_float2(f[2 * i] * inv[c], f[2 * i + 1] * inv[c]), __NV_SATFINITE, __NV_E4M3);
             if (live) {
                 *reinterpret_cast<uint2 *>(row + first) = raw;
-                if (first % HD == 0) *reinterpret_cast<float *>(row + p.kv_dim + first / HD * 4) = none ? 0.0f : amax / 448.0f;
+                if (first % HD == 0) *reinterpret_cast<float *>(row + p.kv_dim + first / HD * 4) = scale[c];
                 // (the zeros behind the scales)
                 if (first + 8 == p.kv_dim)
                     for (int at = p.kv_dim + 4 * (p.kv_dim / HD); at < p.cache.row_bytes; at += 4) *reinterpret_cast<uint32_t *>(row + at) = 0;
@@ -283,13 +338,11 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_read_kernel(const MovePara
     const int slot = move_slot(p, u.r);
     if (slot == -1) return;
     uint8_t * row = (u.is_v ? p.cache.v : p.cache.k) + (int64_t)max(slot, 0) * p.cache.row_bytes;
-    float x[MOVE_CHUNKS][8];
-#pragma unroll
-    for (int c = 0; c < MOVE_CHUNKS; c++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[c][i] = __uint_as_float(0x7fffffffu);
-    if (slot >= 0) {
-        if constexpr (FMT == YUUKA_KV_Q8_0) {
+    // loads of all chunks first, then the values
+    Eight<typename std::conditional<FMT == YUUKA_KV_F32, float, __half>::type> x[MOVE_CHUNKS];  // (F8: half of one)
+    float d[MOVE_CHUNKS];
+    if constexpr (FMT == YUUKA_KV_Q8_0) {
+        if (slot >= 0) {
 #pragma unroll
             for (int c = 0; c < MOVE_CHUNKS; c++)
                 if (c < u.chunks)
@@ -297,38 +350,52 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_read_kernel(const MovePara
                                          p.kv_dim - u.first - c * 256, p.cache.row_bytes % 16 == 0);
             __syncwarp();
         }
+    } else {
 #pragma unroll
         for (int c = 0; c < MOVE_CHUNKS; c++) {
             const int first = u.first + c * 256 + lane * 8;
-            if (first >= p.kv_dim) continue;
-            if constexpr (FMT == YUUKA_KV_F32) load8(reinterpret_cast<const float *>(row) + first, x[c]);
-            else if constexpr (FMT == YUUKA_KV_F16) load8(reinterpret_cast<const __half *>(row) + first, x[c]);
-            else if constexpr (FMT == YUUKA_KV_Q8_0) {
-                const uint16_t * blk = reinterpret_cast<const uint16_t *>(stage_all + (warp * MOVE_CHUNKS + c) * Q8_CHUNK + (lane >> 2) * 34);
-                const float d = __half2float(__ushort_as_half(blk[0]));
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint16_t q = blk[1 + (lane & 3) * 4 + i];
-                    x[c][2 * i] = d * (float)(int8_t)(q & 0xff);
-                    x[c][2 * i + 1] = d * (float)(int8_t)(q >> 8);
-                }
-            } else {
+            if (slot < 0 || first >= p.kv_dim) continue;
+            if constexpr (FMT == YUUKA_KV_F32) x[c].load(row + 4 * first);
+            else if constexpr (FMT == YUUKA_KV_F16) x[c].load(row + 2 * first);
+            else {
                 const uint2 raw = __ldg(reinterpret_cast<const uint2 *>(row + first));
-                const float d = __ldg(reinterpret_cast<const float *>(row + p.kv_dim) + first / HD);
-                const __nv_fp8x2_storage_t * e = reinterpret_cast<const __nv_fp8x2_storage_t *>(&raw);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 v = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(e[i], __NV_E4M3)));
-                    x[c][2 * i] = d * v.x;
-                    x[c][2 * i + 1] = d * v.y;
-                }
+                x[c].raw[0].x = raw.x;
+                x[c].raw[0].y = raw.y;
+                d[c] = __ldg(reinterpret_cast<const float *>(row + p.kv_dim) + first / HD);
             }
         }
     }
     T * dst = reinterpret_cast<T *>(u.is_v ? p.v : p.k) + (int64_t)u.r * (u.is_v ? p.v_stride : p.k_stride) + u.first + lane * 8;
 #pragma unroll
-    for (int c = 0; c < MOVE_CHUNKS; c++)
-        if (u.first + c * 256 + lane * 8 < p.kv_dim) store8(dst + c * 256, x[c]);
+    for (int c = 0; c < MOVE_CHUNKS; c++) {
+        if (u.first + c * 256 + lane * 8 >= p.kv_dim) break;
+        float f[8];
+        if constexpr (FMT == YUUKA_KV_Q8_0) {
+            const uint16_t * blk = reinterpret_cast<const uint16_t *>(stage_all + (warp * MOVE_CHUNKS + c) * Q8_CHUNK + (lane >> 2) * 34);
+            const float s = __half2float(__ushort_as_half(blk[0]));
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint16_t q = blk[1 + (lane & 3) * 4 + i];
+                f[2 * i] = s * (float)(int8_t)(q & 0xff);
+                f[2 * i + 1] = s * (float)(int8_t)(q >> 8);
+            }
+        } else if constexpr (FMT == YUUKA_KV_F8) {
+            const uint32_t raw[2] = {x[c].raw[0].x, x[c].raw[0].y};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const __nv_fp8x2_storage_t e = (__nv_fp8x2_storage_t)(raw[i >> 1] >> (16 * (i & 1)));
+                const float2 v = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(e, __NV_E4M3)));
+                f[2 * i] = d[c] * v.x;
+                f[2 * i + 1] = d[c] * v.y;
+            }
+        } else {
+            x[c].get(f);
+        }
+        if (slot < 0)
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] = __uint_as_float(0x7fffffffu);
+        store8(dst + c * 256, f);
+    }
 }
 
 template <int FMT, int HD, typename T>
