@@ -223,7 +223,8 @@ YUUKA_API yuuka_status yuuka_weights_tile(yuuka_stream * stream, yuuka_buffer * 
  *   Q8_0      blocks of 32 values: f16 scale amax / 127, int8 x / scale rounded half away from zero (kv_format.go:97-131)
  *   F8        kv_heads * head_dim E4M3 values x * (448 / amax), rounded to nearest even, amax over a token's head; then
  *             kv_heads f32 scales amax / 448; zeros up to a multiple of 16 bytes. A value is its E4M3 times the scale.
- *             A head for which 448 / amax passes 3e38 (amax below 1.5e-36) is stored as zeros.
+ *             A head for which 448 / amax passes 3e38 (amax below 1.5e-36) is stored as zeros, one with a NaN with a NaN
+ *             for its scale.
  * head_dim is 64, 128 or 256. Offsets of pools are multiples of 16 bytes, of tables of 4. */
 typedef struct yuuka_kv_cache {
     yuuka_buffer * k;

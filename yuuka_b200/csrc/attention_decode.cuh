@@ -55,7 +55,11 @@ struct DecodeParams {
 constexpr int DEC_WARPS = 4096;         // of a grid, at most
 constexpr size_t DEC_PARTIAL_BYTES = 24u << 20;
 enum { DEC_SHORT, DEC_LONG, DEC_DONE, DEC_COUNTERS };
-constexpr int DEC_SHORT_MOST = 32;      // partials that a warp joins
+#ifndef DEC_SHORT_N
+#define DEC_SHORT_N 32
+#define DEC_JOIN_SM 4
+#endif
+constexpr int DEC_SHORT_MOST = DEC_SHORT_N;      // partials that a warp joins
 constexpr float DEC_P_LOG2 = 7.0f;      // log2 of the factor that probabilities carry
 constexpr float DEC_SLACK = 8.0f;       // log2 of what a score may pass the running maximum by before sums are rescaled
 constexpr int DEC_SMEM_SM = 233472;     // shared memory of an SM
@@ -131,6 +135,14 @@ __device__ __forceinline__ uint2 dec_e4m3(uint32_t four) {
                  : "r"(four));
     return h;
 }
+// The same by integer instructions, as pairs of f16 that are 2^-8 of the values: an E4M3's bits shifted to where an f16 has its
+// exponent and fraction mean 2^-8 of its value (subnormals too; a NaN's do not stay one). The conversions share a pipe with the
+// exponentials that takes eight cycles for one; with K and V both converted there it was 92 % busy.
+__device__ __forceinline__ uint2 dec_e4m3_bits(uint32_t four) {
+    const uint32_t lo = __byte_perm(four, 0u, 0x4140), hi = __byte_perm(four, 0u, 0x4342);  // one byte in each half
+    // twice the sign's place takes it to the place above, and all goes up by seven
+    return make_uint2((lo + (lo & 0x00800080u)) * 128u, (hi + (hi & 0x00800080u)) * 128u);
+}
 // bytes 0 and 1 (PAIR 0) or 2 and 3 of x, unsigned with an offset of 128, as f16 pairs of the signed values: exact
 template <int PAIR> __device__ __forceinline__ uint32_t dec_int8(uint32_t x) {
     const uint32_t h = __byte_perm(x, 0x64646464u, PAIR ? 0x4342 : 0x4140);  // 1024 + byte
@@ -171,15 +183,15 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     static constexpr int K16 = IS_F32 ? HD * 64 : (IS_Q8 ? 64 * Q8_K : (IS_F8 ? HD * 16 : HD * 32));  // bytes of sixteen keys
     static constexpr int V16 = IS_F32 ? HD * 64 : (IS_Q8 ? 64 * Q8_V : (IS_F8 ? HD * 16 : HD * 32));
     static constexpr int K_BYTES = K16 * HALVES + (IS_F8 ? 8 * KEYS : 0), V_BYTES = V16 * HALVES;
-    // K of the other formats: a key's row, its 16-byte pieces copied by lines of 128 bytes, eight lanes to a line (one request
-    // to memory instead of two: 239 -> 227 us for 8 sequences of 32768, 8 KV heads of 128). In odd keys the halves of a line
-    // trade places, so that the eight lanes that read four pieces of two keys find them on different banks.
-    static constexpr int K_ROW = IS_Q8 ? 0 : IS_F32 ? HD * 4 : IS_F8 ? HD : HD * 2;
-    static constexpr bool K_LINES = K_ROW >= 128;
-    // where piece q (16 bytes) of a key's row lies
-    __device__ static __forceinline__ uint32_t k_piece(int key, int q) {
-        return key * K_ROW + 16 * (K_LINES ? q ^ ((key & 1) << 2) : q);
-    }
+    // Rows of the other formats, K and V: their 16-byte pieces are copied by lines of 128 bytes, eight neighbouring lanes to a
+    // line. (With lanes that copy what they will read themselves, four to a piece of K and every fourth to a line of V, the SMs
+    // fetched V's sectors twice: 1.61 GB for 1.07.) Pieces trade places within their line so that the eight lanes of a read find
+    // them on different banks: four pieces of two keys (K), two pieces of every other of eight keys (V).
+    static constexpr int ROW = IS_Q8 ? 0 : IS_F32 ? HD * 4 : IS_F8 ? HD : HD * 2;
+    static constexpr int LINE = ROW >= 128 ? 128 : 64, LANES = LINE / 16;  // bytes and lanes of a line
+    // where piece q of a key's row lies
+    __device__ static __forceinline__ uint32_t k_piece(int key, int q) { return key * ROW + 16 * (LINE == 128 ? q ^ ((key & 1) << 2) : q); }
+    __device__ static __forceinline__ uint32_t v_piece(int key, int q) { return key * ROW + 16 * (q ^ ((key >> 1 & (LINE == 128 ? 3 : 1)) << 1)); }
     static constexpr int SLOT = (K_BYTES > V_BYTES ? K_BYTES : V_BYTES);
     static constexpr int PART_FLOATS = COLS * (HD + 2);
     // queries in registers, or in shared memory where the sums leave too few (f32: 8 heads of all dimensions, split at use)
@@ -422,8 +434,8 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
         // the pools at the unit's head and this lane's piece
         constexpr int HEAD_BYTES = FMT == YUUKA_KV_F32 ? HD * 4 : (FMT == YUUKA_KV_F16 ? HD * 2 : (FMT == YUUKA_KV_Q8_0 ? HD / 32 * 34 : HD));
         const int kv_head = unit / p.head_tiles;
-        const uint8_t * const k_at = p.cache.k + (int64_t)kv_head * HEAD_BYTES + (S::IS_Q8 ? 4 * (lane & 7) : 16 * (S::K_LINES ? lane & 7 : t));
-        const uint8_t * const v_at = p.cache.v + (int64_t)kv_head * HEAD_BYTES + (S::IS_Q8 ? 4 * (lane & 7) : (S::IS_F8 ? S::F8_V : 16) * g);
+        const uint8_t * const k_at = p.cache.k + (int64_t)kv_head * HEAD_BYTES + (S::IS_Q8 ? 4 * (lane & 7) : 16 * (lane & (S::LANES - 1)));
+        const uint8_t * const v_at = p.cache.v + (int64_t)kv_head * HEAD_BYTES + (S::IS_Q8 ? 4 * (lane & 7) : 16 * (lane & (S::LANES - 1)));
         const int32_t * table = nullptr;
         const unsigned row_bytes = (unsigned)p.cache.row_bytes;
         auto look_up = [&] {
@@ -471,20 +483,17 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                                 if (8 * i + 7 < WORDS || w < WORDS) dec_copy<4>(dst + 32 * i + 4 * gap, src + 32 * i);
                             }
                         }
-                    } else if constexpr (!V) {
-                        if constexpr (S::K_LINES) {
+                    } else {
+                        constexpr int AT_ONCE = 32 / S::LANES;  // keys
 #pragma unroll
-                            for (int k = 0; k < KEYS / 4; k++) {
-                                const int key = 4 * k + (lane >> 3);
-                                const uint8_t * src = row_of(key);
+                        for (int k = 0; k < KEYS / AT_ONCE; k++) {
+                            const int key = AT_ONCE * k + lane / S::LANES, q = lane & (S::LANES - 1);
+                            const uint8_t * src = row_of(key);
+                            const uint32_t dst = put + (V ? S::v_piece(key, q) : S::k_piece(key, q));
 #pragma unroll
-                                for (int i = 0; i < S::K_ROW / 128; i++) dec_copy<16>(put + S::k_piece(key, lane & 7) + 128 * i, src + 128 * i);
-                            }
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < KEYS / 8; k++) dec_copy<16>(put + S::k_piece(g + 8 * k, t), row_of(g + 8 * k));
+                            for (int i = 0; i < S::ROW / S::LINE; i++) dec_copy<16>(dst + S::LINE * i, src + S::LINE * i);
                         }
-                        if constexpr (FMT == YUUKA_KV_F8) {
+                        if constexpr (FMT == YUUKA_KV_F8 && !V) {
                             // scales of K and behind them of V
                             const uint64_t at = (uint64_t)pool_row * row_bytes + (p.cache.kv_heads * HD + 4 * kv_head);
                             const uint32_t dst = put + S::K16 * HALVES + 4 * lane;
@@ -495,18 +504,6 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                                 dec_copy<4>(dst, (lane < 16 ? p.cache.k : p.cache.v) + at);
                             }
                         }
-                    } else {
-                        constexpr int PIECE = FMT == YUUKA_KV_F8 ? S::F8_V : 16;  // a lane's bytes of keys 2t, 2t + 1, 2t + 8, 2t + 9
-                        constexpr int PIECES = S::V16 / (128 * PIECE);
-#pragma unroll
-                        for (int h = 0; h < HALVES; h++)
-#pragma unroll
-                            for (int k = 0; k < 4; k++) {
-                                const uint8_t * src = row_of(16 * h + 2 * t + (k & 1) + 8 * (k >> 1));
-                                const uint32_t dst = put + S::V16 * h + lane * PIECE + k * 32 * PIECE;
-#pragma unroll
-                                for (int i = 0; i < PIECES; i++) dec_copy<PIECE>(dst + i * 128 * PIECE, src + 8 * PIECE * i);
-                            }
                     }
                 }
                 if constexpr (V) {
@@ -801,7 +798,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const uint2 x = dec_e4m3(wa[i]), y = dec_e4m3(wb[i]);
+                            const uint2 x = dec_e4m3_bits(wa[i]), y = dec_e4m3_bits(wb[i]);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
                                 const uint4 f = query(nt, 4 * c + i);
@@ -833,7 +830,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         for (int e = 0; e < 4; e++) s[nt][e] += s2[nt][e];
                 if constexpr (S::IS_F8) {
                     const uint32_t at = ks + S::K16 * HALVES + 64 * half + 4 * g;
-                    const float d0 = __uint_as_float(dec_lds(at)), d1 = __uint_as_float(dec_lds(at + 32));
+                    const float d0 = 256.0f * __uint_as_float(dec_lds(at)), d1 = 256.0f * __uint_as_float(dec_lds(at + 32));
                     vd[half][0] = __uint_as_float(dec_lds(at + 4 * KEYS));
                     vd[half][1] = __uint_as_float(dec_lds(at + 4 * KEYS + 32));
 #pragma unroll
@@ -935,7 +932,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                             uint32_t v[4][4];
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
-                                const uint4 r = dec_lds4(vs + half * S::V16 + lane * 16 + (c * 4 + k) * 512);
+                                const uint4 r = dec_lds4(vs + half * S::V16 + S::v_piece(2 * t + (k & 1) + 8 * (k >> 1), 8 * c + g));
                                 v[k][0] = r.x; v[k][1] = r.y; v[k][2] = r.z; v[k][3] = r.w;
                             }
 #pragma unroll
@@ -1011,7 +1008,8 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         for (int h = 0; h < HALVES; h++)
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
-                                const uint32_t at = vs + h * S::V16 + lane * S::F8_V + (c * 4 + k) * 32 * S::F8_V;
+                                const int key = 2 * t + (k & 1) + 8 * (k >> 1);
+                                const uint32_t at = vs + h * S::V16 + S::v_piece(key, WORDS == 4 ? 8 * c + g : g >> 1) + (WORDS == 4 ? 0 : 8 * (g & 1));
                                 if constexpr (WORDS == 4) {
                                     const uint4 r = dec_lds4(at);
                                     v[h][k][0] = r.x; v[h][k][1] = r.y; v[h][k][2] = r.z; v[h][k][3] = r.w;
@@ -1044,7 +1042,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         for (int h = 0; h < HALVES; h++)
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
-                                const uint4 r = dec_lds4(vs + h * S::V16 + lane * 16 + (c * 4 + k) * 512);
+                                const uint4 r = dec_lds4(vs + h * S::V16 + S::v_piece(2 * t + (k & 1) + 8 * (k >> 1), 8 * c + g));
                                 v[h][k][0] = r.x; v[h][k][1] = r.y; v[h][k][2] = r.z; v[h][k][3] = r.w;
                             }
 #pragma unroll
@@ -1145,7 +1143,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 // The units that several teams share. Few partials: a CTA takes a unit, a warp a column, a lane HD / 32 dimensions. Many: a CTA
 // takes 64 dimensions of a column at a time; groups of 16 threads take every 16th partial, so that many loads are in flight, and
 // are added in their order.
-constexpr int JOIN_THREADS = 256, JOIN_CTAS_SM = 4, JOIN_LANES = 16, JOIN_GROUPS = JOIN_THREADS / JOIN_LANES;
+constexpr int JOIN_THREADS = 256, JOIN_CTAS_SM = DEC_JOIN_SM, JOIN_LANES = 16, JOIN_GROUPS = JOIN_THREADS / JOIN_LANES;
 template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_THREADS) attention_decode_join_kernel(const DecodeParams p) {
     constexpr int PART = COLS * (HD + 2), SLICES = HD / (4 * JOIN_LANES), DIMS = HD / 32;
     __shared__ float factor[DEC_WARPS], reduce[2][JOIN_THREADS / 32];

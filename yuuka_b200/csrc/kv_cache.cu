@@ -106,6 +106,12 @@ struct MoveParams {
     int rows, kv_dim, groups;  // groups of 1024 values in a row
 };
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
 // Eight neighbouring values as they come from memory.
 template <typename T> struct Eight {
     uint4 raw[sizeof(T) / 2];
@@ -122,16 +128,21 @@ template <typename T> struct Eight {
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = (float)e[i];
     }
-    __device__ __forceinline__ float largest() const {  // magnitude; a NaN does not count
+    // largest magnitude; a NaN does not count, or makes it one
+    template <bool NANS> __device__ __forceinline__ float largest() const {
         if constexpr (sizeof(T) == 4) {
             const float * e = reinterpret_cast<const float *>(raw);
             float m = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; i++) m = fmaxf(m, fabsf(e[i]));
+            for (int i = 0; i < 8; i++) m = NANS ? max_nan(m, fabsf(e[i])) : fmaxf(m, fabsf(e[i]));
             return m;
         } else {
             using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
             const Pair * e = reinterpret_cast<const Pair *>(raw);
+            if constexpr (NANS) {
+                const Pair m = __hmax2_nan(__hmax2_nan(__habs2(e[0]), __habs2(e[1])), __hmax2_nan(__habs2(e[2]), __habs2(e[3])));
+                return max_nan((float)m.x, (float)m.y);
+            }
             const Pair m = __hmax2(__hmax2(__habs2(e[0]), __habs2(e[1])), __hmax2(__habs2(e[2]), __habs2(e[3])));
             return fmaxf(fmaxf((float)m.x, (float)m.y), 0.0f);
         }
@@ -249,9 +260,12 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MovePar
         float amax[MOVE_CHUNKS];
 #pragma unroll
         for (int c = 0; c < MOVE_CHUNKS; c++) {
-            amax[c] = x[c].largest();
+            amax[c] = x[c].template largest<FMT == YUUKA_KV_F8>();
 #pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) amax[c] = fmaxf(amax[c], __shfl_xor_sync(0xffffffffu, amax[c], o));
+            for (int o = LANES / 2; o > 0; o >>= 1) {
+                const float other = __shfl_xor_sync(0xffffffffu, amax[c], o);
+                amax[c] = FMT == YUUKA_KV_F8 ? max_nan(amax[c], other) : fmaxf(amax[c], other);
+            }
         }
         if constexpr (FMT == YUUKA_KV_Q8_0) {
             float mine = 0.0f;
@@ -275,8 +289,8 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MovePar
             for (int c = 0; c < MOVE_CHUNKS; c++) {
                 inv[c] = __shfl_sync(0xffffffffu, r, lane - at + c);
                 scale[c] = __shfl_sync(0xffffffffu, r, lane - at + 4 + c);
-                // (nothing but zeros, or too small for a finite factor; 0 keeps a NaN)
-                if (!(inv[c] <= 3.0e38f)) inv[c] = scale[c] = 0.0f;
+                if (inv[c] > 3.0e38f) scale[c] = 0.0f;  // (nothing but zeros, or too small for a finite factor)
+                if (!(inv[c] <= 3.0e38f)) inv[c] = 0.0f;  // (a NaN among the values makes the scale one)
             }
         }
     }
