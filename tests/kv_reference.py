@@ -42,19 +42,28 @@ def encode_e4m3(y):
 
 
 def encode(x, fmt, oracle):
-    """Rows [n, heads, dim] f32 -> bytes [n, row_bytes]; F32, F16 and Q8_0 by the oracle's codec (the sessions' own)."""
+    """Rows [n, heads, dim] f32 -> bytes [n, row_bytes]; f32 and f16 numbers by the oracle's codec (the sessions' own)."""
     n, h, d = x.shape
-    if fmt != "f8":
-        flat = np.ascontiguousarray(x.reshape(n, h * d), np.float32)
-        return np.stack([oracle.kv_encode_row(FORMATS[fmt], r) for r in flat])
+    x = np.ascontiguousarray(x, np.float32)
+    if fmt in ("f32", "f16"):
+        return np.stack([oracle.kv_encode_row(FORMATS[fmt], r) for r in x.reshape(n, h * d)])
+    if fmt == "q8_0":
+        blocks = x.reshape(n, h * d // 32, 32)
+        scale = np.fmax.reduce(np.abs(blocks), -1) * (np.float32(1) / np.float32(127))
+        with np.errstate(divide="ignore", invalid="ignore", over="ignore"):
+            y = (blocks / scale[..., None]).astype(np.float64)
+            q = np.trunc(y + np.copysign(0.5, y))
+        q = np.where(np.isfinite(q) & (scale[..., None] != 0), q, 0).astype(np.int64).astype(np.int8)
+        bits = oracle.kv_encode_row(FORMATS["f16"], np.ascontiguousarray(scale.reshape(-1))).reshape(n, h * d // 32, 2)
+        return np.concatenate([bits, q.view(np.uint8)], -1).reshape(n, -1)
     out = np.zeros((n, cuda.kv_row_bytes(cuda.KV_F8, h, d)), np.uint8)
     amax = np.abs(x).max(-1).astype(np.float32)
     with np.errstate(divide="ignore"):
-        inv = np.float32(448.0) / amax
+        inv = np.float32(1.0) / amax * np.float32(448.0)
     live = inv <= np.float32(3e38)
     inv = np.where(live, inv, np.float32(0))
     out[:, :h * d] = encode_e4m3((x * inv[..., None]).astype(np.float32)).reshape(n, h * d)
-    out[:, h * d:h * d + 4 * h] = np.where(live, amax / np.float32(448.0), np.float32(0)).astype(np.float32).view(np.uint8).reshape(n, 4 * h)
+    out[:, h * d:h * d + 4 * h] = np.where(live, amax * (np.float32(1) / np.float32(448)), np.float32(0)).astype(np.float32).view(np.uint8).reshape(n, 4 * h)
     return out
 
 

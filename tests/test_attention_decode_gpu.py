@@ -156,6 +156,36 @@ def test_many_rows_of_ragged_lengths(dev, stream, scratch, fmt, dtype):
     step.free()
 
 
+@pytest.mark.parametrize("fmt,kv_heads,group,dim", [("f32", 640, 1, 256), ("f16", 300, 3, 64), ("f8", 40, 40, 128)])
+def test_more_heads_than_warps(dev, stream, scratch, fmt, kv_heads, group, dim):
+    """Units (KV heads times tiles of query heads) that pass the warps of the machine, or take a good part of them."""
+    step = Step(dev, stream, 3, fmt, "f32", kv_heads, group, dim, 16, [3, 0, 35])
+    step.check(*step.run(scratch))
+    step.free()
+
+
+def test_a_batch_of_thousands(dev, stream, scratch):
+    rng = np.random.default_rng(17)
+    lens = rng.integers(0, 40, 300)
+    step = Step(dev, stream, 19, "f16", "bf16", 1, 4, 64, 8, lens, seq_ids=rng.integers(0, 300, 5000))
+    out, lse = step.run(scratch)
+    keep = set(range(0, 5000, 37)) | {4999}
+    step.check(out, lse, skip=set(range(5000)) - keep)
+    # rows of one sequence with one query would be equal: here the statistics depend on the row's own query alone
+    assert np.all(np.isfinite(out))
+    step.free()
+
+
+@pytest.mark.parametrize("fmt,dtype", [("f16", "f32"), ("f8", "f32"), ("q8_0", "f32"), ("f32", "f32")])
+def test_long_runs_keep_f32(dev, stream, scratch, fmt, dtype):
+    """Many tiles in one warp's run: sums of thousands of products stay within f32's rounding (the machine is filled with other
+    rows, so that a row is not split)."""
+    step = Step(dev, stream, 4, fmt, dtype, 8, 1, 64, 64, [2000, 1500, 1900] + [1700] * 5, seq_ids=list(range(8)) * 60)
+    out, lse = step.run(scratch)
+    step.check(out, lse, skip=set(range(480)) - {0, 1, 2, 100, 479})
+    step.free()
+
+
 @pytest.mark.parametrize("fmt", list(FORMATS))
 @pytest.mark.parametrize("window", [1, 16, 50, 1000])
 def test_window(dev, stream, scratch, fmt, window):

@@ -99,6 +99,27 @@ def test_write_then_read(dev, stream, oracle, fmt, dtype, heads, dim, block, row
     paged.free()
 
 
+def test_q8_rows_are_within_a_rounding_of_a_sessions(dev, stream, oracle):
+    """The sessions' codec takes the quotient amax / 127, kv_write the product with 1 / 127: the f16 scales are the same or
+    neighbours, and the whole numbers the same or one apart where a value lies next to a half."""
+    rng = np.random.default_rng(8)
+    x = (rng.standard_normal((400, 8, 256)) * np.exp2(rng.uniform(-6, 6, (400, 8, 1)))).astype(np.float32)
+    paged = Paged(dev, rng, "q8_0", 8, 256, 16, [400])
+    b, pb, sb = dev.upload(x), dev.upload(np.arange(400, dtype=np.int32)), dev.upload(np.zeros(400, np.int32))
+    cuda.kv_write(stream, paged.cache, cuda.KvRows(b, b, pb, 400, seq=sb))
+    stream.synchronize()
+    got = paged.download()[0][paged.slots(0, np.arange(400))].reshape(400, -1, 34)
+    want = np.stack([oracle.kv_encode_row(cuda.KV_Q8_0, r) for r in x.reshape(400, -1)]).reshape(400, -1, 34)
+    scales = [np.ascontiguousarray(a[:, :, :2]).view(np.uint16).astype(int) for a in (got, want)]
+    apart = np.abs(scales[0] - scales[1])
+    assert apart.max() <= 1 and apart.mean() < 1e-3
+    off = np.abs(got[:, :, 2:].view(np.int8).astype(int) - want[:, :, 2:].view(np.int8).astype(int))
+    assert off.max() <= 1 and off.mean() < 1e-4
+    for q in (b, pb, sb):
+        q.free()
+    paged.free()
+
+
 @pytest.mark.parametrize("fmt", list(FORMATS))
 def test_strided_rows_of_a_fused_projection(dev, stream, oracle, fmt):
     """K and V as columns of one array, written from and read into; what lies between the columns stays."""

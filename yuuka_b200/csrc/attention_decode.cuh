@@ -49,17 +49,10 @@ struct DecodeParams {
     int * counters;    // zero between calls: joins of both lists, CTAs of the joining kernel done
 };
 
-#ifndef DEC_MIN_TILES
-#define DEC_MIN_TILES 1
-#endif
 constexpr int DEC_WARPS = 4096;         // of a grid, at most
 constexpr size_t DEC_PARTIAL_BYTES = 24u << 20;
 enum { DEC_SHORT, DEC_LONG, DEC_DONE, DEC_COUNTERS };
-#ifndef DEC_SHORT_N
-#define DEC_SHORT_N 32
-#define DEC_JOIN_SM 4
-#endif
-constexpr int DEC_SHORT_MOST = DEC_SHORT_N;      // partials that a warp joins
+constexpr int DEC_SHORT_MOST = 32;      // partials that a warp joins
 constexpr float DEC_P_LOG2 = 7.0f;      // log2 of the factor that probabilities carry
 constexpr float DEC_SLACK = 8.0f;       // log2 of what a score may pass the running maximum by before sums are rescaled
 constexpr int DEC_SMEM_SM = 233472;     // shared memory of an SM
@@ -156,25 +149,15 @@ template <int PAIR> __device__ __forceinline__ uint32_t dec_int8(uint32_t x) {
 // the products as two parts (22 bits); otherwise f16 or bf16 and one part (11 bits, no less than such an output can tell).
 template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     static constexpr bool IS_F32 = FMT == YUUKA_KV_F32, IS_Q8 = FMT == YUUKA_KV_Q8_0, IS_F8 = FMT == YUUKA_KV_F8;
-        // warps of a CTA, CTAs of an SM
-#ifndef DEC_W64
-#define DEC_W64 4
-#define DEC_R64 2
-#define DEC_W128 4
-#define DEC_R128 2
-#define DEC_W256 4
-#define DEC_R256 1
-#endif
+        // Warps of a CTA and CTAs of an SM: twelve warps, or eight where the sums, queries and copies of 256 dimensions take the
+    // registers (at 12 and 8 instead of 8 and 4 warps, 8 sequences of 32768 with 8 KV heads of 128 took 160 us instead of 164, 32 of
+    // 256 to 4000 with 4 of 256 took 41 instead of 44). Small CTAs are resident sooner: one short sequence took 7.4 us with 2 of
+    // four warps, 7.6 with one of eight.
     static constexpr bool NARROW = NT == 2 || (IS_F32 && HD > 64);
-    static constexpr int W = NARROW ? 4 : HD == 256 ? DEC_W256 : HD == 128 ? DEC_W128 : DEC_W64;
-    static constexpr int RESIDENT = NARROW ? (HD == 256 ? 1 : 2) : HD == 256 ? DEC_R256 : HD == 128 ? DEC_R128 : DEC_R64;
-#ifndef DEC_K256
-#define DEC_K256 1
-#define DEC_K128 2
-#define DEC_K64 2
-#endif
-    // keys of a tile: sixteen make one row tile of the products
-    static constexpr int HALVES = IS_F32 && HD > 64 ? 1 : HD == 256 ? DEC_K256 : HD == 128 ? DEC_K128 : DEC_K64, KEYS = 16 * HALVES;
+    static constexpr int W = 4, RESIDENT = NARROW ? (HD == 256 ? 1 : 2) : (HD == 256 ? 2 : 3);
+    // keys of a tile: sixteen make one row tile of the products, and two of them share the walk, the maximum and the queries' reads
+    // where registers allow (64 sequences of 500 to 8000 in F8: 106 -> 99 us)
+    static constexpr int HALVES = HD == 256 || (HD == 128 && (WIDE || IS_F32)) ? 1 : 2, KEYS = 16 * HALVES;
     static constexpr int COLS = 8 * NT, PARTS = WIDE ? 2 : 1;
     // Q8_0: words from key to key. K: 8 or 24 modulo 32, V: 4 or 12 modulo 16, which keeps the lanes' reads on different banks
     static constexpr int Q8_K = HD == 64 ? 24 : (HD == 128 ? 40 : 88), Q8_V = HD == 64 ? 20 : (HD == 128 ? 36 : 68);
@@ -389,7 +372,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
     total = __reduce_add_sync(0xffffffffu, total);
     const unsigned units = p.cache.kv_heads * p.head_tiles, warps = gridDim.x * W, self = blockIdx.x * W + warp;
     const unsigned teams = max(warps / units, 1u), team = min(self / units, units > warps ? 0u : ~0u);
-    const unsigned share = max((total + teams - 1) / teams, (unsigned)DEC_MIN_TILES);
+    const unsigned share = (total + teams - 1) / teams;
     const unsigned begin = team * share;
     const int count = team < teams && begin < total ? (int)min(share, total - begin) : 0;
 #pragma unroll 1
@@ -724,7 +707,8 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 #pragma unroll
                     for (int e = 0; e < 4; e++) s[nt][e] = s2[nt][e] = 0.0f;
                 if constexpr (S::IS_F32) {
-                    // three products of tf32 parts: hi hi, hi lo, lo hi (the tensor core itself drops what a first part leaves)
+                    // three products of tf32 parts: hi hi, hi lo, lo hi (the tensor core itself drops what a first part leaves). What
+                    // the first ones cut off counts (see add_values): two at a time, added in f32
 #pragma unroll
                     for (int c = 0; c < HD / 16; c++) {
                         const uint4 ka = dec_lds4(kh + S::k_piece(g, 4 * c + t)), kb = dec_lds4(kh + S::k_piece(g + 8, 4 * c + t));
@@ -736,14 +720,17 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         for (int i = 0; i < 8; i++) al[i] = dec_rest(a[i]);
 #pragma unroll
                         for (int i = 0; i < 4; i++) bl[i] = dec_rest(b[i]);
-                        dec_mma8(s[0], a[0], a[1], a[2], a[3], b[0], b[1]);
-                        dec_mma8(s2[0], a[4], a[5], a[6], a[7], b[2], b[3]);
-                        dec_mma8(s[0], al[0], al[1], al[2], al[3], b[0], b[1]);
+                        float d[4] = {0.f, 0.f, 0.f, 0.f};
+                        dec_mma8(d, a[0], a[1], a[2], a[3], b[0], b[1]);
+                        dec_mma8(d, a[4], a[5], a[6], a[7], b[2], b[3]);
+                        dec_mma8(s2[0], al[0], al[1], al[2], al[3], b[0], b[1]);
                         dec_mma8(s2[0], al[4], al[5], al[6], al[7], b[2], b[3]);
                         if constexpr (WIDE) {  // (16-bit queries have no second part)
-                            dec_mma8(s[0], a[0], a[1], a[2], a[3], bl[0], bl[1]);
+                            dec_mma8(s2[0], a[0], a[1], a[2], a[3], bl[0], bl[1]);
                             dec_mma8(s2[0], a[4], a[5], a[6], a[7], bl[2], bl[3]);
                         }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[0][e] += d[e];
                     }
                 } else if constexpr (S::IS_Q8) {
                     const uint32_t ka = kh + 4 * (g * S::Q8_K + 1), kb = ka + 32 * S::Q8_K;  // keys g and g + 8
@@ -937,7 +924,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                             }
 #pragma unroll
                             for (int j = 0; j < 2; j++) {
-                                float d[4] = {0.f, 0.f, 0.f, 0.f};  // (summed on its own, as in add_values)
+                                float d[4] = {0.f, 0.f, 0.f, 0.f};  // (summed on its own, as in add_values; small terms first)
 #pragma unroll
                                 for (int h = 0; h < 2; h++) {
                                     const uint32_t a[4] = {v[2 * h][2 * j], v[2 * h][2 * j + 1], v[2 * h + 1][2 * j], v[2 * h + 1][2 * j + 1]};
@@ -946,8 +933,10 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                                     for (int i = 0; i < 4; i++) al[i] = dec_rest(a[i]);
                                     dec_mma8(d, al[0], al[1], al[2], al[3], pk[2 * h], pk[2 * h + 1]);
                                     dec_mma8(d, a[0], a[1], a[2], a[3], pl[2 * h], pl[2 * h + 1]);
-                                    dec_mma8(d, a[0], a[1], a[2], a[3], pk[2 * h], pk[2 * h + 1]);
                                 }
+#pragma unroll
+                                for (int h = 0; h < 2; h++)
+                                    dec_mma8(d, v[2 * h][2 * j], v[2 * h][2 * j + 1], v[2 * h + 1][2 * j], v[2 * h + 1][2 * j + 1], pk[2 * h], pk[2 * h + 1]);
 #pragma unroll
                                 for (int e = 0; e < 4; e++) o[0][c][j][e] += d[e];
                             }
@@ -1128,7 +1117,8 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                     if (from_start && lane == 0) {
                         const int last = (int)((begin + it + use.left - 1) / share);
                         const int list = last - (int)team < DEC_SHORT_MOST ? DEC_SHORT : DEC_LONG;
-                        p.joins[list * DEC_WARPS + atomicAdd(p.counters + list, 1)] = make_int4(use.b, (int)unit, (int)team, last);
+                        const int at = atomicAdd(p.counters + list, 1);
+                        if (at < DEC_WARPS) p.joins[list * DEC_WARPS + at] = make_int4(use.b, (int)unit, (int)team, last);
                     }
                 }
                 fresh = true;
@@ -1143,17 +1133,22 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 // The units that several teams share. Few partials: a CTA takes a unit, a warp a column, a lane HD / 32 dimensions. Many: a CTA
 // takes 64 dimensions of a column at a time; groups of 16 threads take every 16th partial, so that many loads are in flight, and
 // are added in their order.
-constexpr int JOIN_THREADS = 256, JOIN_CTAS_SM = DEC_JOIN_SM, JOIN_LANES = 16, JOIN_GROUPS = JOIN_THREADS / JOIN_LANES;
+constexpr int JOIN_THREADS = 256, JOIN_CTAS_SM = 4, JOIN_LANES = 16, JOIN_GROUPS = JOIN_THREADS / JOIN_LANES;
 template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_THREADS) attention_decode_join_kernel(const DecodeParams p) {
     constexpr int PART = COLS * (HD + 2), SLICES = HD / (4 * JOIN_LANES), DIMS = HD / 32;
     __shared__ float factor[DEC_WARPS], reduce[2][JOIN_THREADS / 32];
     __shared__ float4 sums[JOIN_GROUPS][JOIN_LANES];
     pdl_entry();
     const int tid = threadIdx.x, units = p.cache.kv_heads * p.head_tiles, group = tid / JOIN_LANES;
-    const int few = p.counters[DEC_SHORT], jobs = p.counters[DEC_LONG] * COLS * SLICES;
+    const int few = min(p.counters[DEC_SHORT], DEC_WARPS), jobs = min(p.counters[DEC_LONG], DEC_WARPS) * COLS * SLICES;
+    // (calls that share scratch memory against the rule may read one another's joins: wrong results, but no other memory)
+    auto sound = [&](const int4 & j) {
+        return (unsigned)j.x < (unsigned)p.batch && (unsigned)j.y < (unsigned)units && j.z >= 0 && j.z < j.w && j.w < DEC_WARPS / units;
+    };
 #pragma unroll 1
     for (int job = blockIdx.x; job < few; job += gridDim.x) {
         const int4 join = p.joins[job];
+        if (!sound(join)) continue;
         const DecodeHeads h = decode_heads(p, join.y);
         const int n = join.w - join.z + 1, lane = tid & 31, dim = lane * DIMS;
         const float * first = p.partial + ((size_t)join.z * units + join.y) * 2 * PART;
@@ -1200,6 +1195,7 @@ template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_TH
 #pragma unroll 1
     for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
         const int4 join = p.joins[DEC_WARPS + job / (COLS * SLICES)];
+        if (!sound(join)) continue;
         const int col = job / SLICES % COLS, dim = 4 * (job % SLICES * JOIN_LANES + tid % JOIN_LANES);
         const DecodeHeads h = decode_heads(p, join.y);
         if (col >= h.count) continue;

@@ -252,6 +252,8 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MovePar
     uint8_t * row = (u.is_v ? p.cache.v : p.cache.k) + (int64_t)slot * p.cache.row_bytes;
 
     // Scales: every division is made once, by one lane, for all chunks at a time, and handed to the lanes that need it.
+    // (amax / 127 and amax / 448 by their inverses: within an ulp of the quotient. Of Q8_0's scales, f16 in the end, about one in
+    // 16,000 is the neighbour of the one that a session's rows would have.)
     float scale[MOVE_CHUNKS], inv[MOVE_CHUNKS];
     uint32_t half_scale = 0;  // Q8_0: of block lane (eight of a chunk)
     if constexpr (FMT == YUUKA_KV_Q8_0 || FMT == YUUKA_KV_F8) {
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MovePar
                 const float a = __shfl_sync(0xffffffffu, amax[c], 4 * (lane & 7));
                 if (lane >> 3 == c) mine = a;
             }
-            const float s = mine / 127.0f, r = 1.0f / s;
+            const float s = mine * (1.0f / 127.0f), r = 1.0f / s;
             half_scale = half_up(s);
 #pragma unroll
             for (int c = 0; c < MOVE_CHUNKS; c++) {
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MovePar
         } else {
             const int at = lane & (LANES - 1);
             const float mine = (at & 2) ? ((at & 1) ? amax[3] : amax[2]) : ((at & 1) ? amax[1] : amax[0]);
-            const float r = (at & 4) ? mine / 448.0f : 448.0f / mine;
+            const float r = (at & 4) ? mine * (1.0f / 448.0f) : 1.0f / mine * 448.0f;
 #pragma unroll
             for (int c = 0; c < MOVE_CHUNKS; c++) {
                 inv[c] = __shfl_sync(0xffffffffu, r, lane - at + c);
