@@ -128,14 +128,6 @@ __device__ __forceinline__ uint2 dec_e4m3(uint32_t four) {
                  : "r"(four));
     return h;
 }
-// The same by integer instructions, as pairs of f16 that are 2^-8 of the values: an E4M3's bits shifted to where an f16 has its
-// exponent and fraction mean 2^-8 of its value (subnormals too; a NaN's do not stay one). The conversions share a pipe with the
-// exponentials that takes eight cycles for one; with K and V both converted there it was 92 % busy.
-__device__ __forceinline__ uint2 dec_e4m3_bits(uint32_t four) {
-    const uint32_t lo = __byte_perm(four, 0u, 0x4140), hi = __byte_perm(four, 0u, 0x4342);  // one byte in each half
-    // twice the sign's place takes it to the place above, and all goes up by seven
-    return make_uint2((lo + (lo & 0x00800080u)) * 128u, (hi + (hi & 0x00800080u)) * 128u);
-}
 // bytes 0 and 1 (PAIR 0) or 2 and 3 of x, unsigned with an offset of 128, as f16 pairs of the signed values: exact
 template <int PAIR> __device__ __forceinline__ uint32_t dec_int8(uint32_t x) {
     const uint32_t h = __byte_perm(x, 0x64646464u, PAIR ? 0x4342 : 0x4140);  // 1024 + byte
@@ -785,7 +777,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
-                            const uint2 x = dec_e4m3_bits(wa[i]), y = dec_e4m3_bits(wb[i]);
+                            const uint2 x = dec_e4m3(wa[i]), y = dec_e4m3(wb[i]);
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
                                 const uint4 f = query(nt, 4 * c + i);
@@ -817,7 +809,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         for (int e = 0; e < 4; e++) s[nt][e] += s2[nt][e];
                 if constexpr (S::IS_F8) {
                     const uint32_t at = ks + S::K16 * HALVES + 64 * half + 4 * g;
-                    const float d0 = 256.0f * __uint_as_float(dec_lds(at)), d1 = 256.0f * __uint_as_float(dec_lds(at + 32));
+                    const float d0 = __uint_as_float(dec_lds(at)), d1 = __uint_as_float(dec_lds(at + 32));
                     vd[half][0] = __uint_as_float(dec_lds(at + 4 * KEYS));
                     vd[half][1] = __uint_as_float(dec_lds(at + 4 * KEYS + 32));
 #pragma unroll
@@ -1131,9 +1123,9 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 }
 
 // The units that several teams share. Few partials: a CTA takes a unit, a warp a column, a lane HD / 32 dimensions. Many: a CTA
-// takes 64 dimensions of a column at a time; groups of 16 threads take every 16th partial, so that many loads are in flight, and
+// takes 32 dimensions of a column at a time; groups of 8 threads take every 32nd partial, so that many loads are in flight, and
 // are added in their order.
-constexpr int JOIN_THREADS = 256, JOIN_CTAS_SM = 4, JOIN_LANES = 16, JOIN_GROUPS = JOIN_THREADS / JOIN_LANES;
+constexpr int JOIN_THREADS = 256, JOIN_CTAS_SM = 4, JOIN_LANES = 8, JOIN_GROUPS = JOIN_THREADS / JOIN_LANES;
 template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_THREADS) attention_decode_join_kernel(const DecodeParams p) {
     constexpr int PART = COLS * (HD + 2), SLICES = HD / (4 * JOIN_LANES), DIMS = HD / 32;
     __shared__ float factor[DEC_WARPS], reduce[2][JOIN_THREADS / 32];
