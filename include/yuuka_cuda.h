@@ -295,7 +295,7 @@ typedef struct yuuka_attention_decode_args {
     int32_t window;        /* 0: none */
     float scale;           /* 0: 1 / sqrt(head_dim) */
 } yuuka_attention_decode_args;
-/* Device memory for the joining of split sequences: one for all shapes, a few MB. Calls that use the same one are
+/* Device memory for the joining of split sequences: one for all shapes, 41 MB. Calls that use the same one are
  * ordered (one stream, or events between them); graphs that may run at the same time are captured with one each. */
 typedef struct yuuka_attention_scratch yuuka_attention_scratch;
 YUUKA_API yuuka_status yuuka_attention_scratch_create(yuuka_device * dev, yuuka_attention_scratch ** out);

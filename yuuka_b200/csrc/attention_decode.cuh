@@ -50,7 +50,7 @@ struct DecodeParams {
 };
 
 constexpr int DEC_WARPS = 4096;         // of a grid, at most
-constexpr size_t DEC_PARTIAL_BYTES = 24u << 20;
+constexpr size_t DEC_PARTIAL_BYTES = 40u << 20;  // two of the 1184 warps with the largest sums (16 columns of 256) take 39
 enum { DEC_SHORT, DEC_LONG, DEC_DONE, DEC_COUNTERS };
 constexpr int DEC_SHORT_MOST = 32;      // partials that a warp joins
 constexpr float DEC_P_LOG2 = 7.0f;      // log2 of the factor that probabilities carry
@@ -93,6 +93,10 @@ template <int BYTES> __device__ __forceinline__ void dec_copy(uint32_t dst, cons
 // the cutting alone would make all scores 2^-22 too small.
 __device__ __forceinline__ uint32_t dec_rest(uint32_t x) {
     return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u)) + 0x1000u;
+}
+// the same of 16 bytes, of which n are read and the others become zeros
+__device__ __forceinline__ void dec_copy_part(uint32_t dst, const uint8_t * src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void dec_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void dec_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -146,18 +150,22 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     // 256 to 4000 with 4 of 256 took 41 instead of 44). Small CTAs are resident sooner: one short sequence took 7.4 us with 2 of
     // four warps, 7.6 with one of eight.
     static constexpr bool NARROW = NT == 2 || (IS_F32 && HD > 64);
-    static constexpr int W = 4, RESIDENT = NARROW ? (HD == 256 ? 1 : 2) : (HD == 256 ? 2 : 3);
+    static constexpr int W = 4, RESIDENT = HD == 256 ? (IS_F32 || (FMT == YUUKA_KV_F16 && NT == 2 && WIDE) ? 1 : 2) : (NARROW ? 2 : 3);
     // keys of a tile: sixteen make one row tile of the products, and two of them share the walk, the maximum and the queries' reads
     // where registers allow (64 sequences of 500 to 8000 in F8: 106 -> 99 us)
     static constexpr int HALVES = HD == 256 || (HD == 128 && (WIDE || IS_F32)) ? 1 : 2, KEYS = 16 * HALVES;
     static constexpr int COLS = 8 * NT, PARTS = WIDE ? 2 : 1;
-    // Q8_0: words from key to key. K: 8 or 24 modulo 32, V: 4 or 12 modulo 16, which keeps the lanes' reads on different banks
-    static constexpr int Q8_K = HD == 64 ? 24 : (HD == 128 ? 40 : 88), Q8_V = HD == 64 ? 20 : (HD == 128 ? 36 : 68);
+    // Q8_0: a head's blocks of 34 bytes, copied as the 16-byte pieces that hold them, which begin up to 12 bytes before. (Copied by
+    // words, 24 sequences of 8000 with 16 KV heads of 64 took 176 us.) A piece more or less from key to key would put the lanes'
+    // reads of V on the same banks.
+    static constexpr int Q8_PIECES = HD == 64 ? 5 : (HD == 128 ? 9 : 17), Q8_ROW = 16 * Q8_PIECES;
+    static constexpr bool Q8_STARTS = IS_Q8 && HD != 256;  // a head of 256 is 17 pieces itself
     // F8: a lane's piece of V, 16 dimensions of 128 or 8 of 64; the scales of the tile's K and V lie behind K
     static constexpr int F8_V = HD == 64 ? 8 : 16;
-    static constexpr int K16 = IS_F32 ? HD * 64 : (IS_Q8 ? 64 * Q8_K : (IS_F8 ? HD * 16 : HD * 32));  // bytes of sixteen keys
-    static constexpr int V16 = IS_F32 ? HD * 64 : (IS_Q8 ? 64 * Q8_V : (IS_F8 ? HD * 16 : HD * 32));
-    static constexpr int K_BYTES = K16 * HALVES + (IS_F8 ? 8 * KEYS : 0), V_BYTES = V16 * HALVES;
+    static constexpr int K16 = IS_F32 ? HD * 64 : (IS_Q8 ? 16 * Q8_ROW : (IS_F8 ? HD * 16 : HD * 32));  // bytes of sixteen keys
+    static constexpr int V16 = IS_F32 ? HD * 64 : (IS_Q8 ? 16 * Q8_ROW : (IS_F8 ? HD * 16 : HD * 32));
+    // (behind the tile: F8's scales of K and V; where in their first pieces Q8_0's rows begin)
+    static constexpr int K_BYTES = K16 * HALVES + (IS_F8 ? 8 * KEYS : Q8_STARTS ? 4 * KEYS : 0), V_BYTES = V16 * HALVES + (Q8_STARTS ? 4 * KEYS : 0);
     // Rows of the other formats, K and V: their 16-byte pieces are copied by lines of 128 bytes, eight neighbouring lanes to a
     // line. (With lanes that copy what they will read themselves, four to a piece of K and every fourth to a line of V, the SMs
     // fetched V's sectors twice: 1.61 GB for 1.07.) Pieces trade places within their line so that the eight lanes of a read find
@@ -196,7 +204,7 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     __device__ static __forceinline__ int q_dim(int m, int half, int t) {
         if constexpr (IS_Q8) {
             const int blk = m >> 1, h = m & 1;
-            return blk * 32 + ((blk & 1) ? 4 * (2 * t + h) + 2 * half : (4 * (1 + 2 * t + h) - 2 + 2 * half) & 31);
+            return blk * 32 + ((blk & 1) ? 4 * (t + 4 * h) + 2 * half : (4 * (1 + t + 4 * h) - 2 + 2 * half) & 31);
         } else if constexpr (IS_F8) {
             return 64 * (m >> 2) + 16 * t + 4 * (m & 3) + 2 * half;
         } else {
@@ -409,8 +417,10 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
         // the pools at the unit's head and this lane's piece
         constexpr int HEAD_BYTES = FMT == YUUKA_KV_F32 ? HD * 4 : (FMT == YUUKA_KV_F16 ? HD * 2 : (FMT == YUUKA_KV_Q8_0 ? HD / 32 * 34 : HD));
         const int kv_head = unit / p.head_tiles;
-        const uint8_t * const k_at = p.cache.k + (int64_t)kv_head * HEAD_BYTES + (S::IS_Q8 ? 4 * (lane & 7) : 16 * (lane & (S::LANES - 1)));
-        const uint8_t * const v_at = p.cache.v + (int64_t)kv_head * HEAD_BYTES + (S::IS_Q8 ? 4 * (lane & 7) : 16 * (lane & (S::LANES - 1)));
+        const unsigned head_at = kv_head * HEAD_BYTES;
+        [[maybe_unused]] const uint8_t * const k_at = p.cache.k + head_at + 16 * (lane & (S::LANES - 1));
+        [[maybe_unused]] const uint8_t * const v_at = p.cache.v + head_at + 16 * (lane & (S::LANES - 1));
+        [[maybe_unused]] const uint64_t pool_bytes = (uint64_t)p.cache.pool_blocks * p.cache.block_size * (uint64_t)p.cache.row_bytes;
         const int32_t * table = nullptr;
         const unsigned row_bytes = (unsigned)p.cache.row_bytes;
         auto look_up = [&] {
@@ -440,23 +450,21 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         }
                     }
                 }
+                if constexpr (S::Q8_STARTS) {  // written for tiles that copy nothing as well: they are read all the same
+                    __syncwarp();
+                    if (lane < KEYS) dec_sts(put + S::K16 * HALVES + 4 * lane, copies ? (uint32_t)((uint64_t)pool_row * row_bytes + head_at) & 15u : 0u);
+                }
                 if (copies) {
-                    auto row_of = [&](int key) { return (V ? v_at : k_at) + (uint64_t)__shfl_sync(0xffffffffu, pool_row, key) * row_bytes; };
+                    [[maybe_unused]] auto row_of = [&](int key) { return (V ? v_at : k_at) + (uint64_t)__shfl_sync(0xffffffffu, pool_row, key) * row_bytes; };
                     if constexpr (S::IS_Q8) {
-                        constexpr int WORDS = HD / 32 * 34 / 4;
-                        const int l8 = lane & 7;
+                        const uint8_t * const base = V ? p.cache.v : p.cache.k;
 #pragma unroll
-                        for (int kg = 0; kg < KEYS / 4; kg++) {
-                            const int key = 4 * kg + (lane >> 3);
-                            const uint8_t * src = row_of(key);
-                            const uint32_t dst = put + 4 * (V ? key * S::Q8_V : key * S::Q8_K + 1) + 4 * l8;
-#pragma unroll
-                            for (int i = 0; i < (WORDS + 7) / 8; i++) {
-                                const int w = 8 * i + l8;
-                                // K: one word between the pairs of blocks (17 words), so that lanes read two aligned words
-                                const int gap = V ? 0 : (w >= 17) + (w >= 34) + (w >= 51);
-                                if (8 * i + 7 < WORDS || w < WORDS) dec_copy<4>(dst + 32 * i + 4 * gap, src + 32 * i);
-                            }
+                        for (int i = 0; i < (KEYS * S::Q8_PIECES + 31) / 32; i++) {
+                            const int at = 32 * i + lane, key = at / S::Q8_PIECES, piece = at - key * S::Q8_PIECES;
+                            const uint64_t from = (((uint64_t)__shfl_sync(0xffffffffu, pool_row, key & 31) * row_bytes + head_at) & ~15ull) + 16 * piece;
+                            // (the last piece of the pool's last row may reach beyond the pool)
+                            if (32 * i + 31 < KEYS * S::Q8_PIECES || key < KEYS)
+                                dec_copy_part(put + key * S::Q8_ROW + 16 * piece, base + from, (int)min((uint64_t)16, pool_bytes - min(from, pool_bytes)));
                         }
                     } else {
                         constexpr int AT_ONCE = 32 / S::LANES;  // keys
@@ -725,15 +733,22 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         for (int e = 0; e < 4; e++) s[0][e] += d[e];
                     }
                 } else if constexpr (S::IS_Q8) {
-                    const uint32_t ka = kh + 4 * (g * S::Q8_K + 1), kb = ka + 32 * S::Q8_K;  // keys g and g + 8
+                    // keys g and g + 8
+                    uint32_t ka = kh + g * S::Q8_ROW, kb = ka + 8 * S::Q8_ROW;
+                    if constexpr (S::Q8_STARTS) {
+                        const uint32_t starts = ks + S::K16 * HALVES + 64 * half + 4 * g;
+                        ka += dec_lds(starts);
+                        kb += dec_lds(starts + 32);
+                    }
 #pragma unroll
                     for (int pair = 0; pair < HD / 64; pair++) {
                         uint32_t w[2][4];   // [key][word]: two of the even block, two of the odd one
                         float d[2][2];      // [key][block]
 #pragma unroll
                         for (int k = 0; k < 2; k++) {
-                            const uint32_t at = (k ? kb : ka) + 72 * pair;
-                            const uint2 even = dec_lds2(at + 4 * (1 + 2 * t)), odd = dec_lds2(at + 4 * (9 + 2 * t));
+                            const uint32_t at = (k ? kb : ka) + 68 * pair;
+                            const uint2 even = make_uint2(dec_lds(at + 4 * (1 + t)), dec_lds(at + 4 * (5 + t)));
+                            const uint2 odd = make_uint2(dec_lds(at + 4 * (9 + t)), dec_lds(at + 4 * (13 + t)));
                             const uint32_t w0 = dec_lds(at), w8 = dec_lds(at + 32);
                             d[k][0] = __half2float(__ushort_as_half((unsigned short)w0));
                             d[k][1] = __half2float(__ushort_as_half((unsigned short)(w8 >> 16)));
@@ -935,18 +950,33 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         }
                     }
                 } else if constexpr (S::IS_Q8) {
+                    // where the rows of keys 2t + (k & 1) + 8 (k >> 1) begin
+                    const uint32_t starts = vs + S::V16 * HALVES;
+                    uint32_t row_at[HALVES][4];
+#pragma unroll
+                    for (int h = 0; h < HALVES; h++)
+#pragma unroll
+                        for (int k = 0; k < 4; k += 2) {
+                            const int key = 16 * h + 2 * t + 8 * (k >> 1);
+                            const uint2 start = S::Q8_STARTS ? dec_lds2(starts + 4 * key) : make_uint2(0, 0);
+                            row_at[h][k] = vs + key * S::Q8_ROW + start.x;
+                            row_at[h][k + 1] = vs + (key + 1) * S::Q8_ROW + start.y;
+                        }
                     // scales of V: of keys g and g + 8, block by block, into the probabilities
                     float d[HALVES][2][HD / 32];
                     uint32_t largest = 0;
 #pragma unroll
                     for (int h = 0; h < HALVES; h++)
 #pragma unroll
-                        for (int k = 0; k < 2; k++)
+                        for (int k = 0; k < 2; k++) {
+                            const int key = 16 * h + g + 8 * k;
+                            const uint32_t at = vs + key * S::Q8_ROW + (S::Q8_STARTS ? dec_lds(starts + 4 * key) : 0);
 #pragma unroll
                             for (int blk = 0; blk < HD / 32; blk++) {
-                                d[h][k][blk] = __half2float(__ushort_as_half((unsigned short)dec_lds_u16(vs + h * S::V16 + 4 * (g + 8 * k) * S::Q8_V + 34 * blk)));
+                                d[h][k][blk] = __half2float(__ushort_as_half((unsigned short)dec_lds_u16(at + 34 * blk)));
                                 largest = max(largest, __float_as_uint(fabsf(d[h][k][blk])));
                             }
+                        }
                     const float inv = take_v_scale(largest);
 #pragma unroll
                     for (int c = 0; c < CHUNKS; c++) {
@@ -957,7 +987,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                             uint32_t w[4];
 #pragma unroll
                             for (int k = 0; k < 4; k++) {
-                                const uint32_t at = vs + h * S::V16 + 4 * (2 * t + (k & 1) + 8 * (k >> 1)) * S::Q8_V + 68 * (c >> 1);
+                                const uint32_t at = row_at[h][k] + 68 * (c >> 1);
                                 if (c & 1) w[k] = dec_lds(at + 4 * (9 + g));
                                 else {
                                     const uint32_t x = dec_lds(at + 4 * (1 + g)), w0 = dec_lds(at);
