@@ -242,7 +242,7 @@ YUUKA_API uint64_t yuuka_kv_row_bytes(int32_t format, int32_t kv_heads, int32_t 
 
 /* Device data (sequence ids, positions, lengths, block ids) is checked by the kernels: a call touches no memory outside
  * its buffers whatever they hold. What is out of range is not written, or read as NaN, and the bits below are or-ed into
- * `status`, an int32 on the device that the caller zeroes (NULL: not recorded). */
+ * `status`, an int32 on the device that the caller zeroes (NULL: not recorded), apart from what else a call reads or writes. */
 #define YUUKA_KV_STATUS_BLOCK 0x1    /* a block id outside 0..pool_blocks-1 */
 #define YUUKA_KV_STATUS_SEQUENCE 0x2 /* a sequence id outside 0..sequences-1 */
 #define YUUKA_KV_STATUS_POSITION 0x4 /* a position or length beyond table_stride * block_size, or a length below 0 */
@@ -261,7 +261,7 @@ typedef struct yuuka_kv_rows {
     uint32_t dtype;
 } yuuka_kv_rows;
 /* Writes the rows into the pools, in the pools' format; rows without a token leave everything as it is. The tokens of a
- * call are distinct: where two rows name the same one, each head of it holds values of either. Asynchronous on stream. k and
+ * call are distinct: where two rows name the same one, its row becomes a mixture of both. Asynchronous on stream. k and
  * v start at multiples of 16 bytes from row to row. */
 YUUKA_API yuuka_status yuuka_kv_write(yuuka_stream * stream, const yuuka_kv_cache * cache, const yuuka_kv_rows * rows,
                                       yuuka_event * completion);

@@ -153,6 +153,21 @@ int main() {
     refuses("out over q", INVALID, "out lies over q", [](World & w) { w.args.out = (yuuka_buffer *)w.args.q; return ATTEND; });
     refuses("out over a pool", INVALID, "lies over", [](World & w) { w.args.out->ptr = w.cache.v->ptr; return ATTEND; });
     refuses("lse over lens", INVALID, "lies over", [](World & w) { w.args.lse->ptr = w.memory + 98304 - 32; return ATTEND; });
+    // status bits are or-ed into memory that the call reads nowhere else
+    refuses("status over pos", INVALID, "status lies over pos", [](World & w) { w.rows.status = (yuuka_buffer *)w.rows.pos; return MOVE; });
+    refuses("status over seq", INVALID, "status lies over seq", [](World & w) { w.rows.status->ptr = w.memory + 49408 + 16; return MOVE; });
+    refuses("status over the table", INVALID, "status lies over the block table", [](World & w) {
+        w.rows.status = w.args.status = (yuuka_buffer *)w.cache.tables;
+        return ALL;
+    });
+    refuses("status over rows that are read", INVALID, "status lies over k", [](World & w) { w.rows.status->ptr = w.memory + 32768 + 64; return WRITE; });
+    refuses("status over a pool that is read", INVALID, "status lies over the V pool", [](World & w) {
+        w.rows.status->ptr = w.args.status->ptr = w.memory + 8192;
+        return READ | ATTEND;
+    });
+    refuses("status over lens", INVALID, "status lies over lens", [](World & w) { w.args.status->ptr = w.memory + 98304 + 4; return ATTEND; });
+    refuses("status over q", INVALID, "status lies over q", [](World & w) { w.args.status->ptr = w.memory + 65536; return ATTEND; });
+    refuses("status over out", INVALID, "out lies over status", [](World & w) { w.args.status->ptr = w.memory + 73728 + 4; return ATTEND; });
     refuses("no lengths", INVALID, "lens is null", [](World & w) { w.args.lens = nullptr; return ATTEND; });
     refuses("scratch of another device", INVALID, "scratch is on device 1", [](World & w) { w.scratch.dev = &w.other; return ATTEND; });
     refuses("too many keys", UNSUPPORTED, "too many", [](World & w) {

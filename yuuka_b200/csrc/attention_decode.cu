@@ -103,18 +103,19 @@ extern "C" yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_atte
             const yuuka_buffer * buf;
             uint64_t offset, bytes;
         };
-        const Range outs[2] = {{"out", a->out, a->out_offset, ob}, {"lse", a->lse, a->lse_offset, lb}};
-        const Range ins[8] = {{"q", a->q, a->q_offset, qb},
+        const Range outs[3] = {{"out", a->out, a->out_offset, ob}, {"lse", a->lse, a->lse_offset, lb}, {"status", a->status, a->status_offset, 4}};
+        const Range ins[7] = {{"q", a->q, a->q_offset, qb},
                               {"gate", a->gate, a->gate_offset, qb},
                               {"lens", a->lens, a->lens_offset, 4 * batch},
                               {"seq_ids", a->seq_ids, a->seq_ids_offset, 4 * batch},
-                              {"status", a->status, a->status_offset, 4},
                               {"the K pool", cache->k, cache->k_offset, pool},
                               {"the V pool", cache->v, cache->v_offset, pool},
                               {"the block table", cache->tables, cache->tables_offset, tb}};
         for (const Range & x : outs)
             for (const Range & y : ins) check_apart(op, x.name, x.buf, x.offset, x.bytes, y.name, y.buf, y.offset, y.bytes);
-        check_apart(op, "out", a->out, a->out_offset, ob, "lse", a->lse, a->lse_offset, lb);
+        for (int i = 0; i < 3; i++)
+            for (int j = 0; j < i; j++)
+                check_apart(op, outs[j].name, outs[j].buf, outs[j].offset, outs[j].bytes, outs[i].name, outs[i].buf, outs[i].offset, outs[i].bytes);
 
         p.q = (const uint8_t *)a->q->ptr + a->q_offset;
         p.gate = a->gate ? (const uint8_t *)a->gate->ptr + a->gate_offset : nullptr;

@@ -465,14 +465,18 @@ static yuuka_status move_rows(const char * op, bool write, yuuka_stream * stream
         };
         const Range pools[2] = {{"the K pool", cache->k, cache->k_offset, pool}, {"the V pool", cache->v, cache->v_offset, pool}};
         const Range nums[2] = {{"k", rows->k, rows->k_offset, kb}, {"v", rows->v, rows->v_offset, vb}};
-        const Range lists[4] = {{"the block table", cache->tables, cache->tables_offset, tb},
+        const Range lists[3] = {{"the block table", cache->tables, cache->tables_offset, tb},
                                 {"pos", rows->pos, rows->pos_offset, 4 * rows->rows},
-                                {"seq", rows->seq, rows->seq_offset, 4 * rows->rows},
-                                {"status", rows->status, rows->status_offset, 4}};
+                                {"seq", rows->seq, rows->seq_offset, 4 * rows->rows}};
+        const Range status = {"status", rows->status, rows->status_offset, 4};
+        auto apart = [&](const Range & a, const Range & b) { check_apart(op, a.name, a.buf, a.offset, a.bytes, b.name, b.buf, b.offset, b.bytes); };
         for (const Range & a : write ? pools : nums) {
-            for (const Range & b : write ? nums : pools) check_apart(op, a.name, a.buf, a.offset, a.bytes, b.name, b.buf, b.offset, b.bytes);
-            for (const Range & b : lists) check_apart(op, a.name, a.buf, a.offset, a.bytes, b.name, b.buf, b.offset, b.bytes);
+            for (const Range & b : write ? nums : pools) apart(a, b);
+            for (const Range & b : lists) apart(a, b);
+            apart(a, status);
         }
+        for (const Range & b : lists) apart(status, b);
+        for (const Range & b : write ? nums : pools) apart(status, b);
         if (!write) {
             // (two strided arrays may lie side by side in one: the rows themselves must not meet)
             const uint64_t k0 = (uint64_t)(uintptr_t)rows->k->ptr + rows->k_offset, v0 = (uint64_t)(uintptr_t)rows->v->ptr + rows->v_offset;
