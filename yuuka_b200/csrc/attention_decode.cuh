@@ -1,17 +1,21 @@
 // Attention of one new token per sequence over a paged cache (yuuka_attention_decode): the kernel.
 //
 // Mathematics. A unit is one KV head of one row of the batch, with up to 8 NT of the query heads that share it as columns.
-// Its keys are taken 16 at a time: S^T = K Q^T (keys as the rows of the product, heads as its 8-wide columns), running
+// Its keys are taken 16 or 32 at a time: S^T = K Q^T (keys as the rows of the product, heads as its 8-wide columns), running
 // maximum m and sum l per head, O^T += V^T P^T. Scores live in the base-2 domain, s = (scale log2 e) q.k, and probabilities
 // carry a factor of 2^7, p = 2^(s - m + 7). m is the maximum when the sums were last rescaled, which they are only when a score
 // passes it by 2^8 (in the first tiles, mostly), so the largest p is 2^15 and those down to 2^-21 of 2^m stay normal in f16.
 //
-// What bounds it: the bytes of the cache, read once. The products run on mma.sync: at 148 x 23 bytes a clock (the measured
-// memory rate) they take 10 to 40 % of its issue rate, and operands go straight from the cache's own layout into fragments.
-// The dimension that a product sums over may be taken in any order and a fragment's rows may stand for any dimensions, so a
-// lane copies (cp.async) the 16 bytes of a key that it will itself multiply, and of V the same dimensions of four keys, whose
-// halves one byte permutation pairs up: no lane reads what another has copied, no barrier, no bank conflict. (Q8_0's blocks of
-// 34 bytes are copied by words, and the word at which a lane starts is chosen so that its two words are never misaligned.)
+// What bounds it: the bytes of the cache, read once, over F32 and F16 pools (80 to 100 % of the memory's measured 6.54 TB/s for
+// long sequences; F32 with heads of 256, whose products are three to one, 40 to 78). Over Q8_0 (40 to 55 %) and F8 (47 to 77 %) the instructions that turn bytes into the products' operands take
+// longer than the bytes' way. The products run on mma.sync, whose operands a warp brings from shared memory into the fragments it
+// needs: with one to eight query heads to a KV head the large tensor-core tiles would be empty but for a few columns, and the
+// narrow ones take 10 to 40 % of the issue rate. The dimension that a product sums over may be taken in any order and a fragment's
+// rows may stand for any dimensions, so a lane reads 16 bytes that lie side by side and takes them as its part of four
+// products' operands; of V it reads the same dimensions of four keys, whose halves byte permutations pair up.
+//
+// A warp has a ring of tiles of its own in shared memory, K and V in turn, that cp.async fills several tiles ahead: no barrier of
+// the CTA is waited for. Copies go by lines of 128 bytes.
 //
 // Work is cut at the granularity of warps. A team of as many warps as a row has units (KV heads) takes a run of tiles, each
 // warp one head of the same keys, so that the heads of a token, which lie side by side in the pool, are read at about the same
@@ -89,14 +93,14 @@ template <int BYTES> __device__ __forceinline__ void dec_copy(uint32_t dst, cons
     if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
+// 16 bytes, of which n are read and the others become zeros
+__device__ __forceinline__ void dec_copy_part(uint32_t dst, const uint8_t * src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
 // What the tensor core's tf32 (an f32 cut off behind 10 bits of its fraction) leaves of an f32, as a tf32: rounded, since
 // the cutting alone would make all scores 2^-22 too small.
 __device__ __forceinline__ uint32_t dec_rest(uint32_t x) {
     return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffffe000u)) + 0x1000u;
-}
-// the same of 16 bytes, of which n are read and the others become zeros
-__device__ __forceinline__ void dec_copy_part(uint32_t dst, const uint8_t * src, int n) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 __device__ __forceinline__ void dec_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void dec_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -145,10 +149,11 @@ template <int PAIR> __device__ __forceinline__ uint32_t dec_int8(uint32_t x) {
 // the products as two parts (22 bits); otherwise f16 or bf16 and one part (11 bits, no less than such an output can tell).
 template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     static constexpr bool IS_F32 = FMT == YUUKA_KV_F32, IS_Q8 = FMT == YUUKA_KV_Q8_0, IS_F8 = FMT == YUUKA_KV_F8;
-        // Warps of a CTA and CTAs of an SM: twelve warps, or eight where the sums, queries and copies of 256 dimensions take the
+    // Warps of a CTA and CTAs of an SM: twelve warps, or eight where the sums, queries and copies of 256 dimensions take the
     // registers (at 12 and 8 instead of 8 and 4 warps, 8 sequences of 32768 with 8 KV heads of 128 took 160 us instead of 164, 32 of
-    // 256 to 4000 with 4 of 256 took 41 instead of 44). Small CTAs are resident sooner: one short sequence took 7.4 us with 2 of
-    // four warps, 7.6 with one of eight.
+    // 256 to 4000 with 4 of 256 took 41 instead of 44; 24 of 8000 in F8 with 16 query heads to each of 4 KV heads of 256 took 110 with
+    // eight, 145 with four). Four where eight spill what a tile needs. Small CTAs are resident sooner: one short sequence took 7.4 us
+    // with 2 of four warps, 7.6 with one of eight.
     static constexpr bool NARROW = NT == 2 || (IS_F32 && HD > 64);
     static constexpr int W = 4, RESIDENT = HD == 256 ? (IS_F32 || (FMT == YUUKA_KV_F16 && NT == 2 && WIDE) ? 1 : 2) : (NARROW ? 2 : 3);
     // keys of a tile: sixteen make one row tile of the products, and two of them share the walk, the maximum and the queries' reads
@@ -180,7 +185,7 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     // queries in registers, or in shared memory where the sums leave too few (f32: 8 heads of all dimensions, split at use)
     static constexpr bool Q_SHARED = IS_F32 || HD / 4 * NT + HD / 8 * PARTS * NT > 128;
     static constexpr int Q_BYTES = !Q_SHARED ? 0 : (IS_F32 ? 8 * HD * 4 : COLS * HD * 2 * PARTS);
-    static constexpr int WARP_BYTES = (DEC_SMEM_SM / RESIDENT - 1536) / W / 16 * 16;  // (the rest: the warps' records, what a CTA takes by itself)
+    static constexpr int WARP_BYTES = (DEC_SMEM_SM / RESIDENT - 1536) / W / 16 * 16;  // (the rest: what the system keeps of a CTA's share)
     static constexpr int FIT = (WARP_BYTES - Q_BYTES) / SLOT;
     static constexpr int SLOTS = FIT > 8 ? 8 : FIT;  // K and V of a tile take one each
     static constexpr int AHEAD = SLOTS - 1;
@@ -377,8 +382,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
     const int count = team < teams && begin < total ? (int)min(share, total - begin) : 0;
 #pragma unroll 1
     for (unsigned unit = units > warps ? self : self - team * units; unit < units; unit += warps) {
-    if (count == 0) break;
-    {
+        if (count == 0) break;
         DecodeCursor<KEYS> use;
         {
             unsigned before = 0;
@@ -1148,7 +1152,6 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
             use.next(p);
         }
         dec_wait<0>();
-    }
     }
 }
 
