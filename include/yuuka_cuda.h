@@ -275,7 +275,7 @@ YUUKA_API yuuka_status yuuka_kv_read(yuuka_stream * stream, const yuuka_kv_cache
  * keys j of positions max(0, n - window) .. n - 1 (the new token's own row is the last: write it first):
  *   s_j = scale * q . k_j    out = sum_j exp(s_j) v_j / sum_j exp(s_j)    lse = ln sum_j exp(s_j)
  * and out *= 1 / (1 + exp(-gate)) with a gate (the qwen35 output gate, model/qwen35/forward.go:188-220). Without keys
- * (length 0) out is 0 and lse -infinity. Scores, statistics and sums are f32; with q of type F32 queries and
+ * (length 0), or with scores of -infinity alone, out is 0 and lse -infinity. Scores, statistics and sums are f32; with q of type F32 queries and
  * probabilities enter the products with 22 bits, with F16 or BF16 with 11. Lengths live on the device, so that a
  * captured call stays valid as sequences grow. A row whose length or sequence or one of whose blocks is out of range
  * becomes NaN. Rows and values of the cache beyond a sequence's length are never used, whatever they hold. */

@@ -316,6 +316,30 @@ def test_scale_and_tiny_values(dev, stream, scratch, fmt):
     step.free()
 
 
+@pytest.mark.parametrize("dtype,fmt", [("bf16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_scores_of_minus_infinity_weigh_nothing(dev, stream, scratch, dtype, fmt, dim):
+    """The first 40 keys of each sequence score -infinity (an infinity in an f16 pool, a product beyond f32's range): as if they
+    were not there, in whole first tiles and in whole runs of a warp; a sequence of them alone is one without keys."""
+    step = Step(dev, stream, 2, fmt, dtype, 1, 2, dim, 16, [300, 57, 41, 40, 5000])
+    q = np.abs(from_dtype(step.qg, dtype)) + 0.5
+    if fmt == "f32":  # sums of -2^132 and 2^66 * (k of the others), and a scale that brings the others back
+        q = np.full(q.shape, 2.0 ** 66)
+        step.scale = step.args.args.scale = 2.0 ** -66 / 8
+    step.qg = to_dtype(q.astype(np.float32), dtype)
+    step.qb.write(step.qg)
+    low = {"f32": np.full(step.paged.row // 4, -2.0 ** 66, np.float32).view(np.uint8), "f16": np.full(step.paged.row // 2, -np.inf, np.float16).view(np.uint8)}
+    for s in range(5):
+        step.paged.k[step.paged.slots(s, np.arange(40))] = low[fmt]
+    step.paged.upload()
+    out, lse = step.run(scratch)
+    assert np.all(out[3] == 0) and np.all(np.isneginf(lse[3]))
+    for b in (0, 1, 2, 4):  # the formula without those keys
+        step.window = int(step.lens[b]) - 40
+        step.check(out, lse, skip=set(range(5)) - {b})
+    step.free()
+
+
 def test_values_of_many_magnitudes(dev, stream, scratch, oracle):
     """Scales of V that grow and shrink along the sequence, zeros among them."""
     for fmt in ("q8_0", "f8"):

@@ -58,6 +58,7 @@ constexpr size_t DEC_PARTIAL_BYTES = 40u << 20;  // two of the 1184 warps with t
 enum { DEC_SHORT, DEC_LONG, DEC_DONE, DEC_COUNTERS };
 constexpr int DEC_SHORT_MOST = 32;      // partials that a warp joins
 constexpr float DEC_P_LOG2 = 7.0f;      // log2 of the factor that probabilities carry
+constexpr float DEC_LOWEST = -3.0e38f;  // of running maxima: finite, so that a score of -infinity weighs nothing even in a run without others
 constexpr float DEC_SLACK = 8.0f;       // log2 of what a score may pass the running maximum by before sums are rescaled
 constexpr int DEC_SMEM_SM = 233472;     // shared memory of an SM
 
@@ -669,7 +670,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 v_scale = __uint_as_float(0x00800000u);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    m[nt][0] = m[nt][1] = -INFINITY;
+                    m[nt][0] = m[nt][1] = DEC_LOWEST;
                     // (a row that is out of range has no keys and becomes NaN)
                     l[nt][0] = l[nt][1] = use.seq < 0 ? __uint_as_float(0x7fffffffu) : 0.0f;
 #pragma unroll
@@ -1212,7 +1213,7 @@ template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_TH
             float gates[DIMS];
             if (p.gate) dec_gates<WIDE, DIMS>(p, raw, gates);
 #pragma unroll
-            for (int d = 0; d < DIMS; d++) x[d] = x[d] / l * (p.gate ? gates[d] : 1.0f);
+            for (int d = 0; d < DIMS; d++) x[d] = l == 0.0f ? 0.0f : x[d] / l * (p.gate ? gates[d] : 1.0f);
             dec_write<WIDE, DIMS>(p, join.x, h.first + col, dim, x);
             if (lane == 0) dec_write_lse(p, join.x, h.first + col, m, l);
         }
@@ -1294,6 +1295,7 @@ template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_TH
                 x.z += y.z;
                 x.w += y.w;
             }
+            if (l == 0.0f) x = make_float4(0.f, 0.f, 0.f, 0.f), l = 1.0f, m = -INFINITY;  // (all scores are -infinity)
             dec_write<WIDE, 4>(p, join.x, h.first + col, dim, {x.x / l * gate[0], x.y / l * gate[1], x.z / l * gate[2], x.w / l * gate[3]});
             if (dim == 0) dec_write_lse(p, join.x, h.first + col, m, l);
         }
