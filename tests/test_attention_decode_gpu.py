@@ -164,6 +164,25 @@ def test_more_heads_than_warps(dev, stream, scratch, fmt, kv_heads, group, dim):
     step.free()
 
 
+@pytest.mark.parametrize("fmt", ["q8_0", "f8"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("kv_heads,dim", [(1, 64), (3, 64), (5, 64), (1, 128), (3, 128), (1, 256)])
+def test_rows_that_are_no_whole_lines(dev, stream, scratch, fmt, dtype, kv_heads, dim):
+    """Heads that begin anywhere in 16 bytes, differently from key to key, in a pool whose last row is in use."""
+    step = Step(dev, stream, kv_heads, fmt, dtype, kv_heads, 2, dim, 3, [60, 7, 1])
+    pages, last = step.paged, step.paged.blocks - 1
+    if last not in pages.tables:  # the first sequence's last page moves there
+        old = int(pages.tables[0, 19])
+        for pool in (pages.k, pages.v):
+            pool[3 * last:3 * last + 3] = pool[3 * old:3 * old + 3]
+            pool[3 * old:3 * old + 3] = 255
+        pages.tables[0, 19] = last
+        pages.tb.write(pages.tables)
+        pages.upload()
+    step.check(*step.run(scratch))
+    step.free()
+
+
 def test_a_batch_of_thousands(dev, stream, scratch):
     rng = np.random.default_rng(17)
     lens = rng.integers(0, 40, 300)
