@@ -8,7 +8,7 @@
 //
 // What bounds it: the bytes of the cache, read once, over F32 and F16 pools (80 to 100 % of the memory's measured 6.54 TB/s for
 // long sequences; F32 with heads of 256, whose products are three to one, 40 to 78). Over Q8_0 (40 to 55 %) and F8 (47 to 77 %) the chain of instructions from a tile's bytes to its products takes
-// longer than the bytes' way (41 % of the issue slots, with the three warps a scheduler that registers allow). The products run on mma.sync, whose operands a warp brings from shared memory into the fragments it
+// longer than the bytes' way (41 % of the issue slots, with the three or four warps a scheduler that registers allow). The products run on mma.sync, whose operands a warp brings from shared memory into the fragments it
 // needs: with one to eight query heads to a KV head the large tensor-core tiles would be empty but for a few columns, and the
 // narrow ones take 10 to 40 % of the issue rate. The dimension that a product sums over may be taken in any order and a fragment's
 // rows may stand for any dimensions, so a lane reads 16 bytes that lie side by side and takes them as its part of four
@@ -150,13 +150,14 @@ template <int PAIR> __device__ __forceinline__ uint32_t dec_int8(uint32_t x) {
 // the products as two parts (22 bits); otherwise f16 or bf16 and one part (11 bits, no less than such an output can tell).
 template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     static constexpr bool IS_F32 = FMT == YUUKA_KV_F32, IS_Q8 = FMT == YUUKA_KV_Q8_0, IS_F8 = FMT == YUUKA_KV_F8;
-    // Warps of a CTA and CTAs of an SM: twelve warps, or eight where the sums, queries and copies of 256 dimensions take the
+    // Warps of a CTA and CTAs of an SM: twelve warps an SM, or eight where the sums, queries and copies of 256 dimensions take the
     // registers (at 12 and 8 instead of 8 and 4 warps, 8 sequences of 32768 with 8 KV heads of 128 took 160 us instead of 164, 32 of
     // 256 to 4000 with 4 of 256 took 41 instead of 44; 24 of 8000 in F8 with 16 query heads to each of 4 KV heads of 256 took 110 with
-    // eight, 145 with four). Four where eight spill what a tile needs. Small CTAs are resident sooner: one short sequence took 7.4 us
-    // with 2 of four warps, 7.6 with one of eight.
+    // eight, 145 with four). Sixteen with heads of 64 and 16-bit queries (24 of 8000 with 16 KV heads of 64: Q8_0 140 instead of 152,
+    // F8 126 instead of 133, F16 125 instead of 130; with heads of 128 they spill: F8 109 instead of 90). Four where eight spill what
+    // a tile needs. Small CTAs are resident sooner: one short sequence took 7.4 us with 2 of four warps, 7.6 with one of eight.
     static constexpr bool NARROW = NT == 2 || (IS_F32 && HD > 64);
-    static constexpr int W = 4, RESIDENT = HD == 256 ? (IS_F32 || (FMT == YUUKA_KV_F16 && NT == 2 && WIDE) ? 1 : 2) : (NARROW ? 2 : 3);
+    static constexpr int W = 4, RESIDENT = HD == 256 ? (IS_F32 || (FMT == YUUKA_KV_F16 && NT == 2 && WIDE) ? 1 : 2) : (NARROW ? 2 : HD == 64 && !WIDE && !IS_F32 ? 4 : 3);
     // keys of a tile: sixteen make one row tile of the products, and two of them share the walk, the maximum and the queries' reads
     // where registers allow (64 sequences of 500 to 8000 in F8: 106 -> 99 us)
     static constexpr int HALVES = HD == 256 || (HD == 128 && (WIDE || IS_F32)) ? 1 : 2, KEYS = 16 * HALVES;
