@@ -154,10 +154,12 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     // registers (at 12 and 8 instead of 8 and 4 warps, 8 sequences of 32768 with 8 KV heads of 128 took 160 us instead of 164, 32 of
     // 256 to 4000 with 4 of 256 took 41 instead of 44; 24 of 8000 in F8 with 16 query heads to each of 4 KV heads of 256 took 110 with
     // eight, 145 with four). Sixteen with heads of 64 and 16-bit queries (24 of 8000 with 16 KV heads of 64: Q8_0 140 instead of 152,
-    // F8 126 instead of 133, F16 125 instead of 130; with heads of 128 they spill: F8 109 instead of 90). Four where eight spill what
-    // a tile needs. Small CTAs are resident sooner: one short sequence took 7.4 us with 2 of four warps, 7.6 with one of eight.
-    static constexpr bool NARROW = NT == 2 || (IS_F32 && HD > 64) || (WIDE && HD == 128);
-    static constexpr int W = 4, RESIDENT = HD == 256 ? (IS_F32 || (FMT == YUUKA_KV_F16 && NT == 2 && WIDE) ? 1 : 2) : (NARROW ? 2 : HD == 64 && !WIDE && !IS_F32 ? 4 : 3);
+    // F8 126 instead of 133, F16 125 instead of 130; with heads of 128 they spill: F8 109 instead of 90). With f32 queries F8 does
+    // better with eight there (118 instead of 133; Q8_0 181 instead of 159, F16 the same). Four where eight spill what a tile needs.
+    // Small CTAs are resident sooner: one short sequence took 7.4 us with 2 of four warps, 7.6 with one of eight.
+    static constexpr bool NARROW = NT == 2 || (IS_F32 && HD > 64) || (WIDE && (HD == 128 || (IS_F8 && HD == 64)));
+    static constexpr int W = 4, RESIDENT = HD == 256 ? (IS_F32 || (FMT == YUUKA_KV_F16 && NT == 2 && WIDE) ? 1 : 2)
+                                                     : (NARROW ? 2 : HD == 64 && !WIDE && !IS_F32 ? 4 : 3);
     // keys of a tile: sixteen make one row tile of the products, and two of them share the walk, the maximum and the queries' reads
     // where registers allow (64 sequences of 500 to 8000 in F8: 106 -> 99 us). With f32 queries and heads of 128 eight warps of two
     // beat twelve of one: 24 of 8000 with 8 KV heads 124 instead of 142 us (F16), 101 instead of 127 (F8), 142 instead of 156 (Q8_0).
