@@ -6,13 +6,15 @@
 // carry a factor of 2^7, p = 2^(s - m + 7). m is the maximum when the sums were last rescaled, which they are only when a score
 // passes it by 2^8 (in the first tiles, mostly), so the largest p is 2^15 and those down to 2^-21 of 2^m stay normal in f16.
 //
-// What bounds it: the bytes of the cache, read once, over F32 and F16 pools (72 to 100 % of the memory's measured 6.54 TB/s for
-// long sequences; F32 with heads of 256, whose products are three to one, 40 to 78). Over Q8_0 (29 to 55 %) and F8 (41 to 77 %) the chain of instructions from a tile's bytes to its products takes
-// longer than the bytes' way (41 % of the issue slots, with the three or four warps a scheduler that registers allow). The products run on mma.sync, whose operands a warp brings from shared memory into the fragments it
-// needs: with one to eight query heads to a KV head the large tensor-core tiles would be empty but for a few columns, and the
-// narrow ones take 10 to 40 % of the issue rate. The dimension that a product sums over may be taken in any order and a fragment's
-// rows may stand for any dimensions, so a lane reads 16 bytes that lie side by side and takes them as its part of four
-// products' operands; of V it reads the same dimensions of four keys, whose halves byte permutations pair up.
+// What bounds it: the bytes of the cache, read once, over F32 and F16 pools (72 to 100 % of the memory's measured 6.54 TB/s
+// for long sequences; F32 with heads of 256, whose products are three to one, 40 to 78). Over Q8_0 (29 to 55 %) and F8 (41 to
+// 77 %) the chain of instructions from a tile's bytes to its products takes longer than the bytes' way (41 % of the issue
+// slots, with the three or four warps a scheduler that registers allow). The products run on mma.sync, whose operands a warp
+// brings from shared memory into the fragments it needs: with one to eight query heads to a KV head the large tensor-core
+// tiles would be empty but for a few columns, and the narrow ones take 10 to 40 % of the issue rate. The dimension that a
+// product sums over may be taken in any order and a fragment's rows may stand for any dimensions, so a lane reads 16 bytes
+// that lie side by side and takes them as its part of four products' operands; of V it reads the same dimensions of four keys,
+// whose halves byte permutations pair up.
 //
 // A warp has a ring of tiles of its own in shared memory, K and V in turn, that cp.async fills several tiles ahead: no barrier of
 // the CTA is waited for. Copies go by lines of 128 bytes.
