@@ -96,7 +96,9 @@ YUUKA_API yuuka_status yuuka_buffer_alloc(yuuka_device * dev, uint64_t bytes, yu
 YUUKA_API void yuuka_buffer_free(yuuka_buffer * buf);
 /* A handle on device memory of another owner (another runtime's allocation, a part of a larger one), for every call
  * that takes a buffer. The memory must be a device allocation of dev, all of it, and stay valid as long as the handle
- * is used; yuuka_buffer_free then frees the handle alone. */
+ * is used; yuuka_buffer_free then frees the handle alone. A view may begin anywhere; where a call asks for a multiple of
+ * some bytes, the address of its range counts (the view's and the offset together), and a call whose kernels read f32 or
+ * int32 asks for a multiple of 4. */
 YUUKA_API yuuka_status yuuka_buffer_view(yuuka_device * dev, void * device_ptr, uint64_t bytes, yuuka_buffer ** out);
 YUUKA_API uint64_t yuuka_buffer_size(const yuuka_buffer * buf);
 YUUKA_API void * yuuka_buffer_ptr(const yuuka_buffer * buf);

@@ -603,11 +603,13 @@ extern "C" yuuka_status yuuka_accept_tree(yuuka_stream * stream, const yuuka_buf
         const uint64_t R = (uint64_t)batch * nodes, need = R * (uint64_t)vocab * sizeof(float);
         YK_REQUIRE(logits->bytes >= need, YUUKA_ERR_INVALID_ARGUMENT, "accept_tree: logits buffer holds fewer than %llu bytes",
                    (unsigned long long)need);
+        check_start("accept_tree", "logits", logits, 0, sizeof(float));
         if (mode == YUUKA_ACCEPT_REJECTION) {
             YK_REQUIRE(temperature > 0.0f && temperature == temperature, YUUKA_ERR_INVALID_ARGUMENT,
                        "accept_tree: rejection sampling needs a temperature above zero");
             YK_REQUIRE(uniforms && draft_probs && draft_probs->bytes >= need, YUUKA_ERR_INVALID_ARGUMENT,
                        "accept_tree: rejection sampling needs uniforms and a draft_probs buffer of %llu bytes", (unsigned long long)need);
+            check_start("accept_tree", "draft_probs", draft_probs, 0, sizeof(float));
             for (uint64_t i = 0; i < R * 2; i++)
                 YK_REQUIRE(uniforms[i] >= 0.0f && uniforms[i] < 1.0f, YUUKA_ERR_INVALID_ARGUMENT,
                            "accept_tree: uniform draw %llu is outside [0, 1)", (unsigned long long)i);

@@ -169,6 +169,11 @@ struct yuuka_event {
 };
 
 namespace yk {
+// What a kernel reads by words starts at a multiple of them: an offset alone does not say so, since a view may begin anywhere.
+inline void check_start(const char * op, const char * what, const yuuka_buffer * buf, uint64_t offset, uint64_t align) {
+    YK_REQUIRE(((uint64_t)(uintptr_t)buf->ptr + offset) % align == 0, YUUKA_ERR_INVALID_ARGUMENT, "%s: %s does not start at a multiple of %llu bytes",
+               op, what, (unsigned long long)align);
+}
 inline void record_completion(yuuka_stream * stream, yuuka_event * completion) {
     if (completion) YK_CUDA(cudaEventRecord(completion->e, stream->s));
 }

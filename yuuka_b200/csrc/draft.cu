@@ -92,6 +92,8 @@ extern "C" yuuka_status yuuka_spec_lookup_draft_device(yuuka_stream * stream, co
                    "lookup_draft_device: history of %d tokens exceeds the buffer", n);
         YK_REQUIRE(max_draft >= 0 && max_draft <= 64 && (uint64_t)(1 + max_draft) * 4 <= out->bytes, YUUKA_ERR_INVALID_ARGUMENT,
                    "lookup_draft_device: output buffer holds fewer than 1 + max_draft ids");
+        check_start("lookup_draft_device", "history", history, 0, sizeof(int32_t));
+        check_start("lookup_draft_device", "out", out, 0, sizeof(int32_t));
         set_device(stream->dev);
         // the history length travels in the first word of out until the kernel overwrites it with the count
         YK_CUDA(cudaMemcpyAsync(out->ptr, &n, sizeof(int32_t), cudaMemcpyHostToDevice, stream->s));

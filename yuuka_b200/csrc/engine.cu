@@ -1293,6 +1293,7 @@ void validate_batch(const yuuka_session * s, const yuuka_verify_batch * b) {
                    "verify: draft_probs must be a device buffer of at least %llu bytes", (unsigned long long)need);
         YK_REQUIRE(b->draft_probs->dev == s->model->dev, YUUKA_ERR_INVALID_ARGUMENT,
                    "verify: draft_probs lives on another device");
+        check_start("verify", "draft_probs", b->draft_probs, 0, sizeof(float));
     }
     YK_REQUIRE(s->logits, YUUKA_ERR_INVALID_ARGUMENT, "verify: the session has no logits buffer");
 }

@@ -241,6 +241,10 @@ extern "C" yuuka_status yuuka_gemm_quant(yuuka_stream * stream, yuuka_buffer * o
                    "gemm_quant: output range exceeds the buffer");
         YK_REQUIRE(x_offset % 16 == 0 && out_offset % 16 == 0, YUUKA_ERR_INVALID_ARGUMENT,
                    "gemm_quant: activation and output offsets must be multiples of 16");
+        check_start("gemm_quant", "the activations", x, x_offset, 16);
+        check_start("gemm_quant", "the output", out, out_offset, 16);
+        // (rows in GGUF order are read by the f16 or f32 words that they hold)
+        check_start("gemm_quant", "the weights", w, w_offset, flags & YUUKA_GEMM_TILED ? 16 : w_dtype == YUUKA_DTYPE_F32 ? 4 : 2);
         yuuka_device * dev = stream->dev;
         YK_REQUIRE(dev->index >= 0 && dev->index < 16, YUUKA_ERR_UNSUPPORTED, "gemm_quant: device index out of range");
         std::lock_guard<std::mutex> lock(g_scratch_mutex);
@@ -308,6 +312,7 @@ extern "C" yuuka_status yuuka_weights_tile(yuuka_stream * stream, yuuka_buffer *
                    "weights_tile: source range exceeds the buffer");
         YK_REQUIRE(dst_offset % 16 == 0 && dst_offset <= dst->bytes && tiled_bytes(dtype, n_out, n_in) <= dst->bytes - dst_offset,
                    YUUKA_ERR_INVALID_ARGUMENT, "weights_tile: destination range exceeds the buffer or is misaligned");
+        check_start("weights_tile", "the destination", dst, dst_offset, 16);
         set_device(stream->dev);
         launch_tile_weights(stream->s, (uint8_t *)dst->ptr + dst_offset, (const uint8_t *)src->ptr + src_offset, dtype,
                             (int)n_out, (int)n_in);

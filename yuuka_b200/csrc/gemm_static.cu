@@ -80,6 +80,9 @@ extern "C" yuuka_status yuuka_gemm_quant_static(yuuka_stream * stream, yuuka_buf
                    "gemm_quant_static: output range exceeds the buffer");
         YK_REQUIRE(x_offset % 16 == 0 && out_offset % 16 == 0, YUUKA_ERR_INVALID_ARGUMENT,
                    "gemm_quant_static: activation and output offsets must be multiples of 16");
+        check_start("gemm_quant_static", "the weights", w, w_offset, 16);
+        check_start("gemm_quant_static", "the activations", x, x_offset, 16);
+        check_start("gemm_quant_static", "the output", out, out_offset, 16);
         yuuka_device * dev = stream->dev;
         YK_REQUIRE(dev->index >= 0 && dev->index < 16, YUUKA_ERR_UNSUPPORTED, "gemm_quant_static: device index out of range");
 

@@ -56,8 +56,7 @@ void check_range(const char * op, const char * what, const yuuka_buffer * buf, u
     YK_REQUIRE(buf->dev->index == dev->index, YUUKA_ERR_INVALID_ARGUMENT, "%s: %s is on device %d, the stream on device %d", op, what,
                buf->dev->index, dev->index);
     YK_REQUIRE(offset <= buf->bytes && bytes <= buf->bytes - offset, YUUKA_ERR_INVALID_ARGUMENT, "%s: %s range exceeds the buffer", op, what);
-    YK_REQUIRE(((uint64_t)(uintptr_t)buf->ptr + offset) % align == 0, YUUKA_ERR_INVALID_ARGUMENT,
-               "%s: %s does not start at a multiple of %llu bytes", op, what, (unsigned long long)align);
+    check_start(op, what, buf, offset, align);
 }
 
 void check_apart(const char * op, const char * a_name, const yuuka_buffer * a, uint64_t a_offset, uint64_t a_bytes, const char * b_name,
