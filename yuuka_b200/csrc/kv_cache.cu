@@ -447,6 +447,8 @@ static yuuka_status move_rows(const char * op, bool write, yuuka_stream * stream
         const uint64_t size = rows->dtype == YUUKA_DTYPE_F32 ? 4 : 2, dim = (uint64_t)cache->kv_heads * (uint64_t)cache->head_dim;
         const uint64_t ks = rows->k_stride ? rows->k_stride : dim, vs = rows->v_stride ? rows->v_stride : dim;
         YK_REQUIRE(ks >= dim && vs >= dim, YUUKA_ERR_INVALID_ARGUMENT, "%s: row stride below %llu elements", op, (unsigned long long)dim);
+        // (beyond it strides in bytes would leave 64 bits)
+        YK_REQUIRE(ks <= 1ull << 48 && vs <= 1ull << 48, YUUKA_ERR_INVALID_ARGUMENT, "%s: row stride range exceeds 2^48 elements", op);
         YK_REQUIRE(ks * size % 16 == 0 && vs * size % 16 == 0, YUUKA_ERR_INVALID_ARGUMENT, "%s: row strides must be multiples of 16 bytes", op);
         const uint64_t kb = span_bytes(rows->rows, ks, 1, 0, dim, size), vb = span_bytes(rows->rows, vs, 1, 0, dim, size);
         check_range(op, "k", rows->k, rows->k_offset, kb, 16, dev);
