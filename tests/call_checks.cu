@@ -4,6 +4,43 @@
 #include "cache_checks.cu"
 #undef main
 
+// Every join that a call's second kernel takes for its own lies in the partial sums, whatever another call has left in the list.
+template <int FMT, int HD, int NT, bool WIDE> static void joins_stay_inside() {
+    using namespace yk;
+    using S = DecodeShape<FMT, HD, NT, WIDE>;
+    DecodeParams p{};
+    p.batch = 8;
+    p.head_tiles = 1;
+    p.warps = 148 * S::RESIDENT * S::W;
+    for (int units : {1, 2, 3, 16, 40, 592, 1024}) {
+        p.cache.kv_heads = units;
+        bool inside = true, taken = units * 2 > p.warps;
+        for (int last = 1; last < 2 * DEC_WARPS; last++) {
+            if (!decode_join_sound(p, make_int4(7, units - 1, last - 1, last))) continue;
+            taken = true;
+            inside &= (((size_t)last * units + units - 1) * 2 + 1) * S::PART_FLOATS * sizeof(float) <= DEC_PARTIAL_BYTES;  // the heads' slot
+            inside &= (((size_t)(last - 1) * units + units - 1) * 2 + 2) * S::PART_FLOATS * sizeof(float) <= DEC_PARTIAL_BYTES;
+        }
+        const int teams = p.warps / units;
+        char name[96];
+        snprintf(name, sizeof name, "joins of format %d, heads of %d, %d columns, %d units", FMT, HD, S::COLS, units);
+        expect(inside && taken && !decode_join_sound(p, make_int4(7, units - 1, 0, teams)) && !decode_join_sound(p, make_int4(7, units, 0, 1)) &&
+                   !decode_join_sound(p, make_int4(8, 0, 0, 1)) && !decode_join_sound(p, make_int4(0, 0, -1, 1)) && !decode_join_sound(p, make_int4(0, 0, 1, 1)) &&
+                   (teams < 2 || decode_join_sound(p, make_int4(0, 0, 0, teams - 1))),
+               name);
+    }
+}
+template <int FMT, bool WIDE> static void joins_of_format() {
+    joins_stay_inside<FMT, 64, 1, WIDE>();
+    joins_stay_inside<FMT, 128, 1, WIDE>();
+    joins_stay_inside<FMT, 256, 1, WIDE>();
+    if constexpr (FMT != YUUKA_KV_F32) {
+        joins_stay_inside<FMT, 64, 2, WIDE>();
+        joins_stay_inside<FMT, 128, 2, WIDE>();
+        joins_stay_inside<FMT, 256, 2, WIDE>();
+    }
+}
+
 int main() {
     using namespace yk;
     constexpr int WRITE = 1, READ = 2, MOVE = 3, ATTEND = 4;
@@ -22,6 +59,15 @@ int main() {
         w.rows.v_stride = ~0ull - 127;
         return MOVE;
     });
+
+    joins_of_format<YUUKA_KV_F32, true>();
+    joins_of_format<YUUKA_KV_F32, false>();
+    joins_of_format<YUUKA_KV_F16, true>();
+    joins_of_format<YUUKA_KV_F16, false>();
+    joins_of_format<YUUKA_KV_Q8_0, true>();
+    joins_of_format<YUUKA_KV_Q8_0, false>();
+    joins_of_format<YUUKA_KV_F8, true>();
+    joins_of_format<YUUKA_KV_F8, false>();
 
     expect(launches == 0, "nothing was launched");
     printf(failures ? "%d checks failed\n" : "all checks passed\n", failures);

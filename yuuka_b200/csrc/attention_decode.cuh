@@ -50,6 +50,7 @@ struct DecodeParams {
     int batch, heads, group, head_tiles, tile_heads;  // group: query heads per KV head; tiles of them, heads per tile
     int window, dtype;
     float scale_log2;  // softmax scale times log2 e
+    int warps;         // of the grid
     float * partial;   // [teams][units][2][part floats]: what a run leaves of its first row (0) and of its last one (1)
     int4 * joins;      // [2][DEC_WARPS] units that several teams share, few and many: x row, y unit of the row, z first and w last team
     int * counters;    // zero between calls: joins of both lists, CTAs of the joining kernel done
@@ -360,6 +361,13 @@ __device__ __forceinline__ DecodeHeads decode_heads(const DecodeParams & p, int 
     h.first = h.kv_head * p.group + ht * p.tile_heads;
     h.count = min(p.tile_heads, p.group - ht * p.tile_heads);
     return h;
+}
+
+// Whether a join is one that this call's teams can have left. (Calls that share scratch memory against the rule may read one
+// another's joins: wrong results, but no memory beyond the partial sums that this call's own warps have.)
+__host__ __device__ __forceinline__ bool decode_join_sound(const DecodeParams & p, const int4 & j) {
+    const int units = p.cache.kv_heads * p.head_tiles;
+    return (unsigned)j.x < (unsigned)p.batch && (unsigned)j.y < (unsigned)units && j.z >= 0 && j.z < j.w && j.w < p.warps / units;
 }
 
 // ---- the kernel ----------------------------------------------------------------------------------------------------
@@ -1173,14 +1181,10 @@ template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_TH
     pdl_entry();
     const int tid = threadIdx.x, units = p.cache.kv_heads * p.head_tiles, group = tid / JOIN_LANES;
     const int few = min(p.counters[DEC_SHORT], DEC_WARPS), jobs = min(p.counters[DEC_LONG], DEC_WARPS) * COLS * SLICES;
-    // (calls that share scratch memory against the rule may read one another's joins: wrong results, but no other memory)
-    auto sound = [&](const int4 & j) {
-        return (unsigned)j.x < (unsigned)p.batch && (unsigned)j.y < (unsigned)units && j.z >= 0 && j.z < j.w && j.w < DEC_WARPS / units;
-    };
 #pragma unroll 1
     for (int job = blockIdx.x; job < few; job += gridDim.x) {
         const int4 join = p.joins[job];
-        if (!sound(join)) continue;
+        if (!decode_join_sound(p, join)) continue;
         const DecodeHeads h = decode_heads(p, join.y);
         const int n = join.w - join.z + 1, lane = tid & 31, dim = lane * DIMS;
         const float * first = p.partial + ((size_t)join.z * units + join.y) * 2 * PART;
@@ -1227,7 +1231,7 @@ template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_TH
 #pragma unroll 1
     for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
         const int4 join = p.joins[DEC_WARPS + job / (COLS * SLICES)];
-        if (!sound(join)) continue;
+        if (!decode_join_sound(p, join)) continue;
         const int col = job / SLICES % COLS, dim = 4 * (job % SLICES * JOIN_LANES + tid % JOIN_LANES);
         const DecodeHeads h = decode_heads(p, join.y);
         if (col >= h.count) continue;
@@ -1325,6 +1329,7 @@ template <int FMT, int HD, int NT, bool WIDE> void launch_decode_as(cudaStream_t
                "attention_decode: %d multiprocessors", sms);
     auto kern = attention_decode_kernel<FMT, HD, NT, WIDE>;
     YK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::LAYOUT_BYTES));
+    p.warps = ctas * S::W;
     launch_k(kern, (unsigned)ctas, S::W * 32, S::LAYOUT_BYTES, s, p);
     launch_k(attention_decode_join_kernel<HD, S::COLS, WIDE>, (unsigned)(sms * JOIN_CTAS_SM), JOIN_THREADS, 0, s, p);
 }
