@@ -295,7 +295,7 @@ typedef struct yuuka_attention_decode_args {
     uint32_t dtype;        /* of q, gate and out: F32, F16 or BF16 */
     int32_t batch, heads;  /* heads a multiple of kv_heads */
     int32_t window;        /* 0: none */
-    float scale;           /* 0: 1 / sqrt(head_dim) */
+    float scale;           /* 0: 1 / sqrt(head_dim); at most 2.3e38 in magnitude */
 } yuuka_attention_decode_args;
 /* Device memory for the joining of split sequences: one for all shapes, 41 MB. Calls that use the same one are
  * ordered (one stream, or events between them); graphs that may run at the same time are captured with one each. */

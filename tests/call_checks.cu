@@ -60,6 +60,10 @@ int main() {
         return MOVE;
     });
 
+    // a scale whose product with log2 e is no f32: all scores would be infinite or NaN
+    for (float scale : {2.4e38f, -3.4e38f, NAN})
+        refuses("scale beyond its base-2 form", INVALID, "finite", [=](World & w) { w.args.scale = scale; return ATTEND; });
+
     joins_of_format<YUUKA_KV_F32, true>();
     joins_of_format<YUUKA_KV_F32, false>();
     joins_of_format<YUUKA_KV_F16, true>();

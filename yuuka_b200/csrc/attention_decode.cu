@@ -79,7 +79,10 @@ extern "C" yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_atte
         YK_REQUIRE(a->seq_ids || a->batch <= cache->sequences, YUUKA_ERR_INVALID_ARGUMENT, "%s: batch %d without sequence ids exceeds %d sequences", op,
                    a->batch, cache->sequences);
         YK_REQUIRE(a->window >= 0, YUUKA_ERR_INVALID_ARGUMENT, "%s: window %d", op, a->window);
-        YK_REQUIRE(std::isfinite(a->scale), YUUKA_ERR_INVALID_ARGUMENT, "%s: scale is not finite", op);
+        // (the kernel's factor, in base 2, is f32 as well)
+        const double scale = a->scale != 0.0f ? (double)a->scale : 1.0 / std::sqrt((double)cache->head_dim);
+        const float scale_log2 = (float)(scale * 1.4426950408889634);
+        YK_REQUIRE(std::isfinite(scale_log2), YUUKA_ERR_INVALID_ARGUMENT, "%s: scale is not finite in f32 times log2 e", op);
         const uint64_t size = a->dtype == YUUKA_DTYPE_F32 ? 4 : 2, hd = (uint64_t)cache->head_dim, heads = (uint64_t)a->heads,
                        batch = (uint64_t)a->batch;
         const uint64_t qh = a->q_head_stride ? a->q_head_stride : hd, oh = a->out_head_stride ? a->out_head_stride : hd;
@@ -138,8 +141,7 @@ extern "C" yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_atte
         const int cols = p.tile_heads <= 8 ? 8 : 16;
         p.window = a->window;
         p.dtype = (int)a->dtype;
-        const double scale = a->scale != 0.0f ? (double)a->scale : 1.0 / std::sqrt((double)cache->head_dim);
-        p.scale_log2 = (float)(scale * 1.4426950408889634);
+        p.scale_log2 = scale_log2;
         p.counters = (int *)scratch->memory;
         p.joins = (int4 *)(scratch->memory + DEC_COUNTER_BYTES);
         p.partial = (float *)(scratch->memory + DEC_COUNTER_BYTES + 2 * DEC_WARPS * sizeof(int4));
