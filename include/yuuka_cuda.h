@@ -303,7 +303,7 @@ typedef struct yuuka_attention_scratch yuuka_attention_scratch;
 YUUKA_API yuuka_status yuuka_attention_scratch_create(yuuka_device * dev, yuuka_attention_scratch ** out);
 YUUKA_API void yuuka_attention_scratch_destroy(yuuka_attention_scratch * scratch);
 /* Asynchronous on stream. q, gate and out start at multiples of 16 bytes from row to row and head to head. out and lse lie
- * over no other operand. */
+ * over no other operand. batch rows of table_stride * block_size keys hold fewer than 2e9 tiles of 16. */
 YUUKA_API yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_attention_scratch * scratch,
                                               const yuuka_kv_cache * cache, const yuuka_attention_decode_args * args,
                                               yuuka_event * completion);

@@ -45,7 +45,8 @@ int main() {
     using namespace yk;
     constexpr int WRITE = 1, READ = 2, MOVE = 3, ATTEND = 4;
     const yuuka_status INVALID = YUUKA_ERR_INVALID_ARGUMENT;
-    (void)WRITE, (void)READ, (void)ATTEND;
+    (void)WRITE, (void)READ;
+    int devices = 0;
 
     // A single row has no second one for a stride to reach: its byte stride may wrap to zero all the same
     for (int power : {49, 61, 62, 63})
@@ -63,6 +64,30 @@ int main() {
     // a scale whose product with log2 e is no f32: all scores would be infinite or NaN
     for (float scale : {2.4e38f, -3.4e38f, NAN})
         refuses("scale beyond its base-2 form", INVALID, "finite", [=](World & w) { w.args.scale = scale; return ATTEND; });
+
+    // 1.5e9 tiles of 65536 rows, whatever the number of heads (nothing but the device is missing; nothing is launched with one)
+    if (cudaGetDeviceCount(&devices) != cudaSuccess || devices == 0)
+        refuses("tables of many keys and heads", YUUKA_ERR_DEVICE, "cudaSetDevice", [](World & w) {
+            auto apart = [&](int i) {
+                yuuka_buffer * b = w.buffer(0, 0);
+                b->ptr = (void *)(uintptr_t)((1ull << 50) + ((uint64_t)i << 42));
+                b->bytes = 1ull << 41;
+                return b;
+            };
+            w.cache.block_size = 122880;
+            w.cache.pool_blocks = 1;
+            w.cache.k = apart(0);
+            w.cache.v = apart(1);
+            w.args.heads = 64;
+            w.args.batch = 65536;
+            w.args.q = apart(2);
+            w.args.out = apart(3);
+            w.args.gate = apart(4);
+            w.args.lse = apart(5);
+            w.args.lens = apart(6);
+            w.args.seq_ids = apart(7);
+            return ATTEND;
+        });
 
     joins_of_format<YUUKA_KV_F32, true>();
     joins_of_format<YUUKA_KV_F32, false>();

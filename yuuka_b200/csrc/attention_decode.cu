@@ -145,8 +145,8 @@ extern "C" yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_atte
         p.counters = (int *)scratch->memory;
         p.joins = (int4 *)(scratch->memory + DEC_COUNTER_BYTES);
         p.partial = (float *)(scratch->memory + DEC_COUNTER_BYTES + 2 * DEC_WARPS * sizeof(int4));
-        // tiles are counted in 31 bits
-        const double tiles = (double)a->batch * cache->kv_heads * p.head_tiles * (p.cache.capacity / 16 + 1.0);
+        // a team's tiles, those of all rows at most, are counted in 31 bits
+        const double tiles = (double)a->batch * (p.cache.capacity / 16 + 1.0);
         YK_REQUIRE(tiles < 2e9, YUUKA_ERR_UNSUPPORTED, "%s: %g tiles of keys are too many for one call", op, tiles);
         set_device(dev);
         switch (cache->format) {
