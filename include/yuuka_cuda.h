@@ -277,10 +277,14 @@ YUUKA_API yuuka_status yuuka_kv_read(yuuka_stream * stream, const yuuka_kv_cache
  * keys j of positions max(0, n - window) .. n - 1 (the new token's own row is the last: write it first):
  *   s_j = scale * q . k_j    out = sum_j exp(s_j) v_j / sum_j exp(s_j)    lse = ln sum_j exp(s_j)
  * and out *= 1 / (1 + exp(-gate)) with a gate (the qwen35 output gate, model/qwen35/forward.go:188-220). Without keys
- * (length 0), or with scores of -infinity alone, out is 0 and lse -infinity. Scores, statistics and sums are f32; with q of type F32 queries and
- * probabilities enter the products with 22 bits, with F16 or BF16 with 11. Lengths live on the device, so that a
- * captured call stays valid as sequences grow. A row whose length or sequence or one of whose blocks is out of range
- * becomes NaN. Rows and values of the cache beyond a sequence's length are never used, whatever they hold. */
+ * (length 0), or with scores of -infinity alone, out is 0 and lse -infinity. Scores, statistics and sums are f32; with q of
+ * type F32 queries and probabilities enter the products with 22 bits, with F16 or BF16 with 11, and what a key adds is
+ * rounded to 2^-35 of the row's largest value besides (over F32 pools it is not). Rows over Q8_0 and F8 whose scales of V lie
+ * further apart than 2^10 (q of type F32) or 2^14 are summed in f32, which takes about ten times as long. An infinity or a
+ * NaN among the values makes the dimensions that it belongs to infinite or NaN (of Q8_0 those of its block, of F8 of its
+ * head), and no others. Lengths live on the device, so that a captured call stays valid as sequences grow. A row whose
+ * length or sequence or one of whose blocks is out of range becomes NaN. Rows and values of the cache beyond a sequence's
+ * length are never used, whatever they hold. */
 typedef struct yuuka_attention_decode_args {
     const yuuka_buffer * q; /* [batch][heads][head_dim] */
     yuuka_buffer * out;     /* the same shape and type */
@@ -297,7 +301,7 @@ typedef struct yuuka_attention_decode_args {
     int32_t window;        /* 0: none */
     float scale;           /* 0: 1 / sqrt(head_dim); at most 2.3e38 in magnitude */
 } yuuka_attention_decode_args;
-/* Device memory for the joining of split sequences: one for all shapes, 41 MB. Calls that use the same one are
+/* Device memory for the joining of split sequences: one for all shapes, 42 MB. Calls that use the same one are
  * ordered (one stream, or events between them); graphs that may run at the same time are captured with one each. */
 typedef struct yuuka_attention_scratch yuuka_attention_scratch;
 YUUKA_API yuuka_status yuuka_attention_scratch_create(yuuka_device * dev, yuuka_attention_scratch ** out);

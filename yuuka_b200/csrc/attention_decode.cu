@@ -12,7 +12,9 @@ struct yuuka_attention_scratch {
 
 namespace yk {
 
-constexpr size_t DEC_COUNTER_BYTES = (DEC_COUNTERS * sizeof(int) + 255) / 256 * 256;
+// the scratch memory: counters, joins of both lists, runs to be done again, partials
+constexpr size_t DEC_JOINS_AT = (DEC_COUNTERS * sizeof(int) + 255) / 256 * 256, DEC_FAR_AT = DEC_JOINS_AT + 2 * DEC_WARPS * sizeof(int4),
+                 DEC_PARTIAL_AT = DEC_FAR_AT + DEC_FAR_MOST * sizeof(int2);
 
 // rows and heads of an output: either all heads of a row behind one another or all rows of a head
 static bool strides_disjoint(uint64_t rows, uint64_t row, uint64_t heads, uint64_t head, uint64_t dim) {
@@ -30,14 +32,14 @@ extern "C" yuuka_status yuuka_attention_scratch_create(yuuka_device * dev, yuuka
         YK_REQUIRE(dev, YUUKA_ERR_INVALID_ARGUMENT, "attention_scratch_create: null argument");
         set_device(dev);
         void * ptr = nullptr;
-        const size_t bytes = DEC_COUNTER_BYTES + 2 * DEC_WARPS * sizeof(int4) + DEC_PARTIAL_BYTES;
+        const size_t bytes = DEC_PARTIAL_AT + DEC_PARTIAL_BYTES;
         const cudaError_t err = cudaMalloc(&ptr, bytes);
         if (err != cudaSuccess) {
             cudaGetLastError();
             YK_REQUIRE(false, YUUKA_ERR_ALLOCATION, "cudaMalloc(%llu) failed: %s", (unsigned long long)bytes, cudaGetErrorString(err));
         }
         auto * s = new (std::nothrow) yuuka_attention_scratch();
-        const cudaError_t zeroed = s ? cudaMemset(ptr, 0, DEC_COUNTER_BYTES) : cudaSuccess;
+        const cudaError_t zeroed = s ? cudaMemset(ptr, 0, DEC_JOINS_AT) : cudaSuccess;
         const cudaError_t waited = s && zeroed == cudaSuccess ? cudaDeviceSynchronize() : zeroed;
         if (!s || waited != cudaSuccess) {
             cudaFree(ptr);
@@ -143,8 +145,9 @@ extern "C" yuuka_status yuuka_attention_decode(yuuka_stream * stream, yuuka_atte
         p.dtype = (int)a->dtype;
         p.scale_log2 = scale_log2;
         p.counters = (int *)scratch->memory;
-        p.joins = (int4 *)(scratch->memory + DEC_COUNTER_BYTES);
-        p.partial = (float *)(scratch->memory + DEC_COUNTER_BYTES + 2 * DEC_WARPS * sizeof(int4));
+        p.joins = (int4 *)(scratch->memory + DEC_JOINS_AT);
+        p.far = (int2 *)(scratch->memory + DEC_FAR_AT);
+        p.partial = (float *)(scratch->memory + DEC_PARTIAL_AT);
         // a team's tiles, those of all rows at most, are counted in 31 bits
         const double tiles = (double)a->batch * (p.cache.capacity / 16 + 1.0);
         YK_REQUIRE(tiles < 2e9, YUUKA_ERR_UNSUPPORTED, "%s: %g tiles of keys are too many for one call", op, tiles);

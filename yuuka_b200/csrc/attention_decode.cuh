@@ -3,8 +3,9 @@
 // Mathematics. A unit is one KV head of one row of the batch, with up to 8 NT of the query heads that share it as columns.
 // Its keys are taken 16 or 32 at a time: S^T = K Q^T (keys as the rows of the product, heads as its 8-wide columns), running
 // maximum m and sum l per head, O^T += V^T P^T. Scores live in the base-2 domain, s = (scale log2 e) q.k, and probabilities
-// carry a factor of 2^7, p = 2^(s - m + 7). m is the maximum when the sums were last rescaled, which they are only when a score
-// passes it by 2^8 (in the first tiles, mostly), so the largest p is 2^15 and those down to 2^-21 of 2^m stay normal in f16.
+// carry a factor of 2^11, p = 2^(s - m + 11). m is the maximum when the sums were last rescaled, which they are only when a score
+// passes it by 2^4 (in the first tiles, mostly), so the largest p is 2^15, those down to 2^-25 of 2^m stay normal in f16, and
+// what is rounded away is below 2^-36 of it. (A slack of 2^8 with a factor of 2^7 took as long.)
 //
 // What bounds it: the bytes of the cache, read once, over F32 and F16 pools (72 to 100 % of the memory's measured 6.54 TB/s
 // for long sequences; F32 with heads of 256, whose products are three to one, 40 to 78). Over Q8_0 (29 to 55 %) and F8 (41 to
@@ -51,18 +52,20 @@ struct DecodeParams {
     int window, dtype;
     float scale_log2;  // softmax scale times log2 e
     int warps;         // of the grid
-    float * partial;   // [teams][units][2][part floats]: what a run leaves of its first row (0) and of its last one (1)
+    float * partial;   // [teams][units][2][part floats]: what a run leaves of its first row (0) and of its last one (1); sums l with a sign: to be done again
     int4 * joins;      // [2][DEC_WARPS] units that several teams share, few and many: x row, y unit of the row, z first and w last team
-    int * counters;    // zero between calls: joins of both lists, CTAs of the joining kernel done
+    int2 * far;        // [DEC_FAR_MOST] runs that have whole rows to be done again: x unit, y team
+    int * counters;    // zero between calls: joins of both lists, runs in far, CTAs of the joining kernel done
 };
 
 constexpr int DEC_WARPS = 4096;         // of a grid, at most
 constexpr size_t DEC_PARTIAL_BYTES = 40u << 20;  // two of the 1184 warps with the largest sums (16 columns of 256) take 39
-enum { DEC_SHORT, DEC_LONG, DEC_DONE, DEC_COUNTERS };
+enum { DEC_SHORT, DEC_LONG, DEC_FAR, DEC_DONE, DEC_COUNTERS };
 constexpr int DEC_SHORT_MOST = 32;      // partials that a warp joins
-constexpr float DEC_P_LOG2 = 7.0f;      // log2 of the factor that probabilities carry
+constexpr int DEC_FAR_MOST = 16384;     // runs to do again: of each warp one, or of each unit where those are more (65536 / 8 + 1024 at most)
+constexpr float DEC_P_LOG2 = 11.0f;      // log2 of the factor that probabilities carry
 constexpr float DEC_LOWEST = -3.0e38f;  // of running maxima: finite, so that a score of -infinity weighs nothing even in a run without others
-constexpr float DEC_SLACK = 8.0f;       // log2 of what a score may pass the running maximum by before sums are rescaled
+constexpr float DEC_SLACK = 4.0f;       // log2 of what a score may pass the running maximum by before sums are rescaled
 constexpr int DEC_SMEM_SM = 233472;     // shared memory of an SM
 
 // ---- small helpers -------------------------------------------------------------------------------------------------
@@ -168,6 +171,10 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     // beat twelve of one: 24 of 8000 with 8 KV heads 124 instead of 142 us (F16), 101 instead of 127 (F8), 142 instead of 156 (Q8_0).
     static constexpr int HALVES = HD == 256 || (HD == 128 && (IS_F32 || (WIDE && NT == 2))) ? 1 : 2, KEYS = 16 * HALVES;
     static constexpr int COLS = 8 * NT, PARTS = WIDE ? 2 : 1;
+    // Q8_0, F8: ratio (log2) of the scales of V from which on a row is done again, in f32. Probabilities of 2^11 for the heaviest key enter
+    // the products in units of the largest scale, rounded to half of f16's 2^-24: at this ratio a key of the smallest scale that has all
+    // the weight is held to 2^-36 * 2 * 2^10 = 2^-25 (f32 queries), or 2^-21, of itself.
+    static constexpr int FAR_LOG2 = WIDE ? 10 : 14;
     // Q8_0: a head's blocks of 34 bytes, copied as the 16-byte pieces that hold them, which begin up to 12 bytes before. (Copied by
     // words, 24 sequences of 8000 with 16 KV heads of 64 took 176 us.) A piece more or less from key to key would put the lanes'
     // reads of V on the same banks.
@@ -263,6 +270,34 @@ template <int KEYS> struct DecodeCursor {
         end = s.end;
         tiles = s.tiles;
         seq = s.seq;
+    }
+    // the whole warp: tile `begin` of the sequence (less than its length: some row holds it)
+    __device__ __forceinline__ void seek(const DecodeParams & p, unsigned begin) {
+        const int lane = threadIdx.x & 31;
+        unsigned before = 0;
+        b = 0;
+        for (int base = 0; base < p.batch; base += 32) {
+            const int at = base + lane;
+            const unsigned mine = at < p.batch ? (unsigned)decode_span(p, at, KEYS).tiles : 0;
+            unsigned sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, before + sum > begin);
+            if (hit) {
+                const int first_hit = __ffs(hit) - 1;
+                b = base + first_hit;
+                before += __shfl_sync(0xffffffffu, sum - mine, first_hit);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        row(p);
+        const int tile = min((int)(begin - before), tiles - 1);  // (it is less, unless lengths change under the call)
+        pos = first + tile * KEYS;
+        left = tiles - tile;
     }
     __device__ __forceinline__ void next(const DecodeParams & p) {
         pos += KEYS;
@@ -399,32 +434,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
     for (unsigned unit = units > warps ? self : self - team * units; unit < units; unit += warps) {
         if (count == 0) break;
         DecodeCursor<KEYS> use;
-        {
-            unsigned before = 0;
-            use.b = 0;
-            for (int base = 0; base < p.batch; base += 32) {  // (begin < total: some row holds it)
-                const int b = base + lane;
-                const unsigned mine = b < p.batch ? (unsigned)decode_span(p, b, KEYS).tiles : 0;
-                unsigned sum = mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned v = __shfl_up_sync(0xffffffffu, sum, o);
-                    if (lane >= o) sum += v;
-                }
-                const unsigned hit = __ballot_sync(0xffffffffu, before + sum > begin);
-                if (hit) {
-                    const int at = __ffs(hit) - 1;
-                    use.b = base + at;
-                    before += __shfl_sync(0xffffffffu, sum - mine, at);
-                    break;
-                }
-                before += __shfl_sync(0xffffffffu, sum, 31);
-            }
-            use.row(p);
-            const int tile = min((int)(begin - before), use.tiles - 1);  // (it is less, unless lengths change under the call)
-            use.pos = use.first + tile * KEYS;
-            use.left = use.tiles - tile;
-        }
+        use.seek(p, begin);
 
         // -- copies. Keys behind the last one of a unit's last tile repeat it (their probabilities become zero), so a copy is
         // always whole; a tile of a bad block becomes NaN, and a unit without keys copies nothing.
@@ -534,6 +544,8 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
         float m[NT][2], l[NT][2];    // l: of this lane's keys
         float o[NT][CHUNKS][DPL / 2][4];
         float v_scale = 1.0f;        // Q8_0, F8: o is in units of it (a power of two)
+        [[maybe_unused]] bool again = false;      // the run has whole rows for the second kernel to do again
+        [[maybe_unused]] uint32_t v_least = ~0u;  // smallest scale of V but zero that the lane has seen: bits of its magnitude less one (Q8_0: f16)
         bool from_start = false, fresh = true;
 
         auto load_queries = [&] {
@@ -686,6 +698,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 from_start = use.left == use.tiles;
                 load_queries();
                 v_scale = __uint_as_float(0x00800000u);
+                v_least = ~0u;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     m[nt][0] = m[nt][1] = DEC_LOWEST;
@@ -919,10 +932,9 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 #pragma unroll
                     for (int h = 0; h < HALVES; h++) fragments(h, 1.0f, 1.0f);
                 } else if constexpr (S::IS_F8) {
-                    uint32_t largest = 0;
-#pragma unroll
-                    for (int h = 0; h < HALVES; h++) largest = max(largest, max(__float_as_uint(fabsf(vd[h][0])), __float_as_uint(fabsf(vd[h][1]))));
-                    const float inv = take_v_scale(largest);
+                    const uint32_t bits = dec_lds(ks + S::K16 * HALVES + 4 * KEYS + 4 * (lane & (KEYS - 1))) & 0x7fffffffu;  // a lane to a key, or two
+                    v_least = min(v_least, bits - 1);
+                    const float inv = take_v_scale(bits);
 #pragma unroll
                     for (int h = 0; h < HALVES; h++) fragments(h, vd[h][0] * inv, vd[h][1] * inv);
                 }
@@ -994,7 +1006,6 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         }
                     // scales of V: of keys g and g + 8, block by block, into the probabilities
                     float d[HALVES][2][HD / 32];
-                    uint32_t largest = 0;
 #pragma unroll
                     for (int h = 0; h < HALVES; h++)
 #pragma unroll
@@ -1002,12 +1013,22 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                             const int key = 16 * h + g + 8 * k;
                             const uint32_t at = vs + key * S::Q8_ROW + (S::Q8_STARTS ? dec_lds(starts + 4 * key) : 0);
 #pragma unroll
-                            for (int blk = 0; blk < HD / 32; blk++) {
-                                d[h][k][blk] = __half2float(__ushort_as_half((unsigned short)dec_lds_u16(at + 34 * blk)));
-                                largest = max(largest, __float_as_uint(fabsf(d[h][k][blk])));
-                            }
+                            for (int blk = 0; blk < HD / 32; blk++) d[h][k][blk] = __half2float(__ushort_as_half((unsigned short)dec_lds_u16(at + 34 * blk)));
                         }
-                    const float inv = take_v_scale(largest);
+                    // the largest and the smallest: a lane to a key, or to half of one's blocks
+                    uint32_t largest = 0;
+                    {
+                        constexpr int EACH = HD / 32 * KEYS / 32;
+                        const int key = lane & (KEYS - 1);
+                        const uint32_t at = vs + key * S::Q8_ROW + 34 * EACH * (lane / KEYS) + (S::Q8_STARTS ? dec_lds(starts + 4 * key) : 0);
+#pragma unroll
+                        for (int i = 0; i < EACH; i++) {
+                            const uint32_t bits = dec_lds_u16(at + 34 * i) & 0x7fffu;
+                            largest = max(largest, bits);
+                            v_least = min(v_least, bits - 1);
+                        }
+                    }
+                    const float inv = take_v_scale(__float_as_uint(__half2float(__ushort_as_half((unsigned short)largest))));
 #pragma unroll
                     for (int c = 0; c < CHUNKS; c++) {
                         uint32_t a[2][HALVES][4];
@@ -1112,6 +1133,11 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                         l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 16);
                     }
                 if constexpr (!S::IS_Q8 && !S::IS_F8) v_scale = 1.0f;
+                [[maybe_unused]] bool far = false;  // the second kernel does it again
+                if constexpr (S::IS_Q8 || S::IS_F8) {  // (for a scale that is not finite as well: it shall make the dimensions that it scales NaN, and no others)
+                    const float least = S::IS_F8 ? __uint_as_float(v_least + 1) : __half2float(__ushort_as_half((unsigned short)(v_least + 1)));
+                    far = __any_sync(0xffffffffu, (v_least != ~0u && least * (float)(1 << S::FAR_LOG2) < v_scale) || !(v_scale < 1.7e38f));
+                }
                 const DecodeHeads h = decode_heads(p, unit);
                 if (ends && from_start) {
 #pragma unroll
@@ -1146,6 +1172,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                             }
                             if (g == 0) dec_write_lse(p, use.b, h.first + col, m[nt][e], l[nt][e]);
                         }
+                    again |= far;
                 } else {
                     // what other teams share: a row begun earlier (head), or one begun here that goes on (tail)
                     float * const part = p.partial + (((size_t)team * units + unit) * 2 + from_start) * S::PART_FLOATS;
@@ -1163,7 +1190,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                                         make_float2(o[nt][c][j][e] * v_scale, o[nt][c][j][e + 2] * v_scale);
                             if (g == 0) {
                                 part[COLS * HD + col] = m[nt][e];
-                                part[COLS * HD + COLS + col] = l[nt][e];
+                                part[COLS * HD + COLS + col] = far ? __uint_as_float(__float_as_uint(l[nt][e]) | 0x80000000u) : l[nt][e];
                             }
                         }
                     if (from_start && lane == 0) {
@@ -1178,6 +1205,249 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
             use.next(p);
         }
         dec_wait<0>();
+        if constexpr (S::IS_Q8 || S::IS_F8)
+            if (again && lane == 0) {
+                const int at = atomicAdd(p.counters + DEC_FAR, 1);
+                if (at < DEC_FAR_MOST) p.far[at] = make_int2((int)unit, (int)team);
+            }
+    }
+}
+
+// Q8_0 and F8 once more, in f32 throughout: rows whose scales of V lie far apart, for which f16 probabilities in units of the largest
+// scale have too few bits. A key that weighs nothing may have the largest scale, so the unit would have to follow the weighted scales, by
+// head and block of dimensions: with such maxima, or with these sums inside the kernel's own loop, ordinary data took 2 to 12 % longer.
+//
+// A row of K or V: the lane's HD / 32 neighbouring dimensions of a head.
+template <int FMT, int HD> __device__ __forceinline__ void decode_row(const uint8_t * row, const PagedCache & c, int kv_head, float (&x)[HD / 32]) {
+    constexpr int DIMS = HD / 32;
+    const int dim = (threadIdx.x & 31) * DIMS;
+    if constexpr (FMT == YUUKA_KV_Q8_0) {
+        const uint8_t * block = row + (kv_head * (HD / 32) + dim / 32) * 34;
+        const float scale = __half2float(__ushort_as_half(__ldg(reinterpret_cast<const unsigned short *>(block))));
+#pragma unroll
+        for (int i = 0; i < DIMS; i += 2) {
+            const unsigned pair = __ldg(reinterpret_cast<const unsigned short *>(block + 2 + dim % 32 + i));
+            x[i] = scale * (float)(int8_t)pair;
+            x[i + 1] = scale * (float)(int8_t)(pair >> 8);
+        }
+    } else {
+        const float scale = __ldg(reinterpret_cast<const float *>(row + c.kv_heads * HD) + kv_head);
+#pragma unroll
+        for (int i = 0; i < DIMS; i += 2) {
+            const float2 v = dec_unpack(dec_e4m3(__ldg(reinterpret_cast<const unsigned short *>(row + kv_head * HD + dim + i))).x);
+            x[i] = scale * v.x;
+            x[i + 1] = scale * v.y;
+        }
+    }
+}
+// What a warp makes of a few query heads of a KV head and keys begin .. end - 1 of a sequence: the lane's dimensions of the sums, maximum
+// and sum of the probabilities (without the factor that the other kernel's carry). Fewer heads of 256, for the registers.
+template <int HD> constexpr int DEC_AT_ONCE = HD == 256 ? 2 : 4;
+template <int HD> struct DecodeColumns {
+    float o[DEC_AT_ONCE<HD>][HD / 32], m[DEC_AT_ONCE<HD>], l[DEC_AT_ONCE<HD>];
+};
+template <int FMT, int HD, bool WIDE>
+__device__ __noinline__ void decode_columns(const DecodeParams & p, int b, int seq, int head, int heads, int kv_head, int begin, int end, DecodeColumns<HD> & result) {
+    constexpr int DIMS = HD / 32, A = DEC_AT_ONCE<HD>, FLIGHT = 4;  // keys whose loads are in flight
+    const int lane = threadIdx.x & 31, dim = lane * DIMS;
+    const PagedCache & c = p.cache;
+    const int32_t * const table = c.tables + (int64_t)seq * c.table_stride;
+    float q[A][DIMS], o[A][DIMS], m[A], l[A];
+#pragma unroll
+    for (int a = 0; a < A; a++) {
+        DecodeRaw<WIDE, DIMS> raw;
+        raw.load(p.q, b * p.q_row + (head + min(a, heads - 1)) * p.q_head + dim);
+#pragma unroll
+        for (int i = 0; i < DIMS; i += 2) {
+            const float2 x = raw.pair(i / 2, p.dtype);
+            q[a][i] = x.x;
+            q[a][i + 1] = x.y;
+            o[a][i] = o[a][i + 1] = 0.0f;
+        }
+        m[a] = DEC_LOWEST;
+        l[a] = 0.0f;
+    }
+#pragma unroll 1
+    for (int pos = begin; pos < end; pos += 32) {
+        const int n = min(32, end - pos), mine = lane < n ? kv_slot(c, table, pos + lane) : 0;
+        float s[A], sum[A][DIMS];
+#pragma unroll
+        for (int a = 0; a < A; a++) s[a] = lane < n ? __uint_as_float(0x7fffffffu) : -INFINITY;  // (NaN stays for a bad block)
+#pragma unroll 1
+        for (int k = 0; k < n; k += FLIGHT) {  // (a lane behind the last key has row 0, and what comes of it goes nowhere)
+            float x[FLIGHT][DIMS];
+#pragma unroll
+            for (int i = 0; i < FLIGHT; i++) decode_row<FMT, HD>(c.k + (int64_t)max(__shfl_sync(0xffffffffu, mine, k + i), 0) * c.row_bytes, c, kv_head, x[i]);
+#pragma unroll
+            for (int i = 0; i < FLIGHT; i++)
+#pragma unroll
+                for (int a = 0; a < A; a++) {
+                    float dot = 0.0f;
+#pragma unroll
+                    for (int d = 0; d < DIMS; d++) dot = fmaf(q[a][d], x[i][d], dot);
+#pragma unroll
+                    for (int w = 16; w > 0; w >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, w);
+                    if (lane == k + i && lane < n && mine >= 0) s[a] = dot * p.scale_log2;
+                }
+        }
+#pragma unroll
+        for (int a = 0; a < A; a++) {
+            float top = s[a];
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            top = fmaxf(top, m[a]);
+            const float corr = exp2f(m[a] - top);
+            m[a] = top;
+            s[a] = exp2f(s[a] - top);
+            float part = s[a];
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) part += __shfl_xor_sync(0xffffffffu, part, w);
+            l[a] = fmaf(l[a], corr, part);
+#pragma unroll
+            for (int d = 0; d < DIMS; d++) {
+                o[a][d] *= corr;
+                sum[a][d] = 0.0f;
+            }
+        }
+#pragma unroll 1
+        for (int k = 0; k < n; k += FLIGHT) {
+            float x[FLIGHT][DIMS];
+#pragma unroll
+            for (int i = 0; i < FLIGHT; i++) decode_row<FMT, HD>(c.v + (int64_t)max(__shfl_sync(0xffffffffu, mine, k + i), 0) * c.row_bytes, c, kv_head, x[i]);
+#pragma unroll
+            for (int i = 0; i < FLIGHT; i++)
+#pragma unroll
+                for (int a = 0; a < A; a++) {
+                    const float w = __shfl_sync(0xffffffffu, s[a], k + i);
+                    if (k + i < n)
+#pragma unroll
+                        for (int d = 0; d < DIMS; d++) sum[a][d] = fmaf(w, x[i][d], sum[a][d]);
+                }
+        }
+#pragma unroll
+        for (int a = 0; a < A; a++)
+#pragma unroll
+            for (int d = 0; d < DIMS; d++) o[a][d] += sum[a][d];  // (32 keys on their own: fewer roundings of the whole sum)
+    }
+#pragma unroll
+    for (int a = 0; a < A; a++) {
+#pragma unroll
+        for (int d = 0; d < DIMS; d++) result.o[a][d] = o[a][d];
+        result.m[a] = m[a];
+        result.l[a] = l[a];
+    }
+}
+// The result of a head whose sums are complete, in the lanes of a warp.
+template <int HD, bool WIDE> __device__ __forceinline__ void decode_column_write(const DecodeParams & p, int b, int head, float (&o)[HD / 32], float m, float l) {
+    constexpr int DIMS = HD / 32;
+    const int lane = threadIdx.x & 31, dim = lane * DIMS;
+    float f[DIMS];
+    if (p.gate) {
+        DecodeRaw<WIDE, DIMS> raw;
+        raw.load(p.gate, b * p.q_row + head * p.q_head + dim);
+        dec_gates<WIDE, DIMS>(p, raw, f);
+    }
+#pragma unroll
+    for (int i = 0; i < DIMS; i++) o[i] = l == 0.0f ? 0.0f : o[i] / l * (p.gate ? f[i] : 1.0f);
+    dec_write<WIDE, DIMS>(p, b, head, dim, o);
+    if (lane == 0) dec_write_lse(p, b, head, m + DEC_P_LOG2, l);
+}
+// DEC_AT_ONCE heads of a row that several teams share, by all warps of a CTA: each takes some of the keys. `store`: shared memory.
+template <int HD> constexpr int DEC_STORE = 8 * DEC_AT_ONCE<HD> * (HD + 2);  // floats
+template <int FMT, int HD, bool WIDE> __device__ __noinline__ void decode_row_again(const DecodeParams & p, int b, int unit, int col, float * store) {
+    constexpr int DIMS = HD / 32, A = DEC_AT_ONCE<HD>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;  // (eight)
+    const DecodeHeads heads = decode_heads(p, unit);
+    const DecodeSpan span = decode_span(p, b, 16);
+    const int each = ((span.end - span.first + 32 * warps - 1) / (32 * warps)) * 32, begin = min(span.first + warp * each, span.end);
+    DecodeColumns<HD> r;
+    decode_columns<FMT, HD, WIDE>(p, b, max(span.seq, 0), heads.first + col, min(A, heads.count - col), heads.kv_head, begin, min(begin + each, span.end), r);
+    __syncthreads();  // (the store's last use)
+#pragma unroll
+    for (int a = 0; a < A; a++) {
+        float * const mine = store + (warp * A + a) * (HD + 2);
+#pragma unroll
+        for (int i = 0; i < DIMS; i++) mine[lane * DIMS + i] = r.o[a][i];
+        if (lane == 0) {
+            mine[HD] = r.m[a];
+            mine[HD + 1] = r.l[a];
+        }
+    }
+    __syncthreads();
+    if (warp < A && col + warp < heads.count) {
+        float o[DIMS], m = DEC_LOWEST, l = 0.0f;
+        for (int w = 0; w < warps; w++) m = fmaxf(m, store[(w * A + warp) * (HD + 2) + HD]);
+#pragma unroll
+        for (int i = 0; i < DIMS; i++) o[i] = 0.0f;
+        for (int w = 0; w < warps; w++) {
+            const float * const part = store + (w * A + warp) * (HD + 2);
+            const float f = exp2f(part[HD] - m);
+            l = fmaf(f, part[HD + 1], l);
+#pragma unroll
+            for (int i = 0; i < DIMS; i++) o[i] = fmaf(f, part[lane * DIMS + i], o[i]);
+        }
+        decode_column_write<HD, WIDE>(p, b, heads.first + col + warp, o, m, l);
+    }
+    __syncthreads();
+}
+// Whole rows of a run: the warps of the CTA take them in turn.
+template <int FMT, int HD, int NT, bool WIDE> __device__ __noinline__ void decode_again(const DecodeParams & p, unsigned unit, unsigned team) {
+    using S = DecodeShape<FMT, HD, NT, WIDE>;
+    constexpr int KEYS = S::KEYS;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const PagedCache & c = p.cache;
+    const unsigned units = c.kv_heads * p.head_tiles, teams = max(p.warps / units, 1u);
+    if (unit >= units || team >= teams) return;
+    unsigned total = 0;
+    for (int b = lane; b < p.batch; b += 32) total += decode_span(p, b, KEYS).tiles;
+    total = __reduce_add_sync(0xffffffffu, total);
+    const unsigned share = (total + teams - 1) / teams, begin = team * share;
+    if (begin >= total) return;
+    const DecodeHeads heads = decode_heads(p, unit);
+    DecodeCursor<KEYS> use;
+    use.seek(p, begin);
+    unsigned left = min(share, total - begin);
+    for (int turn = 0; left > 0 && use.b < p.batch; turn++) {
+        const unsigned tiles = min((unsigned)use.left, left);
+        if (use.left == use.tiles && tiles == (unsigned)use.tiles && use.end > use.first && turn % warps == warp) {
+            // The row's largest and smallest scale of V but zero, as the other kernel has seen them. (Half its ratio: its unit is the next
+            // power of two.)
+            const int32_t * const table = c.tables + (int64_t)use.seq * c.table_stride;
+            float largest = 0.0f, least = INFINITY;
+            bool wild = false;
+            for (int pos = use.first + lane; pos < use.end; pos += 32) {
+                const int slot = kv_slot(c, table, pos);
+                if (slot < 0) continue;
+                const uint8_t * const row = c.v + (int64_t)slot * c.row_bytes;
+                for (int i = 0; i < (FMT == YUUKA_KV_Q8_0 ? HD / 32 : 1); i++) {
+                    float d;
+                    if constexpr (FMT == YUUKA_KV_Q8_0)
+                        d = fabsf(__half2float(__ushort_as_half(__ldg(reinterpret_cast<const unsigned short *>(row + (heads.kv_head * (HD / 32) + i) * 34)))));
+                    else d = fabsf(__ldg(reinterpret_cast<const float *>(row + c.kv_heads * HD) + heads.kv_head));
+                    wild |= !(d < 1.7e38f);
+                    largest = fmaxf(largest, d);
+                    if (d != 0.0f) least = fminf(least, d);
+                }
+            }
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) {
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, w));
+                least = fminf(least, __shfl_xor_sync(0xffffffffu, least, w));
+            }
+            if (__any_sync(0xffffffffu, wild || least * (float)(1 << (S::FAR_LOG2 - 1)) < largest || least < 1.2e-38f))
+                for (int col = 0; col < heads.count; col += DEC_AT_ONCE<HD>) {
+                    const int n = min(DEC_AT_ONCE<HD>, heads.count - col);
+                    DecodeColumns<HD> r;
+                    decode_columns<FMT, HD, WIDE>(p, use.b, use.seq, heads.first + col, n, heads.kv_head, use.first, use.end, r);
+#pragma unroll
+                    for (int a = 0; a < DEC_AT_ONCE<HD>; a++)
+                        if (a < n) decode_column_write<HD, WIDE>(p, use.b, heads.first + col + a, r.o[a], r.m[a], r.l[a]);
+                }
+        }
+        left -= tiles;
+        if (++use.b < p.batch) use.row(p);
+        use.pos = use.first;
+        use.left = use.tiles;
     }
 }
 
@@ -1185,13 +1455,17 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 // takes 32 dimensions of a column at a time; groups of 8 threads take every 32nd partial, so that many loads are in flight, and
 // are added in their order.
 constexpr int JOIN_THREADS = 256, JOIN_CTAS_SM = 4, JOIN_LANES = 8, JOIN_GROUPS = JOIN_THREADS / JOIN_LANES;
-template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_THREADS) attention_decode_join_kernel(const DecodeParams p) {
-    constexpr int PART = COLS * (HD + 2), SLICES = HD / (4 * JOIN_LANES), DIMS = HD / 32;
-    __shared__ float factor[DEC_WARPS], reduce[2][JOIN_THREADS / 32];
+template <int FMT, int HD, int NT, bool WIDE>  // (FMT: Q8_0, F8 or any other)
+__global__ void __launch_bounds__(JOIN_THREADS, 2) attention_decode_join_kernel(const __grid_constant__ DecodeParams p) {
+    using S = DecodeShape<FMT, HD, NT, WIDE>;
+    constexpr int COLS = S::COLS, PART = COLS * (HD + 2), SLICES = HD / (4 * JOIN_LANES), DIMS = HD / 32;
+    constexpr bool FAR = S::IS_Q8 || S::IS_F8;  // (joins of which a part's sum has a sign are rows to be done again)
+    __shared__ float factor[FAR && DEC_STORE<HD> > DEC_WARPS ? DEC_STORE<HD> : DEC_WARPS], reduce[2][JOIN_THREADS / 32];
     __shared__ float4 sums[JOIN_GROUPS][JOIN_LANES];
     pdl_entry();
     const int tid = threadIdx.x, units = p.cache.kv_heads * p.head_tiles, group = tid / JOIN_LANES;
-    const int few = min(p.counters[DEC_SHORT], DEC_WARPS), jobs = min(p.counters[DEC_LONG], DEC_WARPS) * COLS * SLICES;
+    const int few = min(p.counters[DEC_SHORT], DEC_WARPS), jobs = min(p.counters[DEC_LONG], DEC_WARPS) * COLS * SLICES,
+              runs = FAR ? min(p.counters[DEC_FAR], DEC_FAR_MOST) : 0;
 #pragma unroll 1
     for (int job = blockIdx.x; job < few; job += gridDim.x) {
         const int4 join = p.joins[job];
@@ -1200,9 +1474,13 @@ template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_TH
         const int n = join.w - join.z + 1, lane = tid & 31, dim = lane * DIMS;
         const float * first = p.partial + ((size_t)join.z * units + join.y) * 2 * PART;
         const int64_t stride = (int64_t)units * 2 * PART;
+        // (of the first column: the same for all, and known to warps without a column)
+        [[maybe_unused]] const float sign = FAR && lane < n ? first[lane * stride + (lane ? 0 : PART) + COLS * HD + COLS] : 0.0f;
         for (int col = tid >> 5; col < h.count; col += JOIN_THREADS / 32) {
             const float * mine = first + lane * stride + (lane ? 0 : PART) + COLS * HD + col;
             const float ms = lane < n ? mine[0] : -INFINITY, ls = lane < n ? mine[COLS] : 0.0f;
+            if constexpr (FAR)
+                if (__any_sync(0xffffffffu, (int)__float_as_uint(sign) < 0)) break;
             DecodeRaw<WIDE, DIMS> raw;
             if (p.gate) raw.load(p.gate, join.x * p.q_row + (h.first + col) * p.q_head + dim);
             float m = ms, x[DIMS];
@@ -1238,6 +1516,9 @@ template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_TH
             dec_write<WIDE, DIMS>(p, join.x, h.first + col, dim, x);
             if (lane == 0) dec_write_lse(p, join.x, h.first + col, m, l);
         }
+        if constexpr (FAR)
+            if (__any_sync(0xffffffffu, (int)__float_as_uint(sign) < 0))  // (the same for all warps)
+                for (int col = 0; col < h.count; col += DEC_AT_ONCE<HD>) decode_row_again<FMT, HD, WIDE>(p, join.x, join.y, col, factor);
     }
 #pragma unroll 1
     for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
@@ -1272,15 +1553,26 @@ template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_TH
 #pragma unroll
         for (int w = 0; w < JOIN_THREADS / 32; w++) m = fmaxf(m, reduce[0][w]);
         float l = 0.0f;
+        [[maybe_unused]] bool far = false;
         for (int k = tid; k < n; k += JOIN_THREADS) {
             const float f = exp2f(part(k)[COLS * HD + col] - m);
             factor[k] = f;
-            l = fmaf(f, part(k)[COLS * HD + COLS + col], l);
+            const float lk = part(k)[COLS * HD + COLS + col];
+            if constexpr (FAR) far |= (int)__float_as_uint(lk) < 0;
+            l = fmaf(f, lk, l);
         }
 #pragma unroll
         for (int w = 16; w > 0; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
         if ((tid & 31) == 0) reduce[1][tid >> 5] = l;
-        __syncthreads();
+        if constexpr (FAR) {
+            if (__syncthreads_or(far)) {
+                // (the CTA of the first dimensions and column does them all)
+                if (dim < 4 * JOIN_LANES && col % DEC_AT_ONCE<HD> == 0) decode_row_again<FMT, HD, WIDE>(p, join.x, join.y, col, factor);
+                continue;
+            }
+        } else {
+            __syncthreads();
+        }
         l = 0.0f;
 #pragma unroll
         for (int w = 0; w < JOIN_THREADS / 32; w++) l += reduce[1][w];
@@ -1322,9 +1614,12 @@ template <int HD, int COLS, bool WIDE> __global__ void __launch_bounds__(JOIN_TH
         }
         __syncthreads();
     }
+    if constexpr (FAR)
+#pragma unroll 1
+        for (int job = blockIdx.x; job < runs; job += gridDim.x) decode_again<FMT, HD, NT, WIDE>(p, p.far[job].x, p.far[job].y);
     // the last CTA leaves the counters as the call found them
     __syncthreads();
-    if (tid == 0 && atomicAdd(p.counters + DEC_DONE, 1) == (int)gridDim.x - 1) p.counters[DEC_SHORT] = p.counters[DEC_LONG] = p.counters[DEC_DONE] = 0;
+    if (tid == 0 && atomicAdd(p.counters + DEC_DONE, 1) == (int)gridDim.x - 1) p.counters[DEC_SHORT] = p.counters[DEC_LONG] = p.counters[DEC_FAR] = p.counters[DEC_DONE] = 0;
 }
 
 // Launches for one format on a device with `sms` multiprocessors.
@@ -1342,7 +1637,8 @@ template <int FMT, int HD, int NT, bool WIDE> void launch_decode_as(cudaStream_t
     YK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::LAYOUT_BYTES));
     p.warps = ctas * S::W;
     launch_k(kern, (unsigned)ctas, S::W * 32, S::LAYOUT_BYTES, s, p);
-    launch_k(attention_decode_join_kernel<HD, S::COLS, WIDE>, (unsigned)(sms * JOIN_CTAS_SM), JOIN_THREADS, 0, s, p);
+    constexpr int JOIN = S::IS_Q8 || S::IS_F8 ? FMT : YUUKA_KV_F16;
+    launch_k(attention_decode_join_kernel<JOIN, HD, NT, WIDE>, (unsigned)(sms * JOIN_CTAS_SM), JOIN_THREADS, 0, s, p);
 }
 template <int FMT, int HD, int NT> void launch_decode_tiles(cudaStream_t s, const DecodeParams & p, int sms) {
     if (p.dtype == YUUKA_DTYPE_F32) launch_decode_as<FMT, HD, NT, true>(s, p, sms);
