@@ -1,8 +1,8 @@
-"""attention_decode where numbers leave the ordinary."""
+"""attention_decode where numbers leave the ordinary: infinite keys and values, values far apart, strong gates."""
 import numpy as np
 import pytest
 
-from tests.kv_reference import DTYPES, attend, attend_bounds, decode, from_dtype, to_dtype
+from tests.kv_reference import DTYPES, HALF_STEP, attend, attend_bounds, decode, encode, from_dtype, to_dtype
 from tests.test_attention_decode_gpu import Step, dev, scratch, stream  # noqa: F401  (fixtures)
 from yuuka_b200 import cuda
 
@@ -204,4 +204,25 @@ def test_values_far_apart_in_more_heads_than_warps(dev, stream, scratch, fmt):  
             want, want_lse, weight, reach = attend(q[b, h].astype(np.float64), k[:, h // 17], v[:, h // 17], step.scale)
             far, far_lse = attend_bounds(want, want_lse, weight, reach, dim, "f32")
             assert np.all(np.abs(out[b, h] - want) <= far) and abs(lse[b, h] - want_lse) <= far_lse, (b, h)
+    step.free()
+
+
+@pytest.mark.parametrize("fmt,dtype", [("f16", "f32"), ("q8_0", "f32"), ("f8", "f32"), ("f32", "f32"), ("f16", "f16"), ("f8", "bf16")])
+def test_strong_gates(dev, stream, scratch, fmt, dtype):  # noqa: F811
+    """Gates from -100 to 100, over one key (the output is its value times the gate) and over joined runs. An exponential is off by
+    an f32 step, sum, quotient and product by half of one each: 2^-22 at most, with the value's own 2^-22 beside it."""
+    step = Step(dev, stream, 9, fmt, dtype, 2, 2, 128, 16, [1, 1, 1500], gate=True)
+    q = from_dtype(step.qg, dtype)
+    q[..., 128:] = np.linspace(-1, 1, 128) * np.array([30.0, 100.0, 30.0])[:, None, None]
+    step.qg = to_dtype(q.astype(np.float32), dtype)
+    step.qb.write(step.qg)
+    q = from_dtype(step.qg, dtype)
+    out, lse = step.run(scratch)
+    if dtype != "f16":  # (f16 outputs below 2^-14 have no relative bound: 2^-25 below)
+        step.check(out, lse)
+    for b in range(2):
+        v = decode(step.paged.v[step.paged.slots(b, np.array([0]))], fmt, 2, 128)[0]
+        want = np.repeat(v, 2, axis=0) / (1 + np.exp(-q[b, :, 128:]))
+        bound = np.abs(want) * (HALF_STEP[dtype] + 2.0 ** -21 + (0 if dtype == "f32" else 2.0 ** -11)) + (1e-36 if dtype != "f16" else 2.0 ** -25)
+        assert np.all(np.abs(out[b] - want) <= bound), float(np.max(np.abs(out[b] - want) / bound))
     step.free()

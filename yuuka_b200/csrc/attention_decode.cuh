@@ -352,9 +352,16 @@ template <bool WIDE, int N> __device__ __forceinline__ void dec_gates(const Deco
 #pragma unroll
     for (int i = 0; i < N / 2; i++) {
         const float2 z = raw.pair(i, p.dtype);
-        // (approximate exponential and reciprocal: 2^-21 in all)
-        f[2 * i] = __fdividef(1.0f, 1.0f + __expf(-z.x));
-        f[2 * i + 1] = __fdividef(1.0f, 1.0f + __expf(-z.y));
+        if constexpr (WIDE) {
+            // of e^-|z|, which does not overflow: within 2^-22 of the gate. (The approximate exponential's error grows with |z|.)
+            const float ex = expf(-fabsf(z.x)), ey = expf(-fabsf(z.y));
+            f[2 * i] = (z.x < 0.0f ? ex : 1.0f) / (1.0f + ex);
+            f[2 * i + 1] = (z.y < 0.0f ? ey : 1.0f) / (1.0f + ey);
+        } else {
+            // (approximate exponential and reciprocal: (4 + |z|) 2^-23, for outputs that are rounded to 2^-11 or 2^-8)
+            f[2 * i] = __fdividef(1.0f, 1.0f + __expf(-z.x));
+            f[2 * i + 1] = __fdividef(1.0f, 1.0f + __expf(-z.y));
+        }
     }
 }
 // N neighbouring values of a head's result, rounded to the output's type
