@@ -745,6 +745,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 float (&s)[NT][4] = sh[half];
                 const uint32_t kh = ks + half * S::K16;
                 float s2[NT][4];
+                [[maybe_unused]] float s3[NT][4] = {};
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -851,27 +852,26 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             const uint4 f = query(nt, 2 * c), f2 = query(nt, 2 * c + 1);
+                            dec_mma16(s[nt], ka.x, kb.x, ka.y, kb.y, f.x, f.y);
+                            dec_mma16(s2[nt], ka.z, kb.z, ka.w, kb.w, f2.x, f2.y);
                             if constexpr (WIDE) {  // second parts on their own: their signs are any
-                                dec_mma16(s[nt], ka.x, kb.x, ka.y, kb.y, f.x, f.y);
-                                dec_mma16(s2[nt], ka.x, kb.x, ka.y, kb.y, f.z, f.w);
-                                dec_mma16(s[nt], ka.z, kb.z, ka.w, kb.w, f2.x, f2.y);
-                                dec_mma16(s2[nt], ka.z, kb.z, ka.w, kb.w, f2.z, f2.w);
-                            } else {
-                                dec_mma16(s[nt], ka.x, kb.x, ka.y, kb.y, f.x, f.y);
-                                dec_mma16(s2[nt], ka.z, kb.z, ka.w, kb.w, f2.x, f2.y);
+                                dec_mma16(s3[nt], ka.x, kb.x, ka.y, kb.y, f.z, f.w);
+                                dec_mma16(s3[nt], ka.z, kb.z, ka.w, kb.w, f2.z, f2.w);
                             }
                         }
                     }
                 }
                 // an infinity of K makes the sum of the first parts infinite or NaN as it should be, and nothing of the second parts,
                 // which it meets with either sign or a zero
-                constexpr bool SPLIT = S::IS_F32 || (FMT == YUUKA_KV_F16 && WIDE);
                 if constexpr (!S::IS_Q8)
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (!SPLIT || fabsf(s[nt][e]) < INFINITY) s[nt][e] += s2[nt][e];
+                        for (int e = 0; e < 4; e++) {
+                            if (!S::IS_F32 || fabsf(s[nt][e]) < INFINITY) s[nt][e] += s2[nt][e];
+                            if constexpr (FMT == YUUKA_KV_F16 && WIDE)
+                                if (fabsf(s[nt][e]) < INFINITY) s[nt][e] += s3[nt][e];
+                        }
                 if constexpr (S::IS_F8) {
                     const uint32_t at = ks + S::K16 * HALVES + 64 * half + 4 * g;
                     const float d0 = __uint_as_float(dec_lds(at)), d1 = __uint_as_float(dec_lds(at + 32));
