@@ -346,6 +346,16 @@ template <bool WIDE, int N> struct DecodeRaw {
             return dtype == YUUKA_DTYPE_F16 ? h : b;
         }
     }
+    __device__ __forceinline__ void set(float2 x, int dtype) {  // values 0 and 1 (which the type can hold)
+        if constexpr (WIDE) {
+            w[0] = __float_as_uint(x.x);
+            w[1] = __float_as_uint(x.y);
+        } else if (dtype == YUUKA_DTYPE_F16) {
+            w[0] = dec_pack(x.x, x.y);
+        } else {
+            w[0] = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+        }
+    }
 };
 // the gates of N neighbouring values of a head: what the values are multiplied with
 template <bool WIDE, int N> __device__ __forceinline__ void dec_gates(const DecodeParams & p, const DecodeRaw<WIDE, N> & raw, float (&f)[N]) {
@@ -581,14 +591,28 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
 #pragma unroll
                     for (int i = 0; i < 2 * QM; i++) raw[i].load(p.q, at + S::q_dim(i >> 1, i & 1, t));
                     float amax = 0.0f;
+                    [[maybe_unused]] float least = INFINITY;
 #pragma unroll
                     for (int i = 0; i < 2 * QM; i++) {
                         const float2 x = raw[i].pair(0, p.dtype);
                         amax = fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y)));
+                        if constexpr (FMT == YUUKA_KV_F16) least = fminf(least, fminf(fabsf(x.x), fabsf(x.y)));
                     }
                     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                     const int e = min(max((int)(__float_as_uint(amax) >> 23), 15), 254);
+                    if constexpr (FMT == YUUKA_KV_F16) {
+                        // no first part is zero but of a zero: its sign decides over an infinite key. 2^-24 in its units, 2^-38 of the largest
+                        const float low = e > 38 ? __int_as_float((e - 38) << 23) : 0.0f;
+                        if (least < low)
+#pragma unroll
+                            for (int i = 0; i < 2 * QM; i++) {
+                                float2 x = raw[i].pair(0, p.dtype);
+                                if (x.x != 0.0f) x.x = copysignf(fmaxf(fabsf(x.x), low), x.x);
+                                if (x.y != 0.0f) x.y = copysignf(fmaxf(fabsf(x.y), low), x.y);
+                                raw[i].set(x, p.dtype);
+                            }
+                    }
                     const float up = has ? sign * __int_as_float((268 - e) << 23) : 0.0f;                          // 2^(14 - (e - 127))
                     const float down = fmaxf(fabsf(p.scale_log2) * __int_as_float((e - 14) << 23), 1e-37f);        // |scale| / up
                     scale[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
@@ -602,10 +626,6 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                             x.x *= up;
                             x.y *= up;
                             hi[half] = dec_pack(x.x, x.y);
-                            if constexpr (FMT == YUUKA_KV_F16) {  // no zero for a tiny value: its sign decides over an infinite key
-                                if (x.x != 0.0f && !(hi[half] & 0x7fffu)) hi[half] |= 1u;
-                                if (x.y != 0.0f && !(hi[half] & 0x7fff0000u)) hi[half] |= 0x10000u;
-                            }
                             const float2 r = dec_unpack(hi[half]);
                             lo[half] = dec_pack(x.x - r.x, x.y - r.y);
                         }
