@@ -104,9 +104,9 @@ def test_values_that_are_not_finite_stay_in_their_place(dev, stream, scratch, fm
     step.free()
 
 
-def apart(step, ratio, gap, where, blocks):
+def apart(step, ratio, gap, where, blocks, only=None):
     """V of magnitude 2^-6 (F8: 1), and of 2^ratio times that in every 50th key from `where` on; the queries of even heads score
-    those keys `gap` nats below the others, of odd heads as much above. blocks: in the second 32 dimensions alone."""
+    those keys `gap` nats below the others, of odd heads as much above. blocks: in the second 32 dimensions alone. only: of these sequences."""
     rng, d, dt = np.random.default_rng(100 + ratio), step.dim, step.dtype
     u = np.where(rng.random(d) < 0.5, -1.0, 1.0)
     q = np.broadcast_to(u, (step.batch, step.heads, d)).copy()
@@ -117,7 +117,7 @@ def apart(step, ratio, gap, where, blocks):
     for s, n in enumerate(step.lens):
         k = rng.standard_normal((n, 1, d)) * 0.25
         v = rng.standard_normal((n, 1, d)) * small
-        far = np.arange(where % n, n, 50)
+        far = np.arange(where % n, n, 50) if only is None or s in only else np.zeros(0, np.int64)
         k[far, 0] = -u * (gap / (d * step.scale)) + 0.01 * rng.standard_normal((len(far), d))
         v[far, :, 32:64] *= 2.0 ** ratio
         if not blocks:
@@ -174,6 +174,19 @@ def test_values_far_apart_in_rows_of_any_split(dev, stream, scratch, fmt, dtype,
     for b in range(step.batch):  # the same row in every split: sums of another order
         assert np.allclose(out[b], out[b % 4], rtol=1e-4 if dtype == "f32" else 0.03, atol=1e-4 * np.abs(out[b]).max()), b
     gb.free()
+    step.free()
+
+
+@pytest.mark.parametrize("fmt,dtype", [("q8_0", "f32"), ("f8", "bf16")])
+@pytest.mark.parametrize("crowd", [1, 7, 60])
+@pytest.mark.parametrize("only", [0, 2, 3])
+def test_one_sequence_with_values_far_apart(dev, stream, scratch, fmt, dtype, crowd, only):  # noqa: F811
+    """Rows that are done again between rows that are not, whole, joined from a few runs and from many."""
+    lens = [70, 1, 333, 2600, 500, 90]
+    step = Step(dev, stream, 3, fmt, dtype, 1, 5, 128, 16, lens, seq_ids=list(range(6)) * crowd)
+    apart(step, 22, 24, 5, False, [only])
+    out, lse = step.run(scratch)
+    check_keys(step, out, lse, lambda s: np.arange(lens[s]), sorted({*range(6), *range(step.batch - 6, step.batch), step.batch // 12 * 6 + only}))
     step.free()
 
 

@@ -1268,13 +1268,13 @@ template <int FMT, int HD> __device__ __forceinline__ void decode_row(const uint
     }
 }
 // What a warp makes of a few query heads of a KV head and keys begin .. end - 1 of a sequence: the lane's dimensions of the sums, maximum
-// and sum of the probabilities (without the factor that the other kernel's carry). Fewer heads of 256, for the registers.
-template <int HD> constexpr int DEC_AT_ONCE = HD == 256 ? 2 : 4;
+// and sum of the probabilities (without the factor that the other kernel's carry). As few heads at once as leave the joins their registers.
+template <int HD> constexpr int DEC_AT_ONCE = HD == 256 ? 1 : 2;
 template <int HD> struct DecodeColumns {
     float o[DEC_AT_ONCE<HD>][HD / 32], m[DEC_AT_ONCE<HD>], l[DEC_AT_ONCE<HD>];
 };
 template <int FMT, int HD, bool WIDE>
-__device__ __noinline__ void decode_columns(const DecodeParams & p, int b, int seq, int head, int heads, int kv_head, int begin, int end, DecodeColumns<HD> & result) {
+__device__ __forceinline__ void decode_columns(const DecodeParams & p, int b, int seq, int head, int heads, int kv_head, int begin, int end, DecodeColumns<HD> & result) {
     constexpr int DIMS = HD / 32, A = DEC_AT_ONCE<HD>, FLIGHT = 4;  // keys whose loads are in flight
     const int lane = threadIdx.x & 31, dim = lane * DIMS;
     const PagedCache & c = p.cache;
@@ -1381,7 +1381,7 @@ template <int HD, bool WIDE> __device__ __forceinline__ void decode_column_write
 }
 // DEC_AT_ONCE heads of a row that several teams share, by all warps of a CTA: each takes some of the keys. `store`: shared memory.
 template <int HD> constexpr int DEC_STORE = 8 * DEC_AT_ONCE<HD> * (HD + 2);  // floats
-template <int FMT, int HD, bool WIDE> __device__ __noinline__ void decode_row_again(const DecodeParams & p, int b, int unit, int col, float * store) {
+template <int FMT, int HD, bool WIDE> __device__ __forceinline__ void decode_row_again(const DecodeParams & p, int b, int unit, int col, float * store) {
     constexpr int DIMS = HD / 32, A = DEC_AT_ONCE<HD>;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;  // (eight)
     const DecodeHeads heads = decode_heads(p, unit);
@@ -1418,7 +1418,7 @@ template <int FMT, int HD, bool WIDE> __device__ __noinline__ void decode_row_ag
     __syncthreads();
 }
 // Whole rows of a run: the warps of the CTA take them in turn.
-template <int FMT, int HD, int NT, bool WIDE> __device__ __noinline__ void decode_again(const DecodeParams & p, unsigned unit, unsigned team) {
+template <int FMT, int HD, int NT, bool WIDE> __device__ __forceinline__ void decode_again(const DecodeParams & p, unsigned unit, unsigned team) {
     using S = DecodeShape<FMT, HD, NT, WIDE>;
     constexpr int KEYS = S::KEYS;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -1486,7 +1486,8 @@ template <int FMT, int HD, int NT, bool WIDE>  // (FMT: Q8_0, F8 or any other)
 __global__ void __launch_bounds__(JOIN_THREADS, 2) attention_decode_join_kernel(const __grid_constant__ DecodeParams p) {
     using S = DecodeShape<FMT, HD, NT, WIDE>;
     constexpr int COLS = S::COLS, PART = COLS * (HD + 2), SLICES = HD / (4 * JOIN_LANES), DIMS = HD / 32;
-    constexpr bool FAR = S::IS_Q8 || S::IS_F8;  // (joins of which a part's sum has a sign are rows to be done again)
+    constexpr bool FAR = S::IS_Q8 || S::IS_F8;  // (joins of which a part's sums have a sign are rows to be done again)
+    [[maybe_unused]] bool again = false;        // this warp has met one
     __shared__ float factor[FAR && DEC_STORE<HD> > DEC_WARPS ? DEC_STORE<HD> : DEC_WARPS], reduce[2][JOIN_THREADS / 32];
     __shared__ float4 sums[JOIN_GROUPS][JOIN_LANES];
     pdl_entry();
@@ -1501,13 +1502,14 @@ __global__ void __launch_bounds__(JOIN_THREADS, 2) attention_decode_join_kernel(
         const int n = join.w - join.z + 1, lane = tid & 31, dim = lane * DIMS;
         const float * first = p.partial + ((size_t)join.z * units + join.y) * 2 * PART;
         const int64_t stride = (int64_t)units * 2 * PART;
-        // (of the first column: the same for all, and known to warps without a column)
-        [[maybe_unused]] const float sign = FAR && lane < n ? first[lane * stride + (lane ? 0 : PART) + COLS * HD + COLS] : 0.0f;
         for (int col = tid >> 5; col < h.count; col += JOIN_THREADS / 32) {
             const float * mine = first + lane * stride + (lane ? 0 : PART) + COLS * HD + col;
             const float ms = lane < n ? mine[0] : -INFINITY, ls = lane < n ? mine[COLS] : 0.0f;
             if constexpr (FAR)
-                if (__any_sync(0xffffffffu, (int)__float_as_uint(sign) < 0)) break;
+                if (__any_sync(0xffffffffu, (int)__float_as_uint(ls) < 0)) {
+                    again = true;
+                    break;
+                }
             DecodeRaw<WIDE, DIMS> raw;
             if (p.gate) raw.load(p.gate, join.x * p.q_row + (h.first + col) * p.q_head + dim);
             float m = ms, x[DIMS];
@@ -1543,9 +1545,6 @@ __global__ void __launch_bounds__(JOIN_THREADS, 2) attention_decode_join_kernel(
             dec_write<WIDE, DIMS>(p, join.x, h.first + col, dim, x);
             if (lane == 0) dec_write_lse(p, join.x, h.first + col, m, l);
         }
-        if constexpr (FAR)
-            if (__any_sync(0xffffffffu, (int)__float_as_uint(sign) < 0))  // (the same for all warps)
-                for (int col = 0; col < h.count; col += DEC_AT_ONCE<HD>) decode_row_again<FMT, HD, WIDE>(p, join.x, join.y, col, factor);
     }
 #pragma unroll 1
     for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
@@ -1593,8 +1592,7 @@ __global__ void __launch_bounds__(JOIN_THREADS, 2) attention_decode_join_kernel(
         if ((tid & 31) == 0) reduce[1][tid >> 5] = l;
         if constexpr (FAR) {
             if (__syncthreads_or(far)) {
-                // (the CTA of the first dimensions and column does them all)
-                if (dim < 4 * JOIN_LANES && col % DEC_AT_ONCE<HD> == 0) decode_row_again<FMT, HD, WIDE>(p, join.x, join.y, col, factor);
+                again = true;
                 continue;
             }
         } else {
@@ -1641,9 +1639,34 @@ __global__ void __launch_bounds__(JOIN_THREADS, 2) attention_decode_join_kernel(
         }
         __syncthreads();
     }
-    if constexpr (FAR)
+    // Rows to be done again, behind the loops: inside them they took registers of theirs
+    if constexpr (FAR) {
 #pragma unroll 1
         for (int job = blockIdx.x; job < runs; job += gridDim.x) decode_again<FMT, HD, NT, WIDE>(p, p.far[job].x, p.far[job].y);
+        if (__syncthreads_or(again)) {  // (the jobs that this CTA has had)
+            auto is_far = [&](const int4 & join) {
+                bool far = false;
+                for (int k = tid; k <= join.w - join.z; k += JOIN_THREADS)
+                    far |= (int)__float_as_uint(p.partial[(((size_t)(join.z + k) * units + join.y) * 2 + (k ? 0 : 1)) * PART + COLS * HD + COLS]) < 0;
+                return __syncthreads_or(far) != 0;
+            };
+#pragma unroll 1
+            for (int job = blockIdx.x; job < few; job += gridDim.x) {
+                const int4 join = p.joins[job];
+                if (!decode_join_sound(p, join) || !is_far(join)) continue;
+                const int count = decode_heads(p, join.y).count;
+                for (int col = 0; col < count; col += DEC_AT_ONCE<HD>) decode_row_again<FMT, HD, WIDE>(p, join.x, join.y, col, factor);
+            }
+            // the job of a long join's first dimensions, and of the first of so many columns, does them all
+#pragma unroll 1
+            for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
+                const int4 join = p.joins[DEC_WARPS + job / (COLS * SLICES)];
+                const int col = job / SLICES % COLS;
+                if (!decode_join_sound(p, join) || job % SLICES != 0 || col % DEC_AT_ONCE<HD> != 0 || col >= decode_heads(p, join.y).count || !is_far(join)) continue;
+                decode_row_again<FMT, HD, WIDE>(p, join.x, join.y, col, factor);
+            }
+        }
+    }
     // the last CTA leaves the counters as the call found them
     __syncthreads();
     if (tid == 0 && atomicAdd(p.counters + DEC_DONE, 1) == (int)gridDim.x - 1) p.counters[DEC_SHORT] = p.counters[DEC_LONG] = p.counters[DEC_FAR] = p.counters[DEC_DONE] = 0;
