@@ -217,13 +217,14 @@ YUUKA_API yuuka_status yuuka_weights_tile(yuuka_stream * stream, yuuka_buffer * 
 /* ---- A paged key-value cache for hosts with layers of their own ----
  * What YUUKA_OP_ATTENTION_PREFILL_PAGED reads and the KV half of ATTENTION_PREP writes (yuuka_hip.h:104-149), as calls on
  * buffers of the caller: rows go into the pools in the pools' format, come back as plain numbers, and are attended to by
- * one new token per sequence. Sessions do the same on pools of their own.
+ * one new token per sequence. Sessions do the same on pools of their own (F32 and F16 rows are theirs byte for byte).
  *
  * K and V pools are [pool_blocks][block_size][yuuka_kv_row_bytes], a row all KV heads of a token behind one another;
  * position p of sequence s lies in row p % block_size of block tables[s][p / block_size] (memory.Table.Map). Formats:
  *   F32, F16  the values; F16 rounds half up on the dropped bits, as sessions do (tensor/half.go:36-68)
  *   Q8_0      blocks of 32 values: f16 scale s = amax * (1 / 127), int8 x / s rounded half away from zero (kv_format.go:97-131;
- *             s is taken in f32 by the inverse, which is within an ulp of the quotient that sessions take)
+ *             s is taken in f32 by the inverse, which is within an ulp of the quotient that sessions take: the same scales in
+ *             f16, and values that differ by one from a session's where x / s lies on or next to a half)
  *   F8        kv_heads * head_dim E4M3 values x * ((1 / amax) * 448), rounded to nearest even, amax over a token's head; then
  *             kv_heads f32 scales amax * (1 / 448); zeros up to a multiple of 16 bytes. A value is its E4M3 times the scale.
  *             A head for which 448 / amax passes 3e38 (amax below 1.5e-36) is stored as zeros, one with a NaN with a NaN

@@ -7,10 +7,10 @@
 // passes it by 2^4 (in the first tiles, mostly), so the largest p is 2^15, those down to 2^-25 of 2^m stay normal in f16, and
 // what is rounded away is below 2^-36 of it. (A slack of 2^8 with a factor of 2^7 took as long.)
 //
-// What bounds it: the bytes of the cache, read once, over F32 and F16 pools (72 to 100 % of the memory's measured 6.54 TB/s
-// for long sequences; F32 with heads of 256, whose products are three to one, 40 to 78). Over Q8_0 (29 to 55 %) and F8 (41 to
-// 77 %) the chain of instructions from a tile's bytes to its products takes longer than the bytes' way (41 % of the issue
-// slots, with the three or four warps a scheduler that registers allow). The products run on mma.sync, whose operands a warp
+// What bounds it: the bytes of the cache, read once, over F32 and F16 pools (77 to 100 % of the memory's measured 6.54 TB/s
+// for long sequences; F32 with heads of 256 or many columns, whose products are three to one, 41 to 78). Over Q8_0 (30 to 54 %) and F8 (41 to
+// 75 %) the chain of instructions from a tile's bytes to its products takes longer than the bytes' way (28 and 40 % of the issue
+// slots, with the two to four warps a scheduler that registers allow). The products run on mma.sync, whose operands a warp
 // brings from shared memory into the fragments it needs: with one to eight query heads to a KV head the large tensor-core
 // tiles would be empty but for a few columns, and the narrow ones take 10 to 40 % of the issue rate. The dimension that a
 // product sums over may be taken in any order and a fragment's rows may stand for any dimensions, so a lane reads 16 bytes
@@ -153,7 +153,8 @@ template <int PAIR> __device__ __forceinline__ uint32_t dec_int8(uint32_t x) {
 // ---- layout --------------------------------------------------------------------------------------------------------
 
 // FMT: format of the pools; NT: tiles of eight query heads; WIDE: q, gate and out are f32, and queries and probabilities enter
-// the products as two parts (22 bits); otherwise f16 or bf16 and one part (11 bits, no less than such an output can tell).
+// the products as two parts (22 bits); otherwise f16 or bf16 and one part (11 bits: as much as an f16 output has, and with its
+// rounding an error of the square root of two of one).
 template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     static constexpr bool IS_F32 = FMT == YUUKA_KV_F32, IS_Q8 = FMT == YUUKA_KV_Q8_0, IS_F8 = FMT == YUUKA_KV_F8;
     // Warps of a CTA and CTAs of an SM: twelve warps an SM, or eight where the sums, queries and copies of 256 dimensions take the

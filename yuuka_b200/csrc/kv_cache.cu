@@ -251,8 +251,9 @@ __global__ void __launch_bounds__(MOVE_WARPS * 32) kv_write_kernel(const MovePar
     uint8_t * row = (u.is_v ? p.cache.v : p.cache.k) + (int64_t)slot * p.cache.row_bytes;
 
     // Scales: every division is made once, by one lane, for all chunks at a time, and handed to the lanes that need it.
-    // (amax / 127 and amax / 448 by their inverses: within an ulp of the quotient. Of Q8_0's scales, f16 in the end, about one in
-    // 16,000 is the neighbour of the one that a session's rows would have.)
+    // (amax / 127 and amax / 448 by their inverses: within an ulp of the quotient. Q8_0's scales, f16 in the end, are the quotient's all the
+    // same: 127 f32(1 / 127) is 1 - 2^-28, and no f32 lies near enough below 127 times a border of f16's rounding. Whole numbers differ
+    // by one from those of a session where a value's quotient is a half, or within an f32 step of one.)
     float scale[MOVE_CHUNKS], inv[MOVE_CHUNKS];
     uint32_t half_scale = 0;  // Q8_0: of block lane (eight of a chunk)
     if constexpr (FMT == YUUKA_KV_Q8_0 || FMT == YUUKA_KV_F8) {

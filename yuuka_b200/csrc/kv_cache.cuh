@@ -22,7 +22,7 @@ constexpr int KV_BAD_BLOCK = YUUKA_KV_STATUS_BLOCK, KV_BAD_SEQUENCE = YUUKA_KV_S
 
 // Bytes of one row, 0 for a format or shape without a form.
 uint64_t kv_row_bytes(int32_t format, int32_t kv_heads, int32_t head_dim);
-// Checks the geometry (geometry_only: nothing that needs the buffers) and gives the kernels' form of it; throws.
+// Checks numbers, ranges and overlaps of a cache and gives the kernels' form of it; throws. The second: the numbers alone.
 PagedCache check_cache(const char * op, const yuuka_kv_cache * cache, const yuuka_device * dev);
 void check_geometry(const char * op, const yuuka_kv_cache * cache);
 
