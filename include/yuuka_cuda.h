@@ -117,7 +117,8 @@ YUUKA_API yuuka_status yuuka_event_record(yuuka_stream * stream, yuuka_event * e
 YUUKA_API yuuka_status yuuka_event_wait(yuuka_event * event);
 YUUKA_API yuuka_status yuuka_event_elapsed_ms(yuuka_event * start, yuuka_event * end, float * ms);
 
-/* yuuka_hip.h:74-79 (+ an offset form for uploads) */
+/* yuuka_hip.h:74-79 (+ an offset form for uploads). Synchronous: what has been written is there for later calls on any
+ * stream, and what earlier calls on other streams have left is read once those are synchronized. */
 YUUKA_API yuuka_status yuuka_memcpy_h2d(yuuka_buffer * dst, const void * src, uint64_t bytes);
 YUUKA_API yuuka_status yuuka_memcpy_h2d_at(yuuka_buffer * dst, uint64_t offset, const void * src, uint64_t bytes);
 YUUKA_API yuuka_status yuuka_memcpy_d2h(void * dst, const yuuka_buffer * src, uint64_t bytes);

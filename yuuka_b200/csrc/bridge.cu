@@ -266,6 +266,7 @@ yuuka_status yuuka_memcpy_h2d_at(yuuka_buffer * dst, uint64_t offset, const void
         if (bytes == 0) return;
         set_device(dst->dev);
         YK_CUDA(cudaMemcpy((char *)dst->ptr + offset, src, bytes, cudaMemcpyHostToDevice));
+        settle_default_stream();
     });
 }
 

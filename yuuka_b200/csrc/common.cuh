@@ -174,6 +174,9 @@ inline void check_start(const char * op, const char * what, const yuuka_buffer *
     YK_REQUIRE(((uint64_t)(uintptr_t)buf->ptr + offset) % align == 0, YUUKA_ERR_INVALID_ARGUMENT, "%s: %s does not start at a multiple of %llu bytes",
                op, what, (unsigned long long)align);
 }
+// Waits for the default stream: a copy from pageable host memory returns before its last part is on the device, a clearing at
+// once, and the streams that calls run on do not wait for the default one.
+inline void settle_default_stream() { YK_CUDA(cudaStreamSynchronize(nullptr)); }
 inline void record_completion(yuuka_stream * stream, yuuka_event * completion) {
     if (completion) YK_CUDA(cudaEventRecord(completion->e, stream->s));
 }

@@ -471,6 +471,7 @@ yuuka_status yuuka_model_finalize(yuuka_model * m) {
             head.tiled = true;
             m->output = head;
         }
+        settle_default_stream();  // (weights as they were loaded and fused)
         m->finalized = true;
     });
 }
@@ -1550,6 +1551,7 @@ yuuka_status yuuka_session_create(yuuka_model * model, const yuuka_session_confi
                                          &L.ffn_down, &L.proj, &L.qk, &L.gate_up, &L.sh_gate, &L.sh_up, &L.sh_down, &L.sh_gate_up})
                     reserve_gemm(s, *t, R);
             reserve_gemm(s, model->output, R);
+            settle_default_stream();  // (what was cleared and copied above)
         } catch (...) {
             yuuka_session_destroy(s);
             throw;
@@ -1585,6 +1587,7 @@ yuuka_status yuuka_session_set_block_table(yuuka_session * s, int32_t seq, const
         YK_CUDA(cudaStreamSynchronize(s->stream.s));
         YK_CUDA(cudaMemcpy(s->d_tables + (int64_t)seq * s->table_stride, blocks, sizeof(int32_t) * s->table_stride,
                            cudaMemcpyHostToDevice));
+        settle_default_stream();
     });
 }
 
@@ -1648,6 +1651,7 @@ yuuka_status yuuka_session_set_position(yuuka_session * s, int32_t seq, int32_t 
         set_device(s->model->dev);
         YK_CUDA(cudaStreamSynchronize(s->stream.s));
         YK_CUDA(cudaMemcpy(s->d_pos0 + seq, &position, sizeof(int32_t), cudaMemcpyHostToDevice));
+        settle_default_stream();
         s->h_pos[seq] = s->h_pos_upper[seq] = position;
     });
 }
@@ -1713,6 +1717,7 @@ yuuka_status yuuka_session_restore(yuuka_session * s, int32_t seq, const void * 
             YK_CUDA(cudaMemcpy(s->layers[i].state + (int64_t)seq * s->s_count, o, s->s_count * 4, cudaMemcpyHostToDevice));
             o += s->s_count * 4;
         }
+        settle_default_stream();
     });
 }
 

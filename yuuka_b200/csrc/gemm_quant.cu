@@ -27,6 +27,7 @@ void clear_device_error(const yuuka_device * dev) {
     const int zero = 0;
     cudaMemcpyToSymbol(g_device_error, &zero, sizeof(int));
     clear_gemm_wait_expired();
+    settle_default_stream();
 }
 
 // The same two flags copied behind the work already queued on `stream`, into two page-locked words.
@@ -174,6 +175,7 @@ void gemm_scratch_reserve(const yuuka_device * dev, GemmScratch & s, uint32_t w_
         cudaError_t err = cudaMalloc(&s.counters, (size_t)tiles * sizeof(int));
         YK_REQUIRE(err == cudaSuccess, YUUKA_ERR_ALLOCATION, "gemm counter allocation failed");
         YK_CUDA(cudaMemset(s.counters, 0, (size_t)tiles * sizeof(int)));
+        settle_default_stream();
         s.counter_count = tiles;
     }
 }
