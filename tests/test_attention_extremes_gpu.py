@@ -72,6 +72,40 @@ def test_infinite_keys_weigh_nothing(dev, stream, scratch, fmt, dtype, exact, di
     step.free()
 
 
+@pytest.mark.parametrize("fmt", ["f16", "f32", "q8_0", "f8"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_infinite_queries(dev, stream, scratch, fmt, dtype, dim):  # noqa: F811
+    """A query of -infinity where all keys are positive scores -infinity alone: a row without keys. One of infinity, or with a NaN, is
+    a NaN. The other heads of the tile do not notice."""
+    lens = [20, 33, 700, 3000]
+    step = Step(dev, stream, dim, fmt, dtype, 1, 4, dim, 16, lens)
+    rng = np.random.default_rng(dim)
+    for s, n in enumerate(lens):
+        k = rng.standard_normal((n, 1, dim))
+        k[..., 7] = np.abs(k[..., 7]) + 0.5
+        bufs = [dev.upload(np.ascontiguousarray(a, t)) for a, t in ((k, np.float32), (rng.standard_normal((n, 1, dim)), np.float32), (np.arange(n), np.int32), (np.full(n, s), np.int32))]
+        cuda.kv_write(stream, step.paged.cache, cuda.KvRows(bufs[0], bufs[1], bufs[2], n, seq=bufs[3]))
+        stream.synchronize()
+        for b in bufs:
+            b.free()
+    step.paged.k, step.paged.v = step.paged.download()
+    q = from_dtype(step.qg, dtype)
+    good = to_dtype(q.astype(np.float32), dtype)
+    q[:, 0, 7], q[:, 1, 7], q[:, 2, 9] = -np.inf, np.inf, np.nan
+    step.qb.write(to_dtype(q.astype(np.float32), dtype))
+    out, lse = step.run(scratch)
+    assert np.all(out[:, 0] == 0) and np.all(np.isneginf(lse[:, 0]))
+    assert np.all(np.isnan(out[:, 1:3]))
+    step.qg = good
+    bad_out, bad_lse = out.copy(), lse.copy()
+    step.qb.write(good)
+    out, lse = step.run(scratch)
+    assert np.array_equal(out[:, 3], bad_out[:, 3]) and np.array_equal(lse[:, 3], bad_lse[:, 3])
+    step.check(out, lse)
+    step.free()
+
+
 @pytest.mark.parametrize("fmt,dtype", [("f16", "f32"), ("f16", "bf16"), ("f32", "f32"), ("f32", "f16"), ("q8_0", "f32"), ("q8_0", "bf16")])
 @pytest.mark.parametrize("dim", [64, 256])
 def test_values_that_are_not_finite_stay_in_their_place(dev, stream, scratch, fmt, dtype, dim):  # noqa: F811

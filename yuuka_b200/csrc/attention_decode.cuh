@@ -604,7 +604,8 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                     const int e = min(max((int)(__float_as_uint(amax) >> 23), 15), 254);
                     if constexpr (FMT == YUUKA_KV_F16) {
                         // no first part is zero but of a zero: its sign decides over an infinite key. 2^-24 in its units, 2^-38 of the largest
-                        const float low = e > 38 ? __int_as_float((e - 38) << 23) : 0.0f;
+                        // (beside an infinite query nothing else counts)
+                        const float low = e > 38 && e < 254 ? __int_as_float((e - 38) << 23) : 0.0f;
                         if (least < low)
 #pragma unroll
                             for (int i = 0; i < 2 * QM; i++) {
@@ -628,7 +629,9 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                             x.y *= up;
                             hi[half] = dec_pack(x.x, x.y);
                             const float2 r = dec_unpack(hi[half]);
-                            lo[half] = dec_pack(x.x - r.x, x.y - r.y);
+                            if constexpr (S::IS_Q8 || S::IS_F8)  // (of an infinite query not NaN: its first part is to decide)
+                                lo[half] = dec_pack(fmaxf(x.x - r.x, -65504.0f), fmaxf(x.y - r.y, -65504.0f));
+                            else lo[half] = dec_pack(x.x - r.x, x.y - r.y);
                         }
                         if constexpr (S::Q_SHARED) {
                             if constexpr (WIDE) dec_sts4(q_at + 512 * (nt * QM + i), make_uint4(hi[0], hi[1], lo[0], lo[1]));
