@@ -72,6 +72,21 @@ def test_infinite_keys_weigh_nothing(dev, stream, scratch, fmt, dtype, exact, di
     step.free()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("size", [1e30, 1e35, 1e-30])
+def test_large_and_small_values_over_f32_pools(dev, stream, scratch, dtype, dim, size):  # noqa: F811
+    """Sums of values near the ends of f32, over rows that are whole, shared by few runs and by many."""
+    step = Step(dev, stream, dim, "f32", dtype, 1, 3, dim, 16, [20, 300, 3000])
+    for s, n in enumerate(step.lens):
+        at = step.paged.slots(s, np.arange(n))
+        pool = step.paged.v.view(np.float32)
+        pool[at] = np.clip(pool[at], -4, 4) * np.float32(size)
+    step.paged.upload()
+    step.check(*step.run(scratch))
+    step.free()
+
+
 @pytest.mark.parametrize("fmt", ["f16", "f32", "q8_0", "f8"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("dim", [64, 128, 256])

@@ -3,7 +3,7 @@
 // Mathematics. A unit is one KV head of one row of the batch, with up to 8 NT of the query heads that share it as columns.
 // Its keys are taken 16 or 32 at a time: S^T = K Q^T (keys as the rows of the product, heads as its 8-wide columns), running
 // maximum m and sum l per head, O^T += V^T P^T. Scores live in the base-2 domain, s = (scale log2 e) q.k, and probabilities
-// carry a factor of 2^11, p = 2^(s - m + 11). m is the maximum when the sums were last rescaled, which they are only when a score
+// carry a factor of 2^11 (over F32 pools none), p = 2^(s - m + 11). m is the maximum when the sums were last rescaled, which they are only when a score
 // passes it by 2^4 (in the first tiles, mostly), so the largest p is 2^15, those down to 2^-25 of 2^m stay normal in f16, and
 // what is rounded away is below 2^-36 of it. (A slack of 2^8 with a factor of 2^7 took as long.)
 //
@@ -63,7 +63,6 @@ constexpr size_t DEC_PARTIAL_BYTES = 40u << 20;  // two of the 1184 warps with t
 enum { DEC_SHORT, DEC_LONG, DEC_FAR, DEC_DONE, DEC_COUNTERS };
 constexpr int DEC_SHORT_MOST = 32;      // partials that a warp joins
 constexpr int DEC_FAR_MOST = 16384;     // runs to do again: of each warp one, or of each unit where those are more (65536 / 8 + 1024 at most)
-constexpr float DEC_P_LOG2 = 11.0f;      // log2 of the factor that probabilities carry
 constexpr float DEC_LOWEST = -3.0e38f;  // of running maxima: finite, so that a score of -infinity weighs nothing even in a run without others
 constexpr float DEC_SLACK = 4.0f;       // log2 of what a score may pass the running maximum by before sums are rescaled
 constexpr int DEC_SMEM_SM = 233472;     // shared memory of an SM
@@ -172,6 +171,8 @@ template <int FMT, int HD, int NT, bool WIDE> struct DecodeShape {
     // beat twelve of one: 24 of 8000 with 8 KV heads 124 instead of 142 us (F16), 101 instead of 127 (F8), 142 instead of 156 (Q8_0).
     static constexpr int HALVES = HD == 256 || (HD == 128 && (IS_F32 || (WIDE && NT == 2))) ? 1 : 2, KEYS = 16 * HALVES;
     static constexpr int COLS = 8 * NT, PARTS = WIDE ? 2 : 1;
+    // log2 of the factor that probabilities carry into f16 (tf32 has the exponents of f32, and sums of large values room without one)
+    static constexpr float P_LOG2 = IS_F32 ? 0.0f : 11.0f;
     // Q8_0, F8: ratio (log2) of the scales of V from which on a row is done again, in f32. Probabilities of 2^11 for the heaviest key enter
     // the products in units of the largest scale, rounded to half of f16's 2^-24: at this ratio a key of the smallest scale that has all
     // the weight is held to 2^-36 * 2 * 2^10 = 2^-25 (f32 queries), or 2^-21, of itself.
@@ -400,8 +401,7 @@ template <bool WIDE, int N> __device__ __forceinline__ void dec_write(const Deco
         for (int i = 0; i < N / 2; i += 4) *reinterpret_cast<uint4 *>(dst + 2 * i) = make_uint4(raw[i], raw[i + 1], raw[i + 2], raw[i + 3]);
 }
 __device__ __forceinline__ void dec_write_lse(const DecodeParams & p, int b, int head, float m, float l) {
-    // (l carries the probabilities' factor)
-    if (p.lse) p.lse[(int64_t)b * p.heads + head] = l == 0.0f ? -INFINITY : (m - DEC_P_LOG2 + log2f(l)) * 0.693147180559945309f;
+    if (p.lse) p.lse[(int64_t)b * p.heads + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
 }
 // query heads of unit u of a row
 struct DecodeHeads {
@@ -951,7 +951,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
-                        const float base = DEC_P_LOG2 - m[nt][c];
+                        const float base = S::P_LOG2 - m[nt][c];
 #pragma unroll
                         for (int h = 0; h < HALVES; h++) {
                             sh[h][nt][c] = dec_exp2(fmaf(sh[h][nt][c], scale[nt][c], base));
@@ -1201,7 +1201,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                                 }
                                 dec_write<WIDE, RUN>(p, use.b, h.first + col, S::out_dim(c, j0, g), x);
                             }
-                            if (g == 0) dec_write_lse(p, use.b, h.first + col, m[nt][e], l[nt][e]);
+                            if (g == 0) dec_write_lse(p, use.b, h.first + col, m[nt][e] - S::P_LOG2, l[nt][e]);
                         }
                     again |= far;
                 } else {
@@ -1220,7 +1220,7 @@ __global__ void __launch_bounds__(DecodeShape<FMT, HD, NT, WIDE>::W * 32, Decode
                                     *reinterpret_cast<float2 *>(part + col * HD + S::out_dim(c, j, g)) =
                                         make_float2(o[nt][c][j][e] * v_scale, o[nt][c][j][e + 2] * v_scale);
                             if (g == 0) {
-                                part[COLS * HD + col] = m[nt][e];
+                                part[COLS * HD + col] = m[nt][e] - S::P_LOG2;  // what 1 in l stands for, as the exponentials had it
                                 part[COLS * HD + COLS + col] = far ? __uint_as_float(__float_as_uint(l[nt][e]) | 0x80000000u) : l[nt][e];
                             }
                         }
@@ -1381,7 +1381,7 @@ template <int HD, bool WIDE> __device__ __forceinline__ void decode_column_write
 #pragma unroll
     for (int i = 0; i < DIMS; i++) o[i] = l == 0.0f ? 0.0f : o[i] / l * (p.gate ? f[i] : 1.0f);
     dec_write<WIDE, DIMS>(p, b, head, dim, o);
-    if (lane == 0) dec_write_lse(p, b, head, m + DEC_P_LOG2, l);
+    if (lane == 0) dec_write_lse(p, b, head, m, l);
 }
 // DEC_AT_ONCE heads of a row that several teams share, by all warps of a CTA: each takes some of the keys. `store`: shared memory.
 template <int HD> constexpr int DEC_STORE = 8 * DEC_AT_ONCE<HD> * (HD + 2);  // floats
